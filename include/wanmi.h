@@ -353,6 +353,78 @@ int wanmi_dmajor_to_mx(const void* x, int64_t B, int heads, int64_t S, int64_t b
                        int64_t d_stride, void* codes, uint8_t* scales, void* stream);
 
 /*
+ * Norms before and after a sub-layer, fused with its gate and residual scale, for packed batches: rows of
+ * several requests in one tensor, modulation per request.
+ *   p = Norm_post(hidden) * post_weight                              (fp32; post_weight may be NULL)
+ *   residual_out = bf16(residual_scale * residual + gate[q] * p)     (gate may be NULL)
+ *   out = Q(bf16(Norm_pre(residual_out) * mul[q] + add[q]))          (mul / add may be NULL)
+ * hidden, residual: bf16 [T, H], rows ld_* elements apart (multiples of 8); residual_out bf16 [T, H]; post_weight
+ * fp32 [H]; gate, mul, add fp32: one row of H per request, ld_* elements apart (multiples of 4), or ld_* 0: one
+ * row for every request; out and scales as wanmi_adaln_quant's. q = request_ids[t] (int32; NULL: every row is request 0). A row whose id is not in
+ * [0, requests) is not read; its outputs are left as they are, or zeroed with zero_rest. residual_out may
+ * be `residual`, out `hidden`, row for row. H as for wanmi_adaln_quant. Both norms use eps.
+ * Stands beside wanmi_adaln_quant (one request, no norm before the gate); no reference counterpart.
+ */
+int wanmi_adaln_sandwich(const void* hidden, int64_t ld_hidden, const void* residual, int64_t ld_residual,
+                         const float* post_weight, const float* gate, int64_t ld_gate, const float* mul,
+                         int64_t ld_mul, const float* add, int64_t ld_add, const int32_t* request_ids,
+                         int64_t requests, float residual_scale, int64_t T, int64_t H, float eps, int post_norm,
+                         int norm_type, int quant_type, int zero_rest, void* residual_out, void* out, uint8_t* scales,
+                         void* stream);
+
+/* Norm of wanmi_qk_norm_rope_axes. */
+#define WANMI_QKNORM_NONE 0
+#define WANMI_QKNORM_PER_HEAD 1     /* RMSNorm over each head's head_dim channels, weight [head_dim] */
+#define WANMI_QKNORM_ACROSS_HEADS 2 /* RMSNorm over all heads of a row, weight [heads * head_dim] */
+
+/*
+ * Q/K norm and rotary positions on several axes (time, height, width, ...), given per token, for packed batches:
+ *   x^ = Norm(x) * gamma;  pair i of a head: (a, b) -> bf16(a cos t - b sin t), bf16(a sin t + b cos t),
+ *   t = positions[token][axis of i] * freqs[i]                        (angles in fp64, the rest in fp32)
+ * q, k, q_out, k_out: bf16, element (t, h, d) at t * token_stride + h * head_stride + d (strides multiples of 8);
+ * k_heads may be 0 (no k); the outputs may be the inputs. positions: int32 or (positions_float) fp32 [T, axes].
+ * axis_dims [axes] and freqs [sum(axis_dims) / 2] are HOST arrays: the axes' channels, which fill the head
+ * from its first one on (even, their sum a multiple of 16, at most head_dim; channels behind it are not turned), and the
+ * angle per unit of position of every pair. rope_pairs: WANMI_ROTATE_* over those channels.
+ * gamma: fp32 [heads * head_dim] or [head_dim] as `norm` says, or NULL (ones).
+ * head_dim 32, 64, 128 or 256, heads * head_dim at most 16384. request_ids, requests, zero_rest as in
+ * wanmi_adaln_sandwich. k_maxnorm (optional, fp32 [requests, k_heads]): a bound on ||k_out|| of each request's
+ * rows: the largest norm before the rounding, times 1 + 2^-8 (0 where a request has no rows). NaN where a row is NaN.
+ * Stands beside wanmi_qk_rmsnorm_rope (one sequence, tables of one grid); no reference counterpart.
+ */
+int wanmi_qk_norm_rope_axes(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads, const float* q_gamma,
+                            void* q_out, int64_t q_out_token_stride, int64_t q_out_head_stride, const void* k,
+                            int64_t k_token_stride, int64_t k_head_stride, int k_heads, const float* k_gamma, void* k_out,
+                            int64_t k_out_token_stride, int64_t k_out_head_stride, int64_t T, int head_dim,
+                            const void* positions, int positions_float, int axes, const int* axis_dims, const double* freqs,
+                            int rope_pairs, int norm, float eps, const int32_t* request_ids, int64_t requests, int zero_rest,
+                            float* k_maxnorm, void* stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection:
+ *   out[t, n] = bf16(base[t, n] + sum_j B[e][n, j] u[t, p(n) rank + j]),
+ *   u[t, i] = adapter_scales[e] * row_scale[t] * sum_k A[e][i, k] x[t, k]           (fp32)
+ * x: bf16 [T, K], rows ldx elements apart, or with x_scales (e8m0 [T, K/32]) e4m3fn codes, rows ldx bytes apart
+ * (16-byte aligned rows); row_scale fp32 [T] or NULL. A: bf16 [adapters, parts * rank, K]; B: bf16
+ * [adapters, N, rank]; the columns of a fused projection fall into `parts` runs of part_widths (HOST array; multiples
+ * of 64 unless there is one), p(n) is the run of column n. adapter_scales fp32 [adapters] or NULL.
+ * e = adapter_ids[q], q = request_ids[t] (NULL: q = t, an id per row). e outside [0, adapters): the row keeps its base.
+ * q outside [0, requests): the row is not computed, its output left as it is or zeroed with zero_rest. base and
+ * out: bf16 [T, N], rows ldb / ldo elements apart; out may be base, row for row. rank a multiple of 16, at most
+ * 1024 (shorter adapters are padded with zeros); K a multiple of 32, N of 8. `workspace`: device
+ * memory of wanmi_lora_workspace bytes, for this call alone (two launches on `stream` use it).
+ * Stands beside wanmi_mxfp8_gemm, whose activation and output it takes; no reference counterpart.
+ */
+int wanmi_lora_add(const void* x, const uint8_t* x_scales, const float* row_scale, int64_t ldx, const void* A, const void* B,
+                   const float* adapter_scales, const int32_t* adapter_ids, const int32_t* request_ids, int64_t requests,
+                   int64_t adapters, int64_t T, int64_t K, int64_t N, int rank, int parts, const int64_t* part_widths,
+                   const void* base, int64_t ldb, void* out, int64_t ldo, int zero_rest, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that wanmi_lora_add needs for these sizes on the current device (0 where there is nothing to compute). */
+int64_t wanmi_lora_workspace(int64_t T, int64_t K, int parts, int rank);
+
+/*
  * Streaming device-to-device copy of `bytes` (a multiple of 16; src and dst 16-byte aligned, not
  * overlapping) on `stream`: 16-byte loads, eight per thread in flight before its non-temporal
  * stores, one 32 KiB chunk per workgroup. Measurement infrastructure with no counterpart in the

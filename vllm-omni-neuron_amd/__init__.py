@@ -10,7 +10,7 @@ The directory name contains dashes, so it is imported under the module name
 """
 
 from . import _lib  # noqa: F401
-from .adaln_kernels import AdaLNQuantKernelArgs, adaln_modulate, adaln_quant_kernel  # noqa: F401
+from .adaln_kernels import AdaLNQuantKernelArgs, adaln_modulate, adaln_quant_kernel, adaln_sandwich  # noqa: F401
 from .common_types import DtypeMode, MXTensor, NormType, QKNormConfig, QKVOutputLayout, QuantizationType  # noqa: F401
 from .row_mx_kernels import (  # noqa: F401
     MXWeight,
@@ -22,11 +22,13 @@ from .row_mx_kernels import (  # noqa: F401
     row_mx_mlp,
     row_quantize_packed,
 )
+from .lora import lora_add, stack_adapters  # noqa: F401
 from . import rope  # noqa: F401
 from .rope import WanRotaryPosEmbed, rope_tables  # noqa: F401
 from . import attention_ops  # noqa: F401
 from .attention_ops import (  # noqa: F401
     _nki_attend,
+    qk_norm_rope_axes,
     ring_attention_const_max_fwd,
     row_mx_o_proj,
     row_mx_qkv_proj,

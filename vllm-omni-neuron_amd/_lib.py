@@ -70,6 +70,13 @@ _SIGNATURES = {
         _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _f32, _i32,
         _vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _f32, _vp,
     ],
+    "wanmi_adaln_sandwich": [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _f32, _i64, _i64, _f32,
+                             _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp],
+    "wanmi_qk_norm_rope_axes": [_vp, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i64, _i64,
+                                _i64, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _i32, _f32, _vp, _i64, _i32, _vp, _vp],
+    "wanmi_lora_add": [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _vp, _vp, _i64,
+                       _vp, _i64, _i32, _vp, _i64, _vp],
+    "wanmi_lora_workspace": [_i64, _i64, _i32, _i32],
 }
 
 _LIB = None
@@ -95,6 +102,7 @@ def load() -> ctypes.CDLL:
         fn.argtypes = argtypes
         fn.restype = _i32
     lib.wanmi_last_error.restype = ctypes.c_char_p
+    lib.wanmi_lora_workspace.restype = _i64
     _LIB = lib
     return lib
 
@@ -158,6 +166,56 @@ def stream_of(t: torch.Tensor) -> int:
     """The current HIP stream of ``t``'s device, as the void* the C ABI takes (the handle that
     ``torch.cuda.current_stream(t.device).cuda_stream`` holds, without the stream object: 0.2 against 2.5 us)."""
     return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def call(name: str, t: torch.Tensor, *args) -> None:
+    """Calls one entry point on ``t``'s device and its current stream (the last argument), whichever device is
+    current, and raises on its status."""
+    fn = getattr(load(), name)
+    index = t.get_device()
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, stream_of(t))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, stream_of(t))
+    check(status, name)
+
+
+def refuse_overlap(out: torch.Tensor, what: str, *inputs: torch.Tensor | None) -> None:
+    """An output may be an input, element for element, or share no byte with it: anything between would be read after
+    it is written. Views of one buffer whose rows are equally far apart are told apart by their columns."""
+    for t in inputs:
+        if t is None or not t.numel() or not out.numel():
+            continue
+        size, tsize = out.element_size(), t.element_size()
+        a0, b0 = out.data_ptr(), t.data_ptr()
+        if a0 == b0 and size == tsize and out.shape == t.shape and out.stride() == t.stride():
+            continue
+        a1 = a0 + size * (1 + sum((n - 1) * s for n, s in zip(out.shape, out.stride())))
+        b1 = b0 + tsize * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+        if a1 <= b0 or b1 <= a0:
+            continue
+        if out.dim() > 1 and t.dim() > 1 and out.stride(0) * size == t.stride(0) * tsize:
+            pitch = out.stride(0) * size
+            wa = size * (1 + sum((n - 1) * s for n, s in zip(out.shape[1:], out.stride()[1:])))
+            wb = tsize * (1 + sum((n - 1) * s for n, s in zip(t.shape[1:], t.stride()[1:])))
+            gap = (b0 - a0) % pitch if pitch else 0
+            if wa <= gap and gap + wb <= pitch:
+                continue
+        raise ValueError(f"{what} overlaps an input that it is not")
+
+
+def refuse_input(out: torch.Tensor, what: str, *inputs: torch.Tensor | None) -> None:
+    """An output that shares memory with an input which other rows still read, even element for element."""
+    for t in inputs:
+        if t is not None and t.numel() and out.numel() and t.data_ptr() == out.data_ptr():
+            raise ValueError(f"{what} may not be that input")
+    refuse_overlap(out, what, *inputs)
+
+
+def request_rows(request_ids: torch.Tensor | None, rows: int) -> None:
+    """Checks ``request_ids``: int32 ``[rows]``, contiguous, or None."""
+    expect(request_ids, "request_ids", dtype=torch.int32, shape=(rows,), optional=True)
 
 
 def expect(t: torch.Tensor | None, what: str, *, dtype: torch.dtype, shape: tuple | None = None,

@@ -179,6 +179,135 @@ def adaln_modulate(
     return _stack(res_outs, lambda p: p.shape[-1]), out
 
 
+def _request_vector(vec: torch.Tensor | None, name: str, H: int, requests: int | None):
+    """fp32 ``[H]`` (or ``[1, H]``: for every request) or ``[R, H]`` (one row per request) -> (elements between
+    requests, requests so far)."""
+    if vec is None:
+        return 0, requests
+    _lib.expect(vec, name, dtype=torch.float32, contiguous=False, row_contiguous=True)
+    if vec.dim() not in (1, 2) or vec.shape[-1] != H:
+        raise ValueError(f"{name} must be [{H}] or [requests, {H}], got {list(vec.shape)}")
+    if vec.data_ptr() % 16:
+        raise ValueError(f"{name} must be 16-byte aligned")
+    if vec.dim() == 1 or vec.shape[0] == 1:
+        return 0, requests
+    if requests is not None and vec.shape[0] != requests:
+        raise ValueError(f"{name} has {vec.shape[0]} rows, the other vectors {requests}")
+    if vec.stride(0) < H or vec.stride(0) % 4:
+        raise ValueError(f"{name} rows must lie a multiple of 4 elements of at least {H} apart")
+    return vec.stride(0), vec.shape[0]
+
+
+def _row_stride(t: torch.Tensor, name: str, T: int, H: int) -> int:
+    _lib.expect(t, name, dtype=torch.bfloat16, shape=(T, H), contiguous=False, row_contiguous=True)
+    ld = t.stride(0) if T > 1 else H
+    if ld < H or ld % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{name} rows must be 16-byte aligned and not overlap")
+    return ld
+
+
+def adaln_sandwich(
+    hidden: torch.Tensor,
+    residual: torch.Tensor,
+    mul: torch.Tensor | None = None,
+    add: torch.Tensor | None = None,
+    *,
+    eps: float,
+    post_norm: str = "rms_norm",
+    post_weight: torch.Tensor | None = None,
+    gate: torch.Tensor | None = None,
+    residual_scale: float = 1.0,
+    norm_type: str = "layer_norm",
+    quant: str = "none",
+    request_ids: torch.Tensor | None = None,
+    residual_out: torch.Tensor | None = None,
+    out=None,
+):
+    """The norms around a sub-layer's residual sum, with the gate and the modulation of each row's request::
+
+        r = bf16(residual_scale * residual + gate[q] * (Norm_post(hidden) * post_weight))
+        y = Quantize(bf16(Norm_pre(r) * mul[q] + add[q]))
+
+    in one pass over a packed batch; returns ``(r, y)`` as :func:`adaln_modulate` does with a residual.
+
+    ``hidden`` (the sub-layer's output) and ``residual``: bf16 ``[T, H]``, any row stride; ``post_weight`` fp32
+    ``[H]``; ``gate`` / ``mul`` / ``add`` fp32 ``[H]`` for every request, or ``[R, H]``, one row per request (rows
+    may be strided: a slice ``mod[:, i]`` of a ``[R, 6, H]`` modulation is taken as it is). ``post_norm`` and
+    ``norm_type`` are ``"layer_norm"``, ``"rms_norm"`` or ``"none"``, both with ``eps``. ``quant`` as in
+    :func:`adaln_modulate`.
+
+    ``request_ids`` int32 ``[T]`` names each row's request q (None: every row is request 0). A row whose id is
+    negative, or at least R, belongs to none: it is not read, and its rows of ``residual_out`` and ``out`` are left
+    as they are where the caller gave them, zeros where they are allocated here. ``residual_out`` may be
+    ``residual`` and ``out`` (contiguous; an :class:`MXTensor` for ``quant="mx"``) may be ``hidden``.
+    """
+    if post_norm not in _SUPPORTED_NORMS:
+        raise ValueError(f"unsupported post_norm {post_norm!r}")
+    _lib.expect(hidden, "hidden", dtype=torch.bfloat16, shape=(None, None), contiguous=False)
+    _validate(hidden, norm_type, quant, True)
+    T, H = hidden.shape
+    if H == 0:
+        raise ValueError("hidden size 0")
+    ld_h = _row_stride(hidden, "hidden", T, H)
+    ld_r = _row_stride(residual, "residual", T, H)
+    _lib.expect(post_weight, "post_weight", dtype=torch.float32, shape=(H,), optional=True)
+    if post_weight is not None and post_weight.data_ptr() % 16:
+        raise ValueError("post_weight must be 16-byte aligned")
+    requests = None
+    ld_gate, requests = _request_vector(gate, "gate", H, requests)
+    ld_mul, requests = _request_vector(mul, "mul", H, requests)
+    ld_add, requests = _request_vector(add, "add", H, requests)
+    _lib.request_rows(request_ids, T)
+    if request_ids is None and requests is not None:
+        raise ValueError("vectors of several requests need request_ids")
+    if not eps >= 0:
+        raise ValueError(f"eps must be non-negative, got {eps}")
+    codes, scales = (out.codes, out.scales) if isinstance(out, MXTensor) else (out, None)
+    if out is not None:
+        if isinstance(out, MXTensor) != (quant == "mx"):
+            raise ValueError("out must be an MXTensor for quant='mx' and a tensor otherwise")
+        _lib.expect(codes, "out", dtype=torch.bfloat16 if quant == "none" else torch.float8_e4m3fn,
+                    shape=(T, H + 4 if quant == "row" else H))
+        _lib.expect(scales, "out.scales", dtype=torch.uint8, shape=(T, H // 32), optional=quant != "mx")
+        if codes.data_ptr() % 16:
+            raise ValueError("out must be 16-byte aligned")
+        _lib.refuse_overlap(codes, "out", hidden, residual)
+    if residual_out is not None:
+        _lib.expect(residual_out, "residual_out", dtype=torch.bfloat16, shape=(T, H))
+        if residual_out.data_ptr() % 16:
+            raise ValueError("residual_out must be 16-byte aligned")
+        _lib.refuse_overlap(residual_out, "residual_out", hidden, residual)
+        if out is not None and _shares(codes, residual_out):
+            raise ValueError("out and residual_out share memory")
+    _lib.require_gpu(hidden, residual, post_weight, gate, mul, add, request_ids, residual_out, codes, scales,
+                     what="adaln_sandwich")
+    dev = hidden.device
+    # rows of no request are zeros in what is allocated here; with one output given, the other is cleared up front
+    both = (out is None) == (residual_out is None)
+    make = torch.empty if both or request_ids is None else torch.zeros
+    zero_rest = out is None and residual_out is None
+    if residual_out is None:
+        residual_out = make((T, H), dtype=torch.bfloat16, device=dev)
+    if out is None:
+        if quant == "none":
+            codes = make((T, H), dtype=torch.bfloat16, device=dev)
+        else:
+            codes = make((T, H + 4 if quant == "row" else H), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+            scales = make((T, H // 32), dtype=torch.uint8, device=dev) if quant == "mx" else None
+    p = _lib.ptr
+    _lib.call("wanmi_adaln_sandwich", hidden, p(hidden), ld_h, p(residual), ld_r, p(post_weight), p(gate), ld_gate, p(mul), ld_mul,
+              p(add), ld_add, p(request_ids), 2**31 - 1 if requests is None else requests, float(residual_scale), T, H,
+              float(eps), _lib.NORM[post_norm], _lib.NORM[norm_type], _lib.QUANT[quant], int(zero_rest), p(residual_out),
+              p(codes), p(scales))
+    return residual_out, MXTensor(codes, scales) if quant == "mx" else codes
+
+
+def _shares(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors have a byte in common."""
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    return a.numel() > 0 and b.numel() > 0 and a0 < b0 + b.numel() * b.element_size() and b0 < a0 + a.numel() * a.element_size()
+
+
 @dataclass(frozen=True)
 class AdaLNQuantKernelArgs:
     """Configuration of :func:`adaln_quant_kernel` (the reference's dataclass of the same name,

@@ -21,6 +21,8 @@ from __future__ import annotations
 
 from typing import NamedTuple
 
+import ctypes
+import functools
 import math
 
 import torch
@@ -140,6 +142,144 @@ def qk_rmsnorm_rope_to(x: torch.Tensor, out: torch.Tensor, gamma: torch.Tensor, 
     )
     _lib.check(st, "wanmi_qk_rmsnorm_rope_to")
     return out
+
+
+_QK_NORM = {"none": 0, "rms_norm": 1, "rms_norm_across_heads": 2}
+
+
+@functools.lru_cache(maxsize=64)
+def _axis_arrays(axes: tuple, theta: tuple):
+    """The host arrays of ``wanmi_qk_norm_rope_axes``: the axes' widths and every pair's angle per unit of position."""
+    freqs = [t ** (-2 * j / d) for d, t in zip(axes, theta) for j in range(d // 2)]
+    return (ctypes.c_int * len(axes))(*axes), (ctypes.c_double * max(1, len(freqs)))(*freqs)
+
+
+def _heads_view(t: torch.Tensor, name: str, T: int, D: int | None = None):
+    """bf16 ``[T, heads, D]`` with unit d stride and 16-byte aligned heads -> (token stride, head stride, heads)."""
+    _lib.expect(t, name, dtype=torch.bfloat16, shape=(T, None, D), contiguous=False, row_contiguous=True)
+    ts, hs = t.stride(0) if T > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0
+    if ts % 8 or hs % 8 or ts < 0 or hs < 0 or t.data_ptr() % 16:
+        raise ValueError(f"{name} rows and heads must be 16-byte aligned")
+    return ts, hs, t.shape[1]
+
+
+def _separate(t: torch.Tensor, name: str) -> None:
+    """Refuses an output whose own elements overlap (an expanded view)."""
+    sizes = sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1)
+    reach = 1
+    for s, n in sizes:
+        if s < reach:
+            raise ValueError(f"{name} has elements that share memory")
+        reach = s * n
+
+
+def qk_norm_rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, *, axes=(44, 42, 42),
+                      theta=10000.0, rope_pairs: str = "interleaved", norm: str = "none",
+                      q_gamma: torch.Tensor | None = None, k_gamma: torch.Tensor | None = None, eps: float = 1e-6,
+                      request_ids: torch.Tensor | None = None, requests: int | None = None, want_max: bool = False,
+                      q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """Q/K norm and rotary positions on several axes, given per token, for a packed batch of requests; one pass.
+
+    ``q`` ``[T, Hq, D]`` and ``k`` ``[T, Hk, D]`` (or None): bf16 views with unit d stride, such as the column blocks
+    of a fused projection; D 32, 64, 128 or 256. ``positions`` int32 or fp32 ``[T, len(axes)]``: the row's place on
+    every axis (frame, row, column of the latent grid; any others; negative and fractional ones too). ``axes``: the
+    even channel counts that the axes take of each head, in order from its first channel; their sum is a multiple of
+    16, and channels behind it are normalized but not turned. ``theta``: the base of the angles, one or one per axis:
+    pair j of an axis of d channels turns by ``position * theta**(-2j/d)``. ``rope_pairs``: ``"interleaved"`` (channels
+    2i and 2i+1) or ``"halves"`` (i and i + half of the turned channels).
+
+    ``norm``: ``"none"``, ``"rms_norm"`` (each head, weight fp32 ``[D]``) or ``"rms_norm_across_heads"`` (the whole row,
+    weight fp32 ``[heads * D]``); a weight left out is ones. Norm and rotation are fp32, rounded once
+    (:func:`qk_rmsnorm_rope_` rounds between them, as its reference does).
+
+    Returns ``(q_out, k_out)``; ``q_out`` / ``k_out`` may be given, and may be ``q`` and ``k`` themselves. With
+    ``want_max`` also fp32 ``[requests, Hk]``: a bound on the norms of each request's K rows, the ``kmax`` of
+    :func:`attention_core` (``requests`` says how many; 1 without ``request_ids``). ``request_ids`` int32 ``[T]``: rows
+    with a negative id (or one not below ``requests``) belong to no request and are not read; their rows are left as
+    they are in a given output, zeros in one allocated here.
+    """
+    if rope_pairs not in _ROTATE:
+        raise ValueError(f"unknown rope_pairs {rope_pairs!r}")
+    if norm not in _QK_NORM:
+        raise ValueError(f"unknown norm {norm!r}")
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        raise ValueError("q must be bf16 [T, heads, head_dim]")
+    T, D = q.shape[0], q.shape[2]
+    if D not in (32, 64, 128, 256):
+        raise NotImplementedError(f"head_dim {D}: 32, 64, 128 and 256 are served")
+    axes = tuple(int(d) for d in axes)
+    if not 1 <= len(axes) <= 8 or any(d < 0 or d % 2 for d in axes) or sum(axes) > D:
+        raise ValueError(f"axes {axes}: 1 to 8 even channel counts of at most {D} in all")
+    if sum(axes) % 16:
+        raise NotImplementedError(f"axes {axes} turn {sum(axes)} channels: a multiple of 16 is served")
+    theta = tuple(float(t) for t in theta) if isinstance(theta, (tuple, list)) else (float(theta),) * len(axes)
+    if len(theta) != len(axes) or not all(0 < t < math.inf for t in theta):
+        raise ValueError(f"theta must be positive, one or one per axis, got {theta}")
+    if not eps >= 0:
+        raise ValueError(f"eps must be non-negative, got {eps}")
+    views = []
+    for name, x, gamma, out in (("q", q, q_gamma, q_out), ("k", k, k_gamma, k_out)):
+        if x is None:
+            if gamma is not None or out is not None:
+                raise ValueError(f"{name}_gamma and {name}_out need {name}")
+            views.append((0, 0, 0, 0, 0))
+            continue
+        ts, hs, heads = _heads_view(x, name, T, D)
+        if heads < 1 or heads * D > 16384:
+            raise NotImplementedError(f"{name}: {heads} heads of {D}: 1 to {16384 // D} are served")
+        if gamma is not None:
+            if norm == "none":
+                raise ValueError(f"{name}_gamma without a norm")
+            _lib.expect(gamma, f"{name}_gamma", dtype=torch.float32, shape=(D if norm == "rms_norm" else heads * D,))
+        ots = ohs = 0
+        if out is not None:
+            ots, ohs, _ = _heads_view(out, f"{name}_out", T, D)
+            if out.shape != x.shape:
+                raise ValueError(f"{name}_out must be {list(x.shape)}, got {list(out.shape)}")
+            _separate(out, f"{name}_out")
+            _lib.refuse_overlap(out, f"{name}_out", q, k)
+            if name == "k" and q_out is not None:
+                _lib.refuse_overlap(out, "k_out", q_out)
+                if out.data_ptr() == q_out.data_ptr() and out.numel():
+                    raise ValueError("q_out and k_out share memory")
+            if name == "q" and k is not None and out.data_ptr() == k.data_ptr() and out.numel():
+                raise ValueError("q_out may not be k")
+            if name == "k" and out.data_ptr() == q.data_ptr() and out.numel():
+                raise ValueError("k_out may not be q")
+        views.append((ts, hs, heads, ots, ohs))
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.float32):
+        raise ValueError("positions must be an int32 or float32 tensor")
+    _lib.expect(positions, "positions", dtype=positions.dtype, shape=(T, len(axes)))
+    _lib.request_rows(request_ids, T)
+    if want_max and (k is None or (request_ids is not None and requests is None)):
+        raise ValueError("want_max needs k, and with request_ids the number of requests")
+    if requests is not None and not 0 <= requests < 2**31:
+        raise ValueError(f"requests must be in [0, 2^31), got {requests}")
+    if request_ids is None and requests not in (None, 1):
+        raise ValueError("several requests need request_ids")
+    _lib.require_gpu(q, k, positions, q_gamma, k_gamma, request_ids, q_out, k_out, what="qk_norm_rope_axes")
+    dev = q.device
+    n = requests if requests is not None else (2**31 - 1 if request_ids is not None else 1)
+    given = [o is not None for x, o in ((q, q_out), (k, k_out)) if x is not None]
+    # rows of no request are zeros in what is allocated here; with one output given, the other is cleared up front
+    zero_rest = not any(given)
+    make = torch.empty if zero_rest or all(given) or request_ids is None else torch.zeros
+    outs = []
+    for i, (x, out) in enumerate(((q, q_out), (k, k_out))):
+        if x is not None and out is None:
+            out = make(x.shape, dtype=torch.bfloat16, device=dev)
+            views[i] = (*views[i][:3], out.stride(0), out.stride(1))
+        outs.append(out)
+    kmax = torch.empty((n, k.shape[1]), dtype=torch.float32, device=dev) if want_max else None
+    if kmax is not None and n == 0:
+        return (*outs, kmax)
+    p = _lib.ptr
+    dims, freqs = _axis_arrays(axes, theta)
+    (qts, qhs, qh, qots, qohs), (kts, khs, kh, kots, kohs) = views
+    _lib.call("wanmi_qk_norm_rope_axes", q, p(q), qts, qhs, qh, p(q_gamma), p(outs[0]), qots, qohs, p(k), kts, khs, kh, p(k_gamma),
+              p(outs[1]), kots, kohs, T, D, p(positions), int(positions.dtype == torch.float32), len(axes), dims, freqs,
+              _ROTATE[rope_pairs], _QK_NORM[norm], float(eps), p(request_ids), n, int(zero_rest), p(kmax))
+    return (*outs, kmax) if want_max else tuple(outs)
 
 
 def transpose_heads(v: torch.Tensor):

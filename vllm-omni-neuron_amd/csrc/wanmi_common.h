@@ -164,6 +164,14 @@ __device__ __forceinline__ void store_b128_guarded(u32x4 v, __amdgpu_buffer_rsrc
   __builtin_amdgcn_sched_barrier(0);
 }
 
+// The same for a 16-byte store to an address of each lane's own.
+__device__ __forceinline__ void store_b128_guarded(u32x4 v, void* p) {
+  *reinterpret_cast<u32x4*>(p) = v;
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 1" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // Lane index recomputed on the spot (volatile, so not merged with earlier copies): code that runs
 // after a register-heavy loop derives its lane-dependent addresses from this instead of keeping
 // them live (and spilled) across the loop.

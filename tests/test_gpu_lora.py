@@ -63,6 +63,40 @@ def test_against_64_bits(pkg, dev, kind, T, K, slices, n, r):
     _check(pkg, dev, base, x, a, b, scales, slices, adapters, kind=kind)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "mx", "row"])
+@pytest.mark.parametrize("lengths,pad,K,slices,r", [
+    ([1024], 0, 128, (64,), 16), ([700, 500], 7, 256, (136,), 32), ([1, 1023, 1], 0, 384, (256, 64), 32), ([300] * 5, 3, 640, (192,), 48),
+    ([1025], 0, 1152, (128, 64, 64), 64), ([600, 0, 900], 100, 2560, (320,), 128), ([2000], 48, 512, (512,), 96),
+    ([900, 200], 0, 256, (72,), 144), ([1100, 300], 1, 416, (1088,), 80), ([257] * 8, 0, 896, (128,) * 4, 32),
+])
+def test_many_rows(pkg, dev, kind, lengths, pad, K, slices, r):
+    ids = ref.packed_ids(lengths, pad)
+    base, x, a, b, scales = _inputs(len(ids), K, slices, 3, r, K + r)
+    adapters = torch.tensor([i % 4 - 1 for i in range(1, len(lengths) + 1)], dtype=torch.int32)
+    _check(pkg, dev, base, x, a, b, scales, slices, adapters, ids, kind=kind)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "mx"])
+def test_many_rows_of_mixed_adapters(pkg, dev, kind):
+    T, n = 1500, 7
+    base, x, a, b, scales = _inputs(T, 384, (192,), n, 32, 78)
+    adapters = torch.randint(-1, n, (T,), generator=torch.Generator().manual_seed(7), dtype=torch.int32)
+    _check(pkg, dev, base, x, a, b, scales, (192,), adapters, kind=kind)
+    x[7], base[9] = float("nan"), float("inf")
+    ids = torch.zeros(T, dtype=torch.int32)
+    ids[1203:] = -1
+    to = lambda t: t.to(dev)  # noqa: E731
+    xd = to(x) if kind == "bf16" else _mx(pkg, dev, x)
+    view = torch.full((T, 200), 5.0, dtype=torch.bfloat16, device=dev)
+    view[:, 8:] = to(base)
+    out = pkg.lora_add(view[:, 8:], xd, to(a), to(b), to(adapters[:1]) * 0, request_ids=to(ids), out=view[:, 8:])
+    assert bool(out[7].isnan().all()) and bool(out[9].isinf().all())
+    assert torch.equal(out[1203:].cpu(), base[1203:]) and bool((view[:, :8] == 5.0).all())
+    rest = torch.ones(T, dtype=torch.bool)
+    rest[[7, 9]] = False
+    assert bool(out[rest.to(dev)].isfinite().all())
+
+
 @pytest.mark.parametrize("kind", ["bf16", "mx"])
 @pytest.mark.parametrize("lengths,pad", [([1], 0), ([1] * 40, 3), ([100, 28], 0), ([130, 1, 0, 200], 17), ([500], 12)])
 def test_requests(pkg, dev, kind, lengths, pad):

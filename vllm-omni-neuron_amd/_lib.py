@@ -168,17 +168,27 @@ def stream_of(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
-def call(name: str, t: torch.Tensor, *args) -> None:
-    """Calls one entry point on ``t``'s device and its current stream (the last argument), whichever device is
-    current, and raises on its status."""
-    fn = getattr(load(), name)
-    index = t.get_device()
+def call(name: str, index: int, *args) -> None:
+    """Calls one entry point on GPU ``index`` and its current stream (the last argument), whichever device is current,
+    and raises on its status."""
+    fn = getattr(_LIB or load(), name)
     if index == torch._C._cuda_getDevice():
-        status = fn(*args, stream_of(t))
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            status = fn(*args, stream_of(t))
-    check(status, name)
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        check(status, name)
+
+
+def plain_ptr(t: torch.Tensor | None, dtype: torch.dtype, shape, dev: int):
+    """The pointer of a contiguous, 16-byte aligned tensor of this type and shape on GPU ``dev`` (None for None), or -1:
+    the ordinary case of an argument in one look. What it does not accept goes through the full checks, which say what
+    is wrong with it or take it as it is (0.5 us an argument here, 1.5 there)."""
+    if t is None:
+        return None
+    p = t.data_ptr()
+    return p if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == dev and not p & 15 else -1
 
 
 def refuse_overlap(out: torch.Tensor, what: str, *inputs: torch.Tensor | None) -> None:

@@ -241,6 +241,74 @@ def adaln_sandwich(
     as they are where the caller gave them, zeros where they are allocated here. ``residual_out`` may be
     ``residual`` and ``out`` (contiguous; an :class:`MXTensor` for ``quant="mx"``) may be ``hidden``.
     """
+    if out is None and residual_out is None:
+        r = _sandwich_plain(hidden, residual, mul, add, eps, post_norm, post_weight, gate, residual_scale, norm_type, quant,
+                            request_ids)
+        if r is not None:
+            return r
+    return _sandwich_checked(hidden, residual, mul, add, eps, post_norm, post_weight, gate, residual_scale, norm_type, quant,
+                             request_ids, residual_out, out)
+
+
+def _request_ptr(vec: torch.Tensor | None, shape, dev: int):
+    """``(pointer, elements between requests)`` of one of the vectors of ordinary form, ``(-1, 0)`` otherwise."""
+    if vec is None:
+        return None, 0
+    p, st = vec.data_ptr(), vec.stride()
+    if vec.dtype is torch.float32 and vec.shape == shape and st[-1] == 1 and vec.get_device() == dev and not p & 15:
+        if len(st) == 1:
+            return p, 0
+        if st[0] >= shape[1] and not st[0] & 3 and shape[0] > 1:
+            return p, st[0]
+    return -1, 0
+
+
+def _sandwich_plain(hidden, residual, mul, add, eps, post_norm, post_weight, gate, alpha, norm_type, quant, ids):
+    """:func:`adaln_sandwich` for arguments of ordinary form (contiguous rows, vectors of one shape, outputs allocated
+    here); None if any is not."""
+    try:
+        T, H = shape = hidden.shape
+        if H & 31 or not 0 < H <= _MAX_HIDDEN or not eps >= 0:
+            return None
+        norms, dev = _lib.NORM, hidden.get_device()
+        n_post, n_pre, n_quant = norms[post_norm], norms[norm_type], _lib.QUANT[quant]
+        ph = _lib.plain_ptr(hidden, torch.bfloat16, shape, dev)
+        pr = _lib.plain_ptr(residual, torch.bfloat16, shape, dev)
+        pw = _lib.plain_ptr(post_weight, torch.float32, (H,), dev)
+        pi = _lib.plain_ptr(ids, torch.int32, (T,), dev)
+        one = mul if mul is not None else gate if gate is not None else add
+        vs, requests = (), 2**31 - 1
+        if one is not None:
+            vs = one.shape
+            if vs[-1] != H or len(vs) > 2:
+                return None
+            if len(vs) == 2:
+                requests = vs[0]
+                if ids is None:
+                    return None
+        pg, lg = _request_ptr(gate, vs, dev)
+        pm, lm = _request_ptr(mul, vs, dev)
+        pa, la = _request_ptr(add, vs, dev)
+    except (AttributeError, KeyError, TypeError, ValueError):
+        return None
+    if dev < 0 or pr is None or T == 0 or -1 in (ph, pr, pw, pi, pg, pm, pa):
+        return None
+    residual_out = torch.empty_like(hidden)
+    scales = ps = None
+    if n_quant == 0:
+        out = torch.empty_like(hidden)
+    else:
+        out = torch.empty((T, H + 4 if n_quant == 2 else H), dtype=torch.float8_e4m3fn, device=hidden.device)
+        if n_quant == 1:
+            scales = torch.empty((T, H >> 5), dtype=torch.uint8, device=hidden.device)
+            ps = scales.data_ptr()
+    _lib.call("wanmi_adaln_sandwich", dev, ph, H, pr, H, pw, pg, lg, pm, lm, pa, la, pi, requests, alpha, T, H, eps, n_post, n_pre,
+              n_quant, 1, residual_out.data_ptr(), out.data_ptr(), ps)
+    return residual_out, out if scales is None else MXTensor(out, scales)
+
+
+def _sandwich_checked(hidden, residual, mul, add, eps, post_norm, post_weight, gate, residual_scale, norm_type, quant,
+                      request_ids, residual_out, out):
     if post_norm not in _SUPPORTED_NORMS:
         raise ValueError(f"unsupported post_norm {post_norm!r}")
     _lib.expect(hidden, "hidden", dtype=torch.bfloat16, shape=(None, None), contiguous=False)
@@ -295,7 +363,7 @@ def adaln_sandwich(
             codes = make((T, H + 4 if quant == "row" else H), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
             scales = make((T, H // 32), dtype=torch.uint8, device=dev) if quant == "mx" else None
     p = _lib.ptr
-    _lib.call("wanmi_adaln_sandwich", hidden, p(hidden), ld_h, p(residual), ld_r, p(post_weight), p(gate), ld_gate, p(mul), ld_mul,
+    _lib.call("wanmi_adaln_sandwich", hidden.get_device(), p(hidden), ld_h, p(residual), ld_r, p(post_weight), p(gate), ld_gate, p(mul), ld_mul,
               p(add), ld_add, p(request_ids), 2**31 - 1 if requests is None else requests, float(residual_scale), T, H,
               float(eps), _lib.NORM[post_norm], _lib.NORM[norm_type], _lib.QUANT[quant], int(zero_rest), p(residual_out),
               p(codes), p(scales))

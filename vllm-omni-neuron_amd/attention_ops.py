@@ -198,6 +198,55 @@ def qk_norm_rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.
     with a negative id (or one not below ``requests``) belong to no request and are not read; their rows are left as
     they are in a given output, zeros in one allocated here.
     """
+    if q_out is None and k_out is None and not want_max and type(axes) is tuple:
+        done = _qk_axes_plain(q, k, positions, axes, theta, rope_pairs, norm, q_gamma, k_gamma, eps, request_ids, requests)
+        if done is not None:
+            return done
+    return _qk_axes_checked(q, k, positions, axes, theta, rope_pairs, norm, q_gamma, k_gamma, eps, request_ids, requests, want_max,
+                            q_out, k_out)
+
+
+@functools.lru_cache(maxsize=64)
+def _axes_fit(axes: tuple, D: int) -> bool:
+    return 1 <= len(axes) <= 8 and all(type(d) is int and d >= 0 and d % 2 == 0 for d in axes) and sum(axes) <= D and sum(axes) % 16 == 0
+
+
+def _qk_axes_plain(q, k, positions, axes, theta, rope_pairs, norm, q_gamma, k_gamma, eps, ids, requests):
+    """:func:`qk_norm_rope_axes` for arguments of ordinary form (q and k given, outputs allocated here); None if any is
+    not."""
+    try:
+        T, qh, D = q.shape
+        kh = k.shape[1]
+        turn, kind, dev = _ROTATE[rope_pairs], _QK_NORM[norm], q.get_device()
+        if D not in (32, 64, 128, 256) or not _axes_fit(axes, D) or not 0 < theta < math.inf or not eps >= 0:
+            return None
+        if not 0 < qh * D <= 16384 or not 0 < kh * D <= 16384 or k.shape != (T, kh, D) or k.get_device() != dev or requests is not None:
+            return None
+        pq, pk, (qts, qhs, qd), (kts, khs, kd) = q.data_ptr(), k.data_ptr(), q.stride(), k.stride()
+        if q.dtype is not torch.bfloat16 or k.dtype is not torch.bfloat16 or qd != 1 or kd != 1 or (pq | pk) & 15 or (qts | qhs | kts | khs) & 7:
+            return None
+        floats = positions.dtype is torch.float32
+        pp = _lib.plain_ptr(positions, torch.float32 if floats else torch.int32, (T, len(axes)), dev)
+        pi = _lib.plain_ptr(ids, torch.int32, (T,), dev)
+        if kind == 0 and (q_gamma is not None or k_gamma is not None):
+            return None
+        gq = _lib.plain_ptr(q_gamma, torch.float32, (D if kind == 1 else qh * D,), dev)
+        gk = _lib.plain_ptr(k_gamma, torch.float32, (D if kind == 1 else kh * D,), dev)
+    except (AttributeError, IndexError, KeyError, TypeError, ValueError):
+        return None
+    if dev < 0 or T == 0 or pp is None or -1 in (pp, pi, gq, gk):
+        return None
+    q_out = torch.empty((T, qh, D), dtype=torch.bfloat16, device=q.device)
+    k_out = torch.empty((T, kh, D), dtype=torch.bfloat16, device=q.device)
+    dims, freqs = _axis_arrays(axes, (theta,) * len(axes))
+    _lib.call("wanmi_qk_norm_rope_axes", dev, pq, qts, qhs, qh, gq, q_out.data_ptr(), qh * D, D, pk, kts, khs, kh, gk,
+              k_out.data_ptr(), kh * D, D, T, D, pp, floats, len(axes), dims, freqs, turn, kind, eps, pi,
+              1 if ids is None else 2**31 - 1, 1, None)
+    return q_out, k_out
+
+
+def _qk_axes_checked(q, k, positions, axes, theta, rope_pairs, norm, q_gamma, k_gamma, eps, request_ids, requests, want_max, q_out,
+                     k_out):
     if rope_pairs not in _ROTATE:
         raise ValueError(f"unknown rope_pairs {rope_pairs!r}")
     if norm not in _QK_NORM:
@@ -276,7 +325,7 @@ def qk_norm_rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.
     p = _lib.ptr
     dims, freqs = _axis_arrays(axes, theta)
     (qts, qhs, qh, qots, qohs), (kts, khs, kh, kots, kohs) = views
-    _lib.call("wanmi_qk_norm_rope_axes", q, p(q), qts, qhs, qh, p(q_gamma), p(outs[0]), qots, qohs, p(k), kts, khs, kh, p(k_gamma),
+    _lib.call("wanmi_qk_norm_rope_axes", q.get_device(), p(q), qts, qhs, qh, p(q_gamma), p(outs[0]), qots, qohs, p(k), kts, khs, kh, p(k_gamma),
               p(outs[1]), kots, kohs, T, D, p(positions), int(positions.dtype == torch.float32), len(axes), dims, freqs,
               _ROTATE[rope_pairs], _QK_NORM[norm], float(eps), p(request_ids), n, int(zero_rest), p(kmax))
     return (*outs, kmax) if want_max else tuple(outs)

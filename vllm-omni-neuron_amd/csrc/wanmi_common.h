@@ -189,6 +189,15 @@ __device__ __forceinline__ int max_with_lane_xor32(int x) {
   return max((int)r[0], (int)r[1]);
 }
 
+// 1 / sqrt(x) for x >= 0 in fp32: the hardware's estimate (within 1 ulp, infinite for 0 and 0 for infinity), one Newton
+// step where that is finite and not zero. A workgroup whose threads all need the root of their row spends a
+// fourth of the time on it that the fp64 division and root take.
+__device__ __forceinline__ float rsqrt_f32(float x) {
+  const float y = __builtin_amdgcn_rsqf(x);
+  const float z = y * fmaf(-0.5f * x * y, y, 1.5f);
+  return y > 0.0f && y < INFINITY ? z : y;
+}
+
 // s_waitcnt immediates (gfx9 encoding: vmcnt[3:0] | expcnt[6:4] | lgkmcnt[11:8] | vmcnt[5:4] << 14)
 constexpr int waitcnt_vm(int n) { return (n & 0xF) | (0x7 << 4) | (0xF << 8) | ((n >> 4) << 14); }
 constexpr int waitcnt_lgkm(int n) { return 0xF | (0x7 << 4) | ((n & 0xF) << 8) | (0x3 << 14); }

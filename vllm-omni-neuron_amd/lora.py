@@ -29,6 +29,19 @@ def _check_slices(slices, N: int) -> tuple:
     return slices
 
 
+def _workspace(T: int, K: int, parts: int, rank: int) -> int:
+    return _lib.load().wanmi_lora_workspace(T, K, parts, rank)
+
+
+@functools.lru_cache(maxsize=64)
+def _fits(slices: tuple, N: int) -> bool:
+    """Whether :func:`_check_slices` takes these widths as they are."""
+    try:
+        return _check_slices(slices, N) == slices
+    except (TypeError, ValueError):
+        return False
+
+
 @functools.lru_cache(maxsize=64)
 def _widths(slices: tuple):
     return (ctypes.c_int64 * len(slices))(*slices)
@@ -84,6 +97,49 @@ def lora_add(base: torch.Tensor, x, a: torch.Tensor, b: torch.Tensor, adapter_id
 
     The sums are fp32 throughout, with one rounding to bf16 at the end.
     """
+    if out is None and (slices is None or type(slices) is tuple):
+        done = _add_plain(base, x, a, b, adapter_ids, scales, slices, request_ids)
+        if done is not None:
+            return done
+    return _add_checked(base, x, a, b, adapter_ids, scales, slices, request_ids, out)
+
+
+def _add_plain(base, x, a, b, adapter_ids, scales, slices, request_ids):
+    """:func:`lora_add` for arguments of ordinary form (contiguous rows, bf16 or MX activations, ``out`` allocated here);
+    None if any is not."""
+    try:
+        T, N = shape = base.shape
+        dev = base.get_device()
+        n, R, K = a.shape
+        r = b.shape[2]
+        slices = (N,) if slices is None else slices
+        parts = len(slices)
+        if not 0 < r <= 1024 or r & 15 or R != parts * r or K & 31 or N & 7 or not _fits(slices, N):
+            return None
+        if type(x) is MXTensor:
+            px, psx = _lib.plain_ptr(x.codes, torch.float8_e4m3fn, (T, K), dev), _lib.plain_ptr(x.scales, torch.uint8, (T, K >> 5), dev)
+        else:
+            px, psx = _lib.plain_ptr(x, torch.bfloat16, (T, K), dev), None
+        pb = _lib.plain_ptr(base, torch.bfloat16, shape, dev)
+        pA = _lib.plain_ptr(a, torch.bfloat16, (n, R, K), dev)
+        pB = _lib.plain_ptr(b, torch.bfloat16, (n, N, r), dev)
+        ps = _lib.plain_ptr(scales, torch.float32, (n,), dev)
+        pq = _lib.plain_ptr(request_ids, torch.int32, (T,), dev)
+        requests = T if request_ids is None else adapter_ids.shape[0]
+        pe = _lib.plain_ptr(adapter_ids, torch.int32, (requests,), dev)
+    except (AttributeError, IndexError, TypeError, ValueError):
+        return None
+    if dev < 0 or T == 0 or n < 1 or None in (px, pA, pB, pe) or -1 in (px, psx, pb, pA, pB, ps, pq, pe):
+        return None
+    out = torch.empty_like(base)
+    size = _workspace(T, K, parts, r)
+    work = torch.empty(size, dtype=torch.uint8, device=base.device)
+    _lib.call("wanmi_lora_add", dev, px, psx, None, K, pA, pB, ps, pe, pq, requests, n, T, K, N, r, parts, _widths(slices), pb, N,
+              out.data_ptr(), N, 1, work.data_ptr(), size)
+    return out
+
+
+def _add_checked(base, x, a, b, adapter_ids, scales, slices, request_ids, out):
     _lib.expect(base, "base", dtype=torch.bfloat16, shape=(None, None), contiguous=False, row_contiguous=True)
     T, N = base.shape
     if isinstance(x, torch.Tensor) and x.dtype == torch.bfloat16:
@@ -130,10 +186,10 @@ def lora_add(base: torch.Tensor, x, a: torch.Tensor, b: torch.Tensor, adapter_id
         out = torch.empty((T, N), dtype=torch.bfloat16, device=base.device)
     if T == 0:
         return out
-    size = _lib.load().wanmi_lora_workspace(T, K, len(slices), r)
+    size = _workspace(T, K, len(slices), r)
     work = torch.empty(size, dtype=torch.uint8, device=base.device)
     p = _lib.ptr
-    _lib.call("wanmi_lora_add", base, p(codes), p(x_scales), p(row_scale), ldx, p(a), p(b), p(scales), p(adapter_ids), p(request_ids),
+    _lib.call("wanmi_lora_add", base.get_device(), p(codes), p(x_scales), p(row_scale), ldx, p(a), p(b), p(scales), p(adapter_ids), p(request_ids),
               T if request_ids is None else adapter_ids.shape[0], n, T, K, N, r, len(slices), _widths(slices), p(base), ldb, p(out),
               out.stride(0) if T > 1 else N, int(zero_rest), p(work), size)
     return out

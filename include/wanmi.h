@@ -361,7 +361,7 @@ int wanmi_dmajor_to_mx(const void* x, int64_t B, int heads, int64_t S, int64_t b
  * hidden, residual: bf16 [T, H], rows ld_* elements apart (multiples of 8); residual_out bf16 [T, H]; post_weight
  * fp32 [H]; gate, mul, add fp32: one row of H per request, ld_* elements apart (multiples of 4), or ld_* 0: one
  * row for every request; out and scales as wanmi_adaln_quant's. q = request_ids[t] (int32; NULL: every row is request 0). A row whose id is not in
- * [0, requests) is not read; its outputs are left as they are, or zeroed with zero_rest. residual_out may
+ * [0, requests) is not computed; its outputs are left as they are, or zeroed with zero_rest. residual_out may
  * be `residual`, out `hidden`, row for row. H as for wanmi_adaln_quant. Both norms use eps.
  * Stands beside wanmi_adaln_quant (one request, no norm before the gate); no reference counterpart.
  */

@@ -195,7 +195,7 @@ def qk_norm_rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.
     Returns ``(q_out, k_out)``; ``q_out`` / ``k_out`` may be given, and may be ``q`` and ``k`` themselves. With
     ``want_max`` also fp32 ``[requests, Hk]``: a bound on the norms of each request's K rows, the ``kmax`` of
     :func:`attention_core` (``requests`` says how many; 1 without ``request_ids``). ``request_ids`` int32 ``[T]``: rows
-    with a negative id (or one not below ``requests``) belong to no request and are not read; their rows are left as
+    with a negative id (or one not below ``requests``) belong to no request and are not computed; their rows are left as
     they are in a given output, zeros in one allocated here.
     """
     if q_out is None and k_out is None and not want_max and type(axes) is tuple:

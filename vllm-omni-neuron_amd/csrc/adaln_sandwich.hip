@@ -365,19 +365,10 @@ __global__ __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_per_eu
                     : (a.add ? a.add + id * a.ld_add : nullptr);
   };
 
-  // the workgroup's requests (one a lane); every wave comes to the same decision
-  const bool in = lane < waves && row0 + lane < a.T;
-  const int theirs = !in ? -1 : a.ids ? a.ids[row0 + lane] : 0;
-  const uint64_t alive = __ballot((uint32_t)theirs < (uint32_t)a.requests);
-  const int first = alive ? __builtin_amdgcn_readlane(theirs, __builtin_ctzll(alive)) : -1;
-  const bool one = alive && __ballot(theirs == first) == alive;
-  const int64_t row = row0 + wave;
-  const int id = __builtin_amdgcn_readlane(theirs, wave);
-  const bool live = (uint32_t)id < (uint32_t)a.requests;
-  // the row itself is under way while the vectors are
+  const int64_t row = row0 + wave, from = min(row, a.T - 1);
+  // the row is under way while its request is looked up and the vectors are copied
   constexpr int kAhead = NCH <= 6 ? NCH : 4;  // chunks of the residual under way (all of it where the registers hold it)
   uint32_t xp[NCH][4], rp[kAhead][4];
-  const int64_t from = live ? row : 0;  // (a row of no request: any row, not used)
   const __amdgpu_buffer_rsrc_t r_x = rsrc(a.hidden + from * a.ld_h, 2 * (int64_t)H);
   const __amdgpu_buffer_rsrc_t r_r = rsrc(a.residual + from * a.ld_r, 2 * (int64_t)H);
   // columns past H in the last chunk lie past the descriptors' extents and read as zero
@@ -393,6 +384,14 @@ __global__ __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
     for (int j = 0; j < 4; ++j) rp[c][j] = v[j];
   }
+  // the workgroup's requests (one a lane); every wave comes to the same decision
+  const bool in = lane < waves && row0 + lane < a.T;
+  const int theirs = !in ? -1 : a.ids ? a.ids[row0 + lane] : 0;
+  const uint64_t alive = __ballot((uint32_t)theirs < (uint32_t)a.requests);
+  const int first = alive ? __builtin_amdgcn_readlane(theirs, __builtin_ctzll(alive)) : -1;
+  const bool one = alive && __ballot(theirs == first) == alive;
+  const int id = __builtin_amdgcn_readlane(theirs, wave);
+  const bool live = (uint32_t)id < (uint32_t)a.requests;
   if (one) {
     held = first;
     for (int k = wave; k < 8 * nch; k += waves) {  // 1 KiB pieces: vector, half, chunk

@@ -12,10 +12,20 @@
 // and only then rounded, so that it is as exact for a far position as for a near one: sine and cosine
 // of at most pi/4 by their power series, whose next terms are below 2e-9 and 3e-8.
 //
-// One wavefront owns a row of Q or of K. A lane holds units of 16 channels (8 pairs): interleaved pairs
-// lie in 32 consecutive bytes, halves in 16 bytes at i and 16 at i + rot/2. A head has D / 16 = 2 .. 16 units, a
-// power of two, so a lane's units have the same place u in every head it serves: its 8 angles are read once
-// per row. The row's angles are computed once, one pair per lane, and passed through LDS.
+// One wavefront owns a row of Q or of K, and a workgroup of eight rows shares the weight of the norm across heads in LDS (fp32,
+// it is as many bytes as the row is read and written: from L2 for every row, 32760 rows of 40 + 40 heads took
+// 283 us). A wave takes one row and ends: the loads of a next one would stand behind the stores of this one in
+// the order that a wave waits for them.
+//
+// A lane holds runs of 8 channels (16 bytes), neighbouring lanes neighbouring runs, so that every instruction moves whole
+// lines. Interleaved pairs lie within a run; a run of 64 x i + lane has the same place in its head for every i, since a
+// head has D / 8 = 4 .. 32 runs, so its 4 angles are the lane's own. For halves a lane holds the two runs whose
+// channels pair up (8 angles), and the same holds for these units of 16 channels. The row's angles are computed
+// once, one pair a lane, and passed through LDS.
+//
+// The largest norm of a request's K rows: the workgroup's largest is compared with what is there already and
+// exchanged only if it is larger, since atomics on these few addresses are served one after another for all the
+// XCDs (a maximum does not depend on their order).
 #include "wanmi_common.h"
 
 namespace wanmi {
@@ -61,62 +71,84 @@ __device__ __forceinline__ void sincos_turns(double turns, float& sn, float& cs)
   cs = (k == 1 || k == 2) ? -b : b;
 }
 
-// Sum over the 2^shift lanes of a head (aligned groups).
+// Sum over the 2^shift lanes of a head (aligned groups, at most 32).
 __device__ __forceinline__ float head_sum(float v, int shift) {
   if (shift > 0) v += dpp_f32<0xB1>(v);
   if (shift > 1) v += dpp_f32<0x4E>(v);
   if (shift > 2) v += dpp_f32<0x141>(v);
   if (shift > 3) v += dpp_f32<0x140>(v);
+  if (shift > 4) v = add_lane_xor16(v);
   return v;
 }
 
-// NU: units per lane at most (heads * D / 16 / 64, rounded up).
-template <int NU, bool kHalves>
-__global__ __launch_bounds__(256) void qk_axes_kernel(QKAxesArgs a) {
-  __shared__ float tab[4][2][kMaxPairs];
+__device__ __forceinline__ void raise_max(float* at, float n) {
+  unsigned int* p = reinterpret_cast<unsigned int*>(at);
+  const unsigned int bits = __float_as_uint(n);  // (not negative: the order of the bits is the order of the values, NaN on top)
+  if (bits > __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(p, bits);
+}
+
+constexpr int kRowWaves = 8;
+
+// NU: units of 16 channels per lane, heads * D / 16 / 64 rounded up; kWhole: every lane has all of them.
+template <int NU, bool kHalves, bool kWhole>
+__global__ __launch_bounds__(64 * kRowWaves) __attribute__((amdgpu_waves_per_eu(NU <= 3 || (NU <= 5 && (kWhole || !kHalves)) ? 4 : 2))) void qk_axes_kernel(QKAxesArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) float gam[];  // [run slot][half][lane] x 4 floats; then the heads' maxima
+  __shared__ float tab[kRowWaves][2][kMaxPairs];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
-  if (row >= a.T) return;
   const QKAxesArgs::Part p = a.part[blockIdx.y];
-  const int id = a.ids ? __builtin_amdgcn_readfirstlane(a.ids[row]) : 0;
-  const bool live = (uint32_t)id < (uint32_t)a.requests;
-  if (!live && !a.zero_rest) return;
-  const int u = lane & ((1 << a.unit_shift) - 1);
-  const int heads_step = 64 >> a.unit_shift;
-  const int h0 = lane >> a.unit_shift;
-  const bool turn = u < a.rot_units;
-  // the unit's two runs of 8 channels
-  const int c0 = kHalves && turn ? 8 * u : 16 * u;
-  const int c1 = kHalves && turn ? a.half + 8 * u : 16 * u + 8;
-  uint16_t* po = p.out + row * p.out_ts;
-  if (!live) {
-    const u32x4 z = {0u, 0u, 0u, 0u};
+  if (p.heads == 0) return;
+  const int D = 16 << a.unit_shift;
+  const int64_t row0 = (int64_t)blockIdx.x * kRowWaves, row = row0 + wave;
+  // the lane's place in its heads, its first head, heads from one of its runs (units) to the next
+  const int shift = kHalves ? a.unit_shift : a.unit_shift + 1;
+  const int u = lane & ((1 << shift) - 1), h0 = lane >> shift, step = 64 >> shift;
+  const bool turn = kHalves ? u < a.rot_units : u < 2 * a.rot_units;
+  constexpr int kRuns = 2 * NU;
+  // channel in its head of run slot i, and its head
+  const int c0 = kHalves ? (turn ? 8 * u : 16 * u) : 8 * u, c1 = kHalves ? (turn ? a.half + 8 * u : 16 * u + 8) : 8 * u;
+  const auto chan = [&](int i) { return kHalves && (i & 1) ? c1 : c0; };
+  const auto head = [&](int i) { return h0 + (kHalves ? i >> 1 : i) * step; };
+  const auto has = [&](int i) { return kWhole || head(i) < p.heads; };
+
+  const int64_t from = min(row, a.T - 1);  // (the loads do not wait to know whether the row has a request)
+  u32x4 x[kRuns];
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      const int h = h0 + i * heads_step;
-      if (h < p.heads) {
-        store_b128_guarded(z, po + h * p.out_hs + c0);
-        store_b128_guarded(z, po + h * p.out_hs + c1);
-      }
-    }
-    return;
+  for (int i = 0; i < kRuns; ++i) {
+    x[i] = u32x4{0u, 0u, 0u, 0u};
+    if (has(i)) x[i] = *reinterpret_cast<const u32x4*>(p.x + from * p.ts + head(i) * p.hs + chan(i));
   }
-  const uint16_t* px = p.x + row * p.ts;
-  u32x4 x0[NU], x1[NU];
+  // the workgroup's requests (one a lane); every wave comes to the same decision
+  const int theirs = lane >= kRowWaves || row0 + lane >= a.T ? -1 : a.ids ? a.ids[row0 + lane] : 0;
+  const uint64_t alive = __ballot((uint32_t)theirs < (uint32_t)a.requests);
+  const int first = alive ? __builtin_amdgcn_readlane(theirs, __builtin_ctzll(alive)) : -1;
+  const bool one = __ballot(theirs == first) == alive;
+  const bool live = alive >> wave & 1;
+  float own[kHalves ? 2 : 1][8];  // the weight of a norm per head: the same for all of the lane's heads
+  const bool each = a.norm == WANMI_QKNORM_PER_HEAD;
+  if (each) {
 #pragma unroll
-  for (int i = 0; i < NU; ++i) {
-    const int h = h0 + i * heads_step;
-    x0[i] = x1[i] = u32x4{0u, 0u, 0u, 0u};
-    if (h < p.heads) {
-      x0[i] = *reinterpret_cast<const u32x4*>(px + h * p.hs + c0);
-      x1[i] = *reinterpret_cast<const u32x4*>(px + h * p.hs + c1);
-    }
+    for (int r = 0; r < (kHalves ? 2 : 1); ++r)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) own[r][j] = p.gamma ? p.gamma[chan(r) + j] : 1.0f;
   }
+  const bool across = a.norm == WANMI_QKNORM_ACROSS_HEADS && p.gamma;
+  if (across) {
+    const u32x4 rg = buffer_rsrc(p.gamma, 4u * (uint32_t)(p.heads * D));  // heads past the end: zeros, not used
+    const uint32_t base = lds_addr(gam);
+#pragma unroll
+    for (int k = 0; k < 2 * kRuns; ++k)
+      if (k % kRowWaves == wave)
+        lds_dma_b128(rg, (uint32_t)((head(k >> 1) * D + chan(k >> 1) + 4 * (k & 1)) * 4), base + k * 1024);
+  }
+  float* maxima = gam + (a.norm == WANMI_QKNORM_ACROSS_HEADS ? 2 * kRuns * 256 : 0);
+  const bool bound = a.kmax && blockIdx.y == 1;
+  if (bound)
+    for (int h = threadIdx.x; h < p.heads; h += 64 * kRowWaves) maxima[h] = 0.0f;
   float* tc = tab[wave][0];
   float* tsn = tab[wave][1];
   for (int i = lane; i < a.pairs; i += 64) {
-    const int64_t at = row * a.axes + a.axis[i];
+    const int64_t at = from * a.axes + a.axis[i];
     const double pos = a.pos_float ? (double)reinterpret_cast<const float*>(a.pos)[at]
                                    : (double)reinterpret_cast<const int32_t*>(a.pos)[at];
     float sn, cs;
@@ -124,100 +156,123 @@ __global__ __launch_bounds__(256) void qk_axes_kernel(QKAxesArgs a) {
     tc[i] = cs;
     tsn[i] = sn;
   }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-  __builtin_amdgcn_wave_barrier();
-  float cs[8], sn[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    cs[j] = turn ? tc[8 * u + j] : 1.0f;
-    sn[j] = turn ? tsn[8 * u + j] : 0.0f;
+  if (across || bound) {
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    __syncthreads();
+  } else {  // nothing that other waves wrote
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
-  float rs = 1.0f;
-  if (a.norm == WANMI_QKNORM_ACROSS_HEADS) {
-    float ss = 0.0f;
+
+  uint16_t* po = p.out + row * p.out_ts;
+  if (live) {
+    constexpr int kAngles = kHalves ? 8 : 4;
+    float cs[kAngles], sn[kAngles];
 #pragma unroll
-    for (int i = 0; i < NU; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        ss += bf16_lo(x0[i][j]) * bf16_lo(x0[i][j]) + bf16_hi(x0[i][j]) * bf16_hi(x0[i][j]);
-        ss += bf16_lo(x1[i][j]) * bf16_lo(x1[i][j]) + bf16_hi(x1[i][j]) * bf16_hi(x1[i][j]);
-      }
-    ss = wave_sum_f32_asc(ss);
-    rs = (float)(1.0 / sqrt((double)(ss / (float)(p.heads << (a.unit_shift + 4))) + (double)a.eps));
-  }
-  const int D = 16 << a.unit_shift;
-#pragma unroll
-  for (int i = 0; i < NU; ++i) {
-    const int h = h0 + i * heads_step;
-    const bool ok = h < p.heads;
-    // the unit's values in memory order: v0 of its first run, v1 of its second
-    float v0[8], v1[8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v0[2 * j] = bf16_lo(x0[i][j]);
-      v0[2 * j + 1] = bf16_hi(x0[i][j]);
-      v1[2 * j] = bf16_lo(x1[i][j]);
-      v1[2 * j + 1] = bf16_hi(x1[i][j]);
+    for (int j = 0; j < kAngles; ++j) {
+      cs[j] = turn ? tc[kAngles * u + j] : 1.0f;
+      sn[j] = turn ? tsn[kAngles * u + j] : 0.0f;
     }
-    if (a.norm != WANMI_QKNORM_NONE) {
-      float g = rs;
-      if (a.norm == WANMI_QKNORM_PER_HEAD) {
-        float ss = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ss += v0[j] * v0[j] + v1[j] * v1[j];
-        ss = head_sum(ss, a.unit_shift);
-        g = (float)(1.0 / sqrt((double)(ss / (float)D) + (double)a.eps));
-      }
-      if (p.gamma && ok) {
-        const float* pg = p.gamma + (a.norm == WANMI_QKNORM_PER_HEAD ? 0 : h * D);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          v0[j] *= g * pg[c0 + j];
-          v1[j] *= g * pg[c1 + j];
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v0[j] *= g, v1[j] *= g;
-      }
-    }
-    if (turn) {
-      if (kHalves) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float x = v0[j], y = v1[j];
-          v0[j] = x * cs[j] - y * sn[j];
-          v1[j] = x * sn[j] + y * cs[j];
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = v0[2 * j], y = v0[2 * j + 1], z = v1[2 * j], w = v1[2 * j + 1];
-          v0[2 * j] = x * cs[j] - y * sn[j];
-          v0[2 * j + 1] = x * sn[j] + y * cs[j];
-          v1[2 * j] = z * cs[4 + j] - w * sn[4 + j];
-          v1[2 * j + 1] = z * sn[4 + j] + w * cs[4 + j];
-        }
-      }
-    }
-    if (a.kmax && blockIdx.y == 1) {
+    float rs = 1.0f;
+    if (a.norm == WANMI_QKNORM_ACROSS_HEADS) {
       float ss = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss += v0[j] * v0[j] + v1[j] * v1[j];
-      ss = head_sum(ss, a.unit_shift);
-      // a rounding to bf16 adds at most 2^-8 of a value: the written row's norm is below this
-      const float n = sqrtf(ss) * 1.00390625f;
-      if (ok && u == 0) atomicMax(reinterpret_cast<unsigned int*>(a.kmax) + (int64_t)id * p.heads + h, __float_as_uint(n));
-    }
-    if (ok) {
-      u32x4 o0, o1;
+      for (int i = 0; i < kRuns; ++i) {
+        float q[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        o0[j] = pack_bf16x2(v0[2 * j], v0[2 * j + 1]);
-        o1[j] = pack_bf16x2(v1[2 * j], v1[2 * j + 1]);
+        for (int j = 0; j < 4; ++j) q[j] = bf16_lo(x[i][j]) * bf16_lo(x[i][j]) + bf16_hi(x[i][j]) * bf16_hi(x[i][j]);
+        ss += (q[0] + q[1]) + (q[2] + q[3]);
       }
-      store_b128_guarded(o0, po + h * p.out_hs + c0);
-      store_b128_guarded(o1, po + h * p.out_hs + c1);
+      rs = rsqrt_f32(wave_sum_f32_asc(ss) / (float)(p.heads * D) + a.eps);
+      // (the row is unpacked anew below instead of being held as fp32)
+#pragma unroll
+      for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t w = x[i][j];
+          asm volatile("" : "+v"(w));
+          x[i][j] = w;
+        }
     }
+#pragma unroll
+    for (int i = 0; i < kRuns; i += kHalves ? 2 : 1) {
+      constexpr int kN = kHalves ? 2 : 1;  // runs taken together
+      float v[kN][8];
+#pragma unroll
+      for (int r = 0; r < kN; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[r][2 * j] = bf16_lo(x[i + r][j]), v[r][2 * j + 1] = bf16_hi(x[i + r][j]);
+      if (each) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kN; ++r) {
+          float q[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) q[j] = v[r][2 * j] * v[r][2 * j] + v[r][2 * j + 1] * v[r][2 * j + 1];
+          ss += (q[0] + q[1]) + (q[2] + q[3]);
+        }
+        const float g = rsqrt_f32(head_sum(ss, shift) / (float)D + a.eps);
+#pragma unroll
+        for (int r = 0; r < kN; ++r)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[r][j] *= g * own[r][j];
+      } else if (across) {
+#pragma unroll
+        for (int r = 0; r < kN; ++r) {
+          const f32x4 lo = reinterpret_cast<const f32x4*>(gam)[(i + r) * 128 + lane], hi = reinterpret_cast<const f32x4*>(gam)[(i + r) * 128 + 64 + lane];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[r][j] *= rs * lo[j], v[r][4 + j] *= rs * hi[j];
+        }
+      } else if (a.norm == WANMI_QKNORM_ACROSS_HEADS) {
+#pragma unroll
+        for (int r = 0; r < kN; ++r)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[r][j] *= rs;
+      }
+      if (turn) {
+        if constexpr (kHalves) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float s = v[0][j], t = v[1][j];
+            v[0][j] = s * cs[j] - t * sn[j];
+            v[1][j] = s * sn[j] + t * cs[j];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float s = v[0][2 * j], t = v[0][2 * j + 1];
+            v[0][2 * j] = s * cs[j] - t * sn[j];
+            v[0][2 * j + 1] = s * sn[j] + t * cs[j];
+          }
+        }
+      }
+      if (bound) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kN; ++r)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ss += v[r][j] * v[r][j];
+        // a rounding to bf16 adds at most 2^-8 of a value: the written row's norm is below this
+        const float n = sqrtf(head_sum(ss, shift)) * 1.00390625f;
+        if (u == 0 && has(i)) {
+          if (one) atomicMax(reinterpret_cast<unsigned int*>(maxima) + head(i), __float_as_uint(n));
+          else raise_max(a.kmax + (int64_t)__builtin_amdgcn_readlane(theirs, wave) * p.heads + head(i), n);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < kN; ++r) {
+        const u32x4 o = {pack_bf16x2(v[r][0], v[r][1]), pack_bf16x2(v[r][2], v[r][3]), pack_bf16x2(v[r][4], v[r][5]), pack_bf16x2(v[r][6], v[r][7])};
+        if (has(i + r)) store_b128_guarded(o, po + head(i + r) * p.out_hs + chan(i + r));
+      }
+    }
+  } else if (a.zero_rest && row < a.T) {
+#pragma unroll
+    for (int i = 0; i < kRuns; ++i)
+      if (has(i)) store_b128_guarded(u32x4{0u, 0u, 0u, 0u}, po + head(i) * p.out_hs + chan(i));
+  }
+  if (bound && one && alive) {
+    __syncthreads();
+    for (int h = threadIdx.x; h < p.heads; h += 64 * kRowWaves) raise_max(a.kmax + (int64_t)first * p.heads + h, maxima[h]);
   }
 }
 
@@ -226,11 +281,37 @@ __global__ __launch_bounds__(256) void qk_axes_zero_kernel(float* p, int64_t n) 
   if (i < n) p[i] = 0.0f;
 }
 
-template <int NU>
-void launch_qk_axes(const QKAxesArgs& a, bool halves, hipStream_t s) {
-  const dim3 grid((unsigned)((a.T + 3) / 4), a.part[1].heads ? 2u : 1u);
-  if (halves) hipLaunchKernelGGL((qk_axes_kernel<NU, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((qk_axes_kernel<NU, false>), grid, dim3(256), 0, s, a);
+// One instantiation for Q and K: the larger part's.
+template <int NU, bool kHalves>
+void launch_qk_axes(const QKAxesArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((a.T + kRowWaves - 1) / kRowWaves), a.part[1].heads ? 2u : 1u);
+  const int per_head = 1 << a.unit_shift;
+  const bool whole = a.part[0].heads * per_head == 64 * NU && (!a.part[1].heads || a.part[1].heads * per_head == 64 * NU);
+  const int bytes = (a.norm == WANMI_QKNORM_ACROSS_HEADS ? 4096 * NU : 0) + (a.kmax ? 4 * a.part[1].heads : 0);
+  // (16 units, more than 8192 channels: past the 64 KB that a launch has by itself, with the angles)
+  if (NU == 16) {
+    static int allowed[64] = {0};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64 || !allowed[dev]) {
+      for (const void* f : {reinterpret_cast<const void*>(&qk_axes_kernel<NU, kHalves, true>), reinterpret_cast<const void*>(&qk_axes_kernel<NU, kHalves, false>)})
+        if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024) != hipSuccess) return;  // (the error is the launch's)
+      if (dev >= 0 && dev < 64) allowed[dev] = 1;
+    }
+  }
+  if (whole) hipLaunchKernelGGL((qk_axes_kernel<NU, kHalves, true>), grid, dim3(64 * kRowWaves), bytes, s, a);
+  else hipLaunchKernelGGL((qk_axes_kernel<NU, kHalves, false>), grid, dim3(64 * kRowWaves), bytes, s, a);
+}
+
+template <bool kHalves>
+void launch_qk_axes(const QKAxesArgs& a, int nu, hipStream_t s) {
+  if (nu <= 1) launch_qk_axes<1, kHalves>(a, s);
+  else if (nu <= 2) launch_qk_axes<2, kHalves>(a, s);
+  else if (nu <= 3) launch_qk_axes<3, kHalves>(a, s);
+  else if (nu <= 4) launch_qk_axes<4, kHalves>(a, s);
+  else if (nu <= 5) launch_qk_axes<5, kHalves>(a, s);
+  else if (nu <= 6) launch_qk_axes<6, kHalves>(a, s);
+  else if (nu <= 8) launch_qk_axes<8, kHalves>(a, s);
+  else launch_qk_axes<16, kHalves>(a, s);
 }
 
 }  // namespace
@@ -309,11 +390,7 @@ extern "C" int wanmi_qk_norm_rope_axes(const void* q, int64_t q_token_stride, in
   a.kmax = k_maxnorm;
   const int units = (k_heads > q_heads ? k_heads : q_heads) * (head_dim / 16);
   const int nu = (units + 63) / 64;
-  const bool halves = rope_pairs == WANMI_ROTATE_HALVES;
-  if (nu <= 1) launch_qk_axes<1>(a, halves, s);
-  else if (nu <= 2) launch_qk_axes<2>(a, halves, s);
-  else if (nu <= 5) launch_qk_axes<5>(a, halves, s);
-  else if (nu <= 8) launch_qk_axes<8>(a, halves, s);
-  else launch_qk_axes<16>(a, halves, s);
+  if (rope_pairs == WANMI_ROTATE_HALVES) launch_qk_axes<true>(a, nu, s);
+  else launch_qk_axes<false>(a, nu, s);
   return check_launch(f);
 }

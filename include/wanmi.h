@@ -356,8 +356,8 @@ int wanmi_dmajor_to_mx(const void* x, int64_t B, int heads, int64_t S, int64_t b
  * Norms before and after a sub-layer, fused with its gate and residual scale, for packed batches: rows of
  * several requests in one tensor, modulation per request.
  *   p = Norm_post(hidden) * post_weight                              (fp32; post_weight may be NULL)
- *   residual_out = bf16(residual_scale * residual + gate[q] * p)     (gate may be NULL)
- *   out = Q(bf16(Norm_pre(residual_out) * mul[q] + add[q]))          (mul / add may be NULL)
+ *   residual_out = bf16(residual_scale * residual + gate[q] * p)     (residual, gate may be NULL)
+ *   out = Q(bf16(Norm_pre(residual_out) * mul[q] + add[q]))          (mul, add may be NULL; out too: not formed)
  * hidden, residual: bf16 [T, H], rows ld_* elements apart (multiples of 8); residual_out bf16 [T, H]; post_weight
  * fp32 [H]; gate, mul, add fp32: one row of H per request, ld_* elements apart (multiples of 4), or ld_* 0: one
  * row for every request; out and scales as wanmi_adaln_quant's. q = request_ids[t] (int32; NULL: every row is request 0). A row whose id is not in
@@ -383,7 +383,7 @@ int wanmi_adaln_sandwich(const void* hidden, int64_t ld_hidden, const void* resi
  *   t = positions[token][axis of i] * freqs[i]                        (angles in fp64, the rest in fp32)
  * q, k, q_out, k_out: bf16, element (t, h, d) at t * token_stride + h * head_stride + d (strides multiples of 8);
  * k_heads may be 0 (no k); the outputs may be the inputs. positions: int32 or (positions_float) fp32 [T, axes].
- * axis_dims [axes] and freqs [sum(axis_dims) / 2] are HOST arrays: the axes' channels, which fill the head
+ * axis_dims [axes] and freqs [sum(axis_dims) / 2] are HOST arrays (no axes: positions and both NULL): the axes' channels, which fill the head
  * from its first one on (even, their sum a multiple of 16, at most head_dim; channels behind it are not turned), and the
  * angle per unit of position of every pair. rope_pairs: WANMI_ROTATE_* over those channels.
  * gamma: fp32 [heads * head_dim] or [head_dim] as `norm` says, or NULL (ones).

@@ -195,3 +195,12 @@ def test_graph_replays_with_other_requests(pkg, dev):
         want = call()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("norm", ["rms_norm", "rms_norm_across_heads"])
+def test_the_norm_alone(pkg, dev, norm):
+    q, k, _, gq, gk = _inputs(20, 5, 3, 128, norm, 19)
+    oq, ok = pkg.qk_norm_rope_axes(q.to(dev), k.to(dev), None, axes=(), norm=norm, q_gamma=gq.to(dev), k_gamma=gk.to(dev), eps=EPS)
+    for x, gamma, got in ((q, gq, oq), (k, gk, ok)):
+        want, bound, _ = ref.rope_axes(x, torch.zeros(20, 0), (), 1.0, "halves", norm, gamma, EPS)
+        ref.within(got, want, bound)

@@ -222,3 +222,25 @@ def test_on_another_stream(pkg, dev):
         got = pkg.adaln_sandwich(h, res, mul, add, eps=EPS, gate=gate)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("T", [9, 700])
+@pytest.mark.parametrize("H", [96, 5120])
+def test_without_a_residual_or_without_a_second_output(pkg, dev, T, H):
+    ids = ref.packed_ids([T - 2], 2)
+    h, res, w, gate, mul, add = _inputs(T, H, 1, 61)
+    h[T - 1] = float("inf")
+    to = lambda t: t.to(dev)  # noqa: E731
+    kw = dict(eps=EPS, post_weight=to(w), gate=to(gate), request_ids=to(ids))
+    r, y = pkg.adaln_sandwich(to(h), None, to(mul), to(add), residual_scale=3.0, **kw)
+    want, bound = ref.sandwich_residual(h, torch.zeros_like(h), gate.expand(T, H), w, 1.0, "rms_norm", EPS)
+    ref.within(r[: T - 2], want[: T - 2], bound[: T - 2])
+    want, bound = ref.sandwich_modulated(r.cpu(), mul.expand(T, H), add.expand(T, H), "layer_norm", EPS)
+    ref.within(y[: T - 2], want[: T - 2], bound[: T - 2])
+    assert not r[T - 2 :].any() and not y[T - 2 :].any()
+    full, _ = pkg.adaln_sandwich(to(h), to(res), to(mul), to(add), **kw)
+    alone, none = pkg.adaln_sandwich(to(h), to(res), norm_type=None, **kw)
+    assert none is None and torch.equal(alone, full)
+    ro = torch.full_like(full, 2.0)
+    pkg.adaln_sandwich(to(h), to(res), norm_type=None, residual_out=ro, **kw)
+    assert torch.equal(ro[: T - 2], full[: T - 2]) and bool((ro[T - 2 :] == 2.0).all())

@@ -38,4 +38,6 @@ attention_ops.register_torch_ops()
 from . import block  # noqa: F401
 from . import comfy_fp8_checkpoint  # noqa: F401
 from . import kernels  # noqa: F401
+from . import packed_block  # noqa: F401
+from .packed_block import PackedRequests, packed_block_forward, packed_dit_forward  # noqa: F401
 from . import row_block  # noqa: F401

@@ -208,7 +208,7 @@ def _row_stride(t: torch.Tensor, name: str, T: int, H: int) -> int:
 
 def adaln_sandwich(
     hidden: torch.Tensor,
-    residual: torch.Tensor,
+    residual: torch.Tensor | None,
     mul: torch.Tensor | None = None,
     add: torch.Tensor | None = None,
     *,
@@ -217,7 +217,7 @@ def adaln_sandwich(
     post_weight: torch.Tensor | None = None,
     gate: torch.Tensor | None = None,
     residual_scale: float = 1.0,
-    norm_type: str = "layer_norm",
+    norm_type: str | None = "layer_norm",
     quant: str = "none",
     request_ids: torch.Tensor | None = None,
     residual_out: torch.Tensor | None = None,
@@ -228,7 +228,8 @@ def adaln_sandwich(
         r = bf16(residual_scale * residual + gate[q] * (Norm_post(hidden) * post_weight))
         y = Quantize(bf16(Norm_pre(r) * mul[q] + add[q]))
 
-    in one pass over a packed batch; returns ``(r, y)`` as :func:`adaln_modulate` does with a residual.
+    in one pass over a packed batch; returns ``(r, y)`` as :func:`adaln_modulate` does with a residual. Without a
+    ``residual`` (None) r is the gated term alone; with ``norm_type=None`` y is not formed and ``(r, None)`` returned.
 
     ``hidden`` (the sub-layer's output) and ``residual``: bf16 ``[T, H]``, any row stride; ``post_weight`` fp32
     ``[H]``; ``gate`` / ``mul`` / ``add`` fp32 ``[H]`` for every request, or ``[R, H]``, one row per request (rows
@@ -271,7 +272,7 @@ def _sandwich_plain(hidden, residual, mul, add, eps, post_norm, post_weight, gat
         if H & 31 or not 0 < H <= _MAX_HIDDEN or not eps >= 0:
             return None
         norms, dev = _lib.NORM, hidden.get_device()
-        n_post, n_pre, n_quant = norms[post_norm], norms[norm_type], _lib.QUANT[quant]
+        n_post, n_pre, n_quant = norms[post_norm], norms[norm_type], _lib.QUANT[quant]  # (norm_type None: the full checks)
         ph = _lib.plain_ptr(hidden, torch.bfloat16, shape, dev)
         pr = _lib.plain_ptr(residual, torch.bfloat16, shape, dev)
         pw = _lib.plain_ptr(post_weight, torch.float32, (H,), dev)
@@ -291,7 +292,7 @@ def _sandwich_plain(hidden, residual, mul, add, eps, post_norm, post_weight, gat
         pa, la = _request_ptr(add, vs, dev)
     except (AttributeError, KeyError, TypeError, ValueError):
         return None
-    if dev < 0 or pr is None or T == 0 or -1 in (ph, pr, pw, pi, pg, pm, pa):
+    if dev < 0 or T == 0 or -1 in (ph, pr, pw, pi, pg, pm, pa):
         return None
     residual_out = torch.empty_like(hidden)
     scales = ps = None
@@ -302,7 +303,7 @@ def _sandwich_plain(hidden, residual, mul, add, eps, post_norm, post_weight, gat
         if n_quant == 1:
             scales = torch.empty((T, H >> 5), dtype=torch.uint8, device=hidden.device)
             ps = scales.data_ptr()
-    _lib.call("wanmi_adaln_sandwich", dev, ph, H, pr, H, pw, pg, lg, pm, lm, pa, la, pi, requests, alpha, T, H, eps, n_post, n_pre,
+    _lib.call("wanmi_adaln_sandwich", dev, ph, H, pr, H, pw, pg, lg, pm, lm, pa, la, pi, requests, float(alpha), T, H, eps, n_post, n_pre,
               n_quant, 1, residual_out.data_ptr(), out.data_ptr(), ps)
     return residual_out, out if scales is None else MXTensor(out, scales)
 
@@ -312,12 +313,15 @@ def _sandwich_checked(hidden, residual, mul, add, eps, post_norm, post_weight, g
     if post_norm not in _SUPPORTED_NORMS:
         raise ValueError(f"unsupported post_norm {post_norm!r}")
     _lib.expect(hidden, "hidden", dtype=torch.bfloat16, shape=(None, None), contiguous=False)
-    _validate(hidden, norm_type, quant, True)
+    form = norm_type is not None
+    if not form and (quant != "none" or out is not None or mul is not None or add is not None):
+        raise ValueError("norm_type=None forms no second output: no mul, add, quant or out")
+    _validate(hidden, norm_type if form else "none", quant, True)
     T, H = hidden.shape
     if H == 0:
         raise ValueError("hidden size 0")
     ld_h = _row_stride(hidden, "hidden", T, H)
-    ld_r = _row_stride(residual, "residual", T, H)
+    ld_r = ld_h if residual is None else _row_stride(residual, "residual", T, H)
     _lib.expect(post_weight, "post_weight", dtype=torch.float32, shape=(H,), optional=True)
     if post_weight is not None and post_weight.data_ptr() % 16:
         raise ValueError("post_weight must be 16-byte aligned")
@@ -351,12 +355,11 @@ def _sandwich_checked(hidden, residual, mul, add, eps, post_norm, post_weight, g
                      what="adaln_sandwich")
     dev = hidden.device
     # rows of no request are zeros in what is allocated here; with one output given, the other is cleared up front
-    both = (out is None) == (residual_out is None)
-    make = torch.empty if both or request_ids is None else torch.zeros
-    zero_rest = out is None and residual_out is None
+    zero_rest = residual_out is None and (out is None or not form)
+    make = torch.empty if zero_rest or request_ids is None or (out is not None and residual_out is not None) else torch.zeros
     if residual_out is None:
         residual_out = make((T, H), dtype=torch.bfloat16, device=dev)
-    if out is None:
+    if out is None and form:
         if quant == "none":
             codes = make((T, H), dtype=torch.bfloat16, device=dev)
         else:
@@ -365,7 +368,7 @@ def _sandwich_checked(hidden, residual, mul, add, eps, post_norm, post_weight, g
     p = _lib.ptr
     _lib.call("wanmi_adaln_sandwich", hidden.get_device(), p(hidden), ld_h, p(residual), ld_r, p(post_weight), p(gate), ld_gate, p(mul), ld_mul,
               p(add), ld_add, p(request_ids), 2**31 - 1 if requests is None else requests, float(residual_scale), T, H,
-              float(eps), _lib.NORM[post_norm], _lib.NORM[norm_type], _lib.QUANT[quant], int(zero_rest), p(residual_out),
+              float(eps), _lib.NORM[post_norm], _lib.NORM[norm_type if form else "none"], _lib.QUANT[quant], int(zero_rest), p(residual_out),
               p(codes), p(scales))
     return residual_out, MXTensor(codes, scales) if quant == "mx" else codes
 

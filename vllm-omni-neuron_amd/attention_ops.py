@@ -173,7 +173,7 @@ def _separate(t: torch.Tensor, name: str) -> None:
         reach = s * n
 
 
-def qk_norm_rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, *, axes=(44, 42, 42),
+def qk_norm_rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor | None, *, axes=(44, 42, 42),
                       theta=10000.0, rope_pairs: str = "interleaved", norm: str = "none",
                       q_gamma: torch.Tensor | None = None, k_gamma: torch.Tensor | None = None, eps: float = 1e-6,
                       request_ids: torch.Tensor | None = None, requests: int | None = None, want_max: bool = False,
@@ -257,8 +257,8 @@ def _qk_axes_checked(q, k, positions, axes, theta, rope_pairs, norm, q_gamma, k_
     if D not in (32, 64, 128, 256):
         raise NotImplementedError(f"head_dim {D}: 32, 64, 128 and 256 are served")
     axes = tuple(int(d) for d in axes)
-    if not 1 <= len(axes) <= 8 or any(d < 0 or d % 2 for d in axes) or sum(axes) > D:
-        raise ValueError(f"axes {axes}: 1 to 8 even channel counts of at most {D} in all")
+    if len(axes) > 8 or any(d < 0 or d % 2 for d in axes) or sum(axes) > D:
+        raise ValueError(f"axes {axes}: at most 8 even channel counts of at most {D} in all")
     if sum(axes) % 16:
         raise NotImplementedError(f"axes {axes} turn {sum(axes)} channels: a multiple of 16 is served")
     theta = tuple(float(t) for t in theta) if isinstance(theta, (tuple, list)) else (float(theta),) * len(axes)
@@ -296,9 +296,11 @@ def _qk_axes_checked(q, k, positions, axes, theta, rope_pairs, norm, q_gamma, k_
             if name == "k" and out.data_ptr() == q.data_ptr() and out.numel():
                 raise ValueError("k_out may not be q")
         views.append((ts, hs, heads, ots, ohs))
-    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.float32):
-        raise ValueError("positions must be an int32 or float32 tensor")
-    _lib.expect(positions, "positions", dtype=positions.dtype, shape=(T, len(axes)))
+    if axes or positions is not None:
+        if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.float32):
+            raise ValueError("positions must be an int32 or float32 tensor")
+        _lib.expect(positions, "positions", dtype=positions.dtype, shape=(T, len(axes)))
+    floats = positions is not None and positions.dtype is torch.float32
     _lib.request_rows(request_ids, T)
     if want_max and (k is None or (request_ids is not None and requests is None)):
         raise ValueError("want_max needs k, and with request_ids the number of requests")
@@ -326,7 +328,7 @@ def _qk_axes_checked(q, k, positions, axes, theta, rope_pairs, norm, q_gamma, k_
     dims, freqs = _axis_arrays(axes, theta)
     (qts, qhs, qh, qots, qohs), (kts, khs, kh, kots, kohs) = views
     _lib.call("wanmi_qk_norm_rope_axes", q.get_device(), p(q), qts, qhs, qh, p(q_gamma), p(outs[0]), qots, qohs, p(k), kts, khs, kh, p(k_gamma),
-              p(outs[1]), kots, kohs, T, D, p(positions), int(positions.dtype == torch.float32), len(axes), dims, freqs,
+              p(outs[1]), kots, kohs, T, D, p(positions), int(floats), len(axes), dims, freqs,
               _ROTATE[rope_pairs], _QK_NORM[norm], float(eps), p(request_ids), n, int(zero_rest), p(kmax))
     return (*outs, kmax) if want_max else tuple(outs)
 

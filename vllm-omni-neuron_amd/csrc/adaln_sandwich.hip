@@ -1,8 +1,8 @@
 // Norms before and after a sub-layer, fused with its gate and residual scale, for packed batches (gfx950).
 //
 //   p = Norm_post(hidden) * post_weight                        (fp32)
-//   r = bf16(alpha * residual + gate[q] * p)                   the carried residual, written
-//   y = bf16(Norm_pre(r) * mul[q] + add[q])                    written as it is, as MX or as ROW codes
+//   r = bf16(alpha * residual + gate[q] * p)                   the carried residual, written (residual optional)
+//   y = bf16(Norm_pre(r) * mul[q] + add[q])                    written as it is, as MX or as ROW codes, or not wanted
 //
 // for every row of a packed [T, H] batch, q the row's request: gate, mul and add are one row of H
 // for all requests or one per request. A row whose id names no request is not computed: it is left as it
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
     for (int c = 0; c < kNC; ++c) {
       hn[c] = ok[c] ? *reinterpret_cast<const u32x4*>(a.hidden + row * a.ld_h + col[c]) : zero;
-      rn[c] = ok[c] ? *reinterpret_cast<const u32x4*>(a.residual + row * a.ld_r + col[c]) : zero;
+      rn[c] = ok[c] && a.residual ? *reinterpret_cast<const u32x4*>(a.residual + row * a.ld_r + col[c]) : zero;
     }
   };
   // the requests of the rows, 64 at a time (one a lane), so that a row's fetch does not wait for its id
@@ -208,7 +208,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((amdgpu_waves_per_eu(
         for (int c = 0; c < kNC; ++c) {
           if (!ok[c]) continue;
           store_b128_guarded(zero, ro + col[c]);
-          if (a.quant == WANMI_QUANT_NONE) {
+          if (!a.out) {
+          } else if (a.quant == WANMI_QUANT_NONE) {
             store_b128_guarded(zero, out + 2 * col[c]);
           } else if (a.quant == WANMI_QUANT_MX) {
             *reinterpret_cast<u32x2*>(out + col[c]) = u32x2{0u, 0u};
@@ -218,7 +219,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((amdgpu_waves_per_eu(
             reinterpret_cast<uint32_t*>(out + col[c])[1] = 0u;
           }
         }
-        if (a.quant == WANMI_QUANT_ROW && tid == 0) *reinterpret_cast<uint32_t*>(out + H) = 0u;
+        if (a.out && a.quant == WANMI_QUANT_ROW && tid == 0) *reinterpret_cast<uint32_t*>(out + H) = 0u;
       }
       id = next;
       if ((uint32_t)id < (uint32_t)a.requests) fetch(row + 1);
@@ -254,6 +255,11 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((amdgpu_waves_per_eu(
         x[c][2 * j + 1] = ok[c] ? bf16_hi(r[c][j]) : 0.0f;
       }
       if (ok[c]) store_b128_guarded(r[c], ro + col[c]);
+    }
+    if (!a.out) {  // (the same for the whole workgroup)
+      id = next;
+      par ^= 1;
+      continue;
     }
     row_stats<kNC>(x, ok, a.norm, (float)H, a.eps, wave, mine, theirs, part[par][1], mu, rs);
     float amax = 0.0f;
@@ -370,7 +376,7 @@ __global__ __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_per_eu
   constexpr int kAhead = NCH <= 6 ? NCH : 4;  // chunks of the residual under way (all of it where the registers hold it)
   uint32_t xp[NCH][4], rp[kAhead][4];
   const __amdgpu_buffer_rsrc_t r_x = rsrc(a.hidden + from * a.ld_h, 2 * (int64_t)H);
-  const __amdgpu_buffer_rsrc_t r_r = rsrc(a.residual + from * a.ld_r, 2 * (int64_t)H);
+  const __amdgpu_buffer_rsrc_t r_r = rsrc(a.residual ? a.residual + from * a.ld_r : a.hidden + from * a.ld_h, 2 * (int64_t)H);
   // columns past H in the last chunk lie past the descriptors' extents and read as zero
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
@@ -409,13 +415,14 @@ __global__ __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_per_eu
   uint8_t* out = reinterpret_cast<uint8_t*>(a.out) + row * out_bytes;
   const __amdgpu_buffer_rsrc_t r_ro = rsrc(a.residual_out + row * H, 2 * (int64_t)H);
   const __amdgpu_buffer_rsrc_t r_o = rsrc(out, a.quant == WANMI_QUANT_ROW ? (int64_t)H : out_bytes);
-  const __amdgpu_buffer_rsrc_t r_s = rsrc(a.quant == WANMI_QUANT_MX ? a.scales + row * (int64_t)(H / 32) : nullptr,
+  const __amdgpu_buffer_rsrc_t r_s = rsrc(a.quant == WANMI_QUANT_MX && a.out ? a.scales + row * (int64_t)(H / 32) : nullptr,
                                           a.quant == WANMI_QUANT_MX ? H / 32 : 0);
   if (!live) {
     if (!a.zero_rest) return;
     for (int c = 0; c < nch; ++c) {
       store_b128_guarded(zero, r_ro, lane * 16, c * 1024);
-      if (a.quant == WANMI_QUANT_NONE) {
+      if (!a.out) {
+      } else if (a.quant == WANMI_QUANT_NONE) {
         store_b128_guarded(zero, r_o, lane * 16, c * 1024);
       } else {
         __builtin_amdgcn_raw_buffer_store_b64(u32x2{0u, 0u}, r_o, lane * 8, c * 512, 0);
@@ -423,7 +430,7 @@ __global__ __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_per_eu
           __builtin_amdgcn_raw_buffer_store_b8((uint8_t)0, r_s, (lane & 3) == 0 ? c * 16 + (lane >> 2) : H, 0, 0);
       }
     }
-    if (a.quant == WANMI_QUANT_ROW && lane == 0) *reinterpret_cast<uint32_t*>(out + H) = 0u;
+    if (a.out && a.quant == WANMI_QUANT_ROW && lane == 0) *reinterpret_cast<uint32_t*>(out + H) = 0u;
     return;
   }
   // (the whole row in one piece of straight code for either place of the vectors)
@@ -459,7 +466,8 @@ __global__ __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float p0 = (bf16_lo(xp[c][j]) - mu) * rs * wv[2 * j], p1 = (bf16_hi(xp[c][j]) - mu) * rs * wv[2 * j + 1];
-        o[j] = pack_bf16x2(a.alpha * bf16_lo(rp[c % kAhead][j]) + gv[2 * j] * p0, a.alpha * bf16_hi(rp[c % kAhead][j]) + gv[2 * j + 1] * p1);
+        o[j] = pack_bf16x2((a.residual ? a.alpha * bf16_lo(rp[c % kAhead][j]) : 0.0f) + gv[2 * j] * p0,
+                             (a.residual ? a.alpha * bf16_hi(rp[c % kAhead][j]) : 0.0f) + gv[2 * j + 1] * p1);
         if (c == NCH - 1 && !inside) o[j] = 0u;
       }
 #pragma unroll
@@ -471,6 +479,7 @@ __global__ __launch_bounds__(64 * kManyWaves) __attribute__((amdgpu_waves_per_eu
       }
       store_b128_guarded(o, r_ro, lane * 16, c * 1024);
     }
+    if (!a.out) return;
     wave_stats<NCH>(x, packed, a.norm, inside, (float)H, a.eps, mu, rs);
     float amax = 0.0f;
 #pragma unroll
@@ -565,10 +574,9 @@ extern "C" int wanmi_adaln_sandwich(const void* hidden, int64_t ld_hidden, const
                 (long long)requests);
   WANMI_REQUIRE(request_ids || requests >= 1 || T == 0, WANMI_ERR_ARG, "wanmi_adaln_sandwich: no request to give the rows to");
   if (T == 0) return WANMI_OK;
-  WANMI_REQUIRE(hidden && residual && residual_out && out, WANMI_ERR_ARG,
-                "wanmi_adaln_sandwich: hidden, residual, residual_out and out must not be null");
-  WANMI_REQUIRE(quant_type != WANMI_QUANT_MX || scales, WANMI_ERR_ARG, "wanmi_adaln_sandwich: MX output needs scales");
-  for (int64_t ld : {ld_hidden, ld_residual})
+  WANMI_REQUIRE(hidden && residual_out, WANMI_ERR_ARG, "wanmi_adaln_sandwich: hidden and residual_out must not be null");
+  WANMI_REQUIRE(!out || quant_type != WANMI_QUANT_MX || scales, WANMI_ERR_ARG, "wanmi_adaln_sandwich: MX output needs scales");
+  for (int64_t ld : {ld_hidden, residual ? ld_residual : ld_hidden})
     WANMI_REQUIRE(ld >= H && ld % 8 == 0, WANMI_ERR_ARG,
                   "wanmi_adaln_sandwich: row strides must be multiples of 8 of at least H, got %lld", (long long)ld);
   for (int64_t ld : {gate ? ld_gate : 0, mul ? ld_mul : 0, add ? ld_add : 0})

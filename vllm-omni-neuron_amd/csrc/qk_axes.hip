@@ -337,7 +337,7 @@ extern "C" int wanmi_qk_norm_rope_axes(const void* q, int64_t q_token_stride, in
   WANMI_REQUIRE(norm == WANMI_QKNORM_NONE || norm == WANMI_QKNORM_PER_HEAD || norm == WANMI_QKNORM_ACROSS_HEADS,
                 WANMI_ERR_ARG, "%s: unknown norm %d", f, norm);
   WANMI_REQUIRE(eps >= 0.0f, WANMI_ERR_ARG, "%s: eps must be >= 0", f);
-  WANMI_REQUIRE(axes >= 1 && axes <= 8 && axis_dims && freqs, WANMI_ERR_ARG, "%s: 1 to 8 axes with their widths and frequencies", f);
+  WANMI_REQUIRE(axes >= 0 && axes <= 8 && (!axes || (axis_dims && freqs)), WANMI_ERR_ARG, "%s: at most 8 axes with their widths and frequencies", f);
   WANMI_REQUIRE(requests >= 0 && requests < (1LL << 31), WANMI_ERR_ARG, "%s: requests=%lld out of range", f, (long long)requests);
   WANMI_REQUIRE(request_ids || requests >= 1 || T == 0, WANMI_ERR_ARG, "%s: no request to give the rows to", f);
   QKAxesArgs a;
@@ -363,7 +363,7 @@ extern "C" int wanmi_qk_norm_rope_axes(const void* q, int64_t q_token_stride, in
     if (st != WANMI_OK) return st;
   }
   if (T == 0) return WANMI_OK;
-  WANMI_REQUIRE(q && positions && q_out && (!k_heads || (k && k_out)), WANMI_ERR_ARG, "%s: null pointer", f);
+  WANMI_REQUIRE(q && (positions || !rot) && q_out && (!k_heads || (k && k_out)), WANMI_ERR_ARG, "%s: null pointer", f);
   const int64_t strides[8] = {q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride,
                               k_heads ? k_token_stride : 0, k_heads ? k_head_stride : 0, k_heads ? k_out_token_stride : 0,
                               k_heads ? k_out_head_stride : 0};

@@ -201,7 +201,8 @@ __global__ __launch_bounds__(256) void lora_shrink_few_kernel(LoraArgs a) {
 // slot p ^ (i & 7) of the row, so that the eight rows that are read together take different banks. The MX
 // scales come with x, four bytes per row.
 // Where requests meet inside a tile, each adapter takes a sweep over K of its own, in which the waves without rows
-// of it only load.
+// of it only load. The sweeps are shared out over two workgroups (slots; the second one ends at once where a tile
+// has one adapter), so that they run side by side where the chip has room: QKV of 7799 rows in 5 requests.
 template <bool kMx, int kNR>
 struct Big {
   static constexpr int kWaves = kNR == 128 ? 8 : 4;
@@ -228,7 +229,8 @@ __global__ __launch_bounds__(kNR == 128 ? 512 : 256, 2) void lora_shrink_kernel(
   const int nranks = min(kNR, a.R - rank0);
   const int m0 = (kNR == 128 ? wave >> 1 : wave) * 16 * P::kMT;  // the wave's first row and rank
   const int r0 = kNR == 128 ? (wave & 1) * 64 : 0;
-  const int ch0 = blockIdx.z * a.chunks_per_split, n = min(a.chunks_per_split, a.K / 64 - ch0);  // (even for MX)
+  const int split = blockIdx.z % a.splits, slot = blockIdx.z / a.splits;
+  const int ch0 = split * a.chunks_per_split, n = min(a.chunks_per_split, a.K / 64 - ch0);  // (even for MX)
 
   int v[P::kRows / 64];  // the tile's adapters
 #pragma unroll
@@ -261,11 +263,12 @@ __global__ __launch_bounds__(kNR == 128 ? 512 : 256, 2) void lora_shrink_kernel(
   const uint8_t* sr = lds + kSAt + (m0 + c) * 4 + (g >> 1);
 
   int e = -1;
-  while (true) {
+  for (int at = 0;; ++at) {
     int next = next_adapter(v[0], v[1], e);
     if (P::kRows > 128) next = min(next, next_adapter(v[P::kRows / 64 - 2], v[P::kRows / 64 - 1], e));
     e = next;
     if (e == 0x7FFFFFFF) break;
+    if (at % a.slots != slot) continue;
     uint64_t here = 0;
 #pragma unroll
     for (int i = 0; i < P::kRows / 64; ++i) {
@@ -357,7 +360,7 @@ __global__ __launch_bounds__(kNR == 128 ? 512 : 256, 2) void lora_shrink_kernel(
 #pragma unroll
       for (int rt = 0; rt < P::kRT; ++rt) {
         const int rank = r0 + 16 * rt + 4 * g;
-        if (rank < nranks) *reinterpret_cast<f32x4*>(a.u + ((int64_t)blockIdx.z * a.T + t) * a.R + rank0 + rank) = acc[m][rt] * f;
+        if (rank < nranks) *reinterpret_cast<f32x4*>(a.u + ((int64_t)split * a.T + t) * a.R + rank0 + rank) = acc[m][rt] * f;
       }
     }
   }
@@ -566,34 +569,60 @@ __global__ __launch_bounds__(256, 2) void lora_expand_many_kernel(LoraArgs a) {
   const int n = (min(a.span, pend - col0) + 63) / 64;
 
   const int v0 = row_adapter(a, t0 + lane), v1 = row_adapter(a, t0 + 64 + lane);
-  // u of the wave's rows (two groups of 16) as the MFMA's operand: high and low halves
+  int e = next_adapter(v0, v1, -1);
+  // u of the wave's rows (two groups of 16) as the MFMA's operand: high and low halves. The splits of K are added two at a time
+  // with all of their loads under way (one by one, each a memory latency, ten splits took half of a call of 4096 rows).
   bf16x8 uh[2][kKS], ul[2][kKS];
+  {
+    float f[2][kKS][8];
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    const int64_t t = min(t0 + 32 * wave + 16 * m + c, a.T - 1);  // (rows without an adapter: whatever lies there, not used)
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int k = 0; k < kKS; ++k) {
-      float f[8];
+      for (int k = 0; k < kKS; ++k)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = 0.0f;
-      if (32 * k + 8 * g < a.r) {
-        const float* pu = a.u + t * a.R + part * a.r + 32 * k + 8 * g;
-        for (int q = 0; q < a.splits; ++q, pu += a.T * a.R) {
-          const f32x4 lo = *reinterpret_cast<const f32x4*>(pu), hi = *reinterpret_cast<const f32x4*>(pu + 4);
+        for (int j = 0; j < 8; ++j) f[m][k][j] = 0.0f;
+    const float* pu[2];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) f[j] += lo[j], f[4 + j] += hi[j];
-        }
-      }
-      u32x4 h, l;
+    for (int m = 0; m < 2; ++m)  // (rows without an adapter: whatever lies there, not used)
+      pu[m] = a.u + min(t0 + 32 * wave + 16 * m + c, a.T - 1) * a.R + part * a.r + 8 * g;
+    for (int q = 0; q < a.splits; q += 2) {
+      f32x4 w[2][2][kKS][2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        h[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
-        const float h0 = bf16_lo(h[j]), h1 = bf16_hi(h[j]);
-        l[j] = pack_bf16x2(fabsf(h0) < INFINITY ? f[2 * j] - h0 : 0.0f, fabsf(h1) < INFINITY ? f[2 * j + 1] - h1 : 0.0f);
-      }
-      uh[m][k] = __builtin_bit_cast(bf16x8, h);
-      ul[m][k] = __builtin_bit_cast(bf16x8, l);
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int k = 0; k < kKS; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              w[h][m][k][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+              if (q + h < a.splits && 32 * k + 8 * g < a.r)
+                w[h][m][k][i] = *reinterpret_cast<const f32x4*>(pu[m] + (q + h) * a.T * a.R + 32 * k + 4 * i);
+            }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int k = 0; k < kKS; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[m][k][j] += w[h][m][k][j >> 2][j & 3];
     }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int k = 0; k < kKS; ++k) {
+        u32x4 h, l;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = f[m][k][2 * j], y = f[m][k][2 * j + 1];
+          h[j] = pack_bf16x2(x, y);
+          const float h0 = bf16_lo(h[j]), h1 = bf16_hi(h[j]);
+          l[j] = pack_bf16x2(fabsf(h0) < INFINITY ? x - h0 : 0.0f, fabsf(h1) < INFINITY ? y - h1 : 0.0f);
+        }
+        uh[m][k] = __builtin_bit_cast(bf16x8, h);
+        ul[m][k] = __builtin_bit_cast(bf16x8, l);
+      }
   }
 
   // the rows that this lane loads and stores: 16 m + 8 h + lane / 8 of the wave's, columns 8 (lane & 7) .. + 7
@@ -618,7 +647,6 @@ __global__ __launch_bounds__(256, 2) void lora_expand_many_kernel(LoraArgs a) {
   float* piece = reinterpret_cast<float*>(lds + P::kStages * P::kB) + wave * 16 * P::kRow;
   const auto swizzle = [](int row) { return kKS == 1 ? (row >> 1) & 3 : row & (kPieces - 1); };
 
-  int e = next_adapter(v0, v1, -1);
   for (int at = 0; at == 0 || e != 0x7FFFFFFF; ++at, e = next_adapter(v0, v1, e)) {
     const bool product = e != 0x7FFFFFFF;
     bool take[4], any = false;
@@ -739,6 +767,7 @@ LoraPlan lora_plan(int64_t T, int64_t K, int64_t R, int64_t adapters, bool plain
     const int64_t per = (pairs + n - 1) / n;
     p.splits = (int)((pairs + per - 1) / per);
     p.chunks_per_split = (int)(2 * per);
+    p.slots = adapters > 1 ? 2 : 1;
     return p;
   }
   const int64_t wgs = (T + kRows - 1) / kRows * ((R + 16 * kRankTiles - 1) / (16 * kRankTiles));
@@ -776,7 +805,7 @@ template <bool kMx, int kNR>
 int launch_big(const LoraArgs& a, hipStream_t s) {
   using P = Big<kMx, kNR>;
   WANMI_REQUIRE(lds_limit(&lora_shrink_kernel<kMx, kNR>, P::kLds), WANMI_ERR_HIP, "wanmi_lora_add: %d bytes of LDS refused", P::kLds);
-  const dim3 grid((unsigned)((a.T + P::kRows - 1) / P::kRows), (unsigned)((a.R + kNR - 1) / kNR), (unsigned)a.splits);
+  const dim3 grid((unsigned)((a.T + P::kRows - 1) / P::kRows), (unsigned)((a.R + kNR - 1) / kNR), (unsigned)(a.splits * a.slots));
   hipLaunchKernelGGL((lora_shrink_kernel<kMx, kNR>), grid, dim3(64 * P::kWaves), P::kLds, s, a);
   return check_launch("wanmi_lora_add");
 }

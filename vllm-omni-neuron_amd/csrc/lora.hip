@@ -70,7 +70,6 @@ __device__ __forceinline__ int row_adapter(const LoraArgs& a, int64_t t) {
   return (uint32_t)e < (uint32_t)a.adapters ? e : -1;
 }
 
-
 // The smallest adapter above `prev` among the rows of a tile (v0, v1: the lane's rows'), INT_MAX if there is none.
 __device__ __forceinline__ int next_adapter(int v0, int v1, int prev) {
   int v = min(v0 > prev ? v0 : 0x7FFFFFFF, v1 > prev ? v1 : 0x7FFFFFFF);
@@ -193,16 +192,19 @@ __global__ __launch_bounds__(256) void lora_shrink_few_kernel(LoraArgs a) {
 // shrink, many rows: 256 rows x 128 ranks a workgroup of eight waves, or 128 rows x 64 or 32 ranks of four
 // ------------------------------------------------------------------------------------------------
 // Both operands pass through LDS, loaded straight into it (16-byte pieces, whole 128-byte runs of a row per
-// eight lanes), in rings of three: A by steps of 64 k, x by 128 bytes of a row (64 k, or 128 of MX codes: in runs
-// of 64 bytes each line was fetched from memory in two requests, and 128 rows x 32 ranks of K = 5120 took 57.6 us at
-// 32768 rows). x is read once per kNR ranks and A once per tile of rows. A wave's tile is 64 rows x 64 ranks at
-// kNR = 128, where its operand reads from LDS take less time than its MFMAs, and 32 rows x kNR ranks below,
-// where x is what there is to read and two workgroups a CU keep more of it under way. Piece p of row i lies in
-// slot p ^ (i & 7) of the row, so that the eight rows that are read together take different banks. The MX
-// scales come with x, four bytes per row.
+// eight lanes), in rings of three: A by steps of 64 k, x by 128 bytes of a row (64 k, or 128 of MX codes). x is read
+// once per kNR ranks and A once per tile of rows. A wave's tile is 64 rows x 64 ranks at kNR = 128, where its operand
+// reads from LDS take less time than its MFMAs, and 32 rows x kNR ranks below, where x is what there is to read and
+// two workgroups a CU keep more of it under way. Piece p of row i lies in slot p ^ (i & 7) of the row, so that the
+// eight rows that are read together take different banks. The MX scales come with x, four bytes per row.
+// 32768 rows of one request, MX: K = 5120, 32 ranks 58 us and 64 ranks 63 (x alone at 5.5 TB/s: 32; 64 rows of x at
+// a time come in runs of 128 bytes, and neither longer runs nor another order of k brought more than 3 TB/s), K =
+// 13824, 128 ranks 154 (753 TFLOP/s).
 // Where requests meet inside a tile, each adapter takes a sweep over K of its own, in which the waves without rows
 // of it only load. The sweeps are shared out over two workgroups (slots; the second one ends at once where a tile
-// has one adapter), so that they run side by side where the chip has room: QKV of 7799 rows in 5 requests.
+// has one adapter), so that they run side by side where the chip has room: QKV of 7799 rows in 5 requests, 4
+// adapters, rank 64: 42 us, one workgroup for all of a tile's sweeps 56; K = 13824, 32760 rows in 3 requests, rank 128: 141
+// and 230.
 template <bool kMx, int kNR>
 struct Big {
   static constexpr int kWaves = kNR == 128 ? 8 : 4;
@@ -571,7 +573,7 @@ __global__ __launch_bounds__(256, 2) void lora_expand_many_kernel(LoraArgs a) {
   const int v0 = row_adapter(a, t0 + lane), v1 = row_adapter(a, t0 + 64 + lane);
   int e = next_adapter(v0, v1, -1);
   // u of the wave's rows (two groups of 16) as the MFMA's operand: high and low halves. The splits of K are added two at a time
-  // with all of their loads under way (one by one, each a memory latency, ten splits took half of a call of 4096 rows).
+  // with all of their loads under way (one by one, each a memory latency, 4096 rows x 5120 columns of ten splits took 38 us instead of 32).
   bf16x8 uh[2][kKS], ul[2][kKS];
   {
     float f[2][kKS][8];

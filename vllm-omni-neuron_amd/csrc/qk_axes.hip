@@ -13,8 +13,8 @@
 // of at most pi/4 by their power series, whose next terms are below 2e-9 and 3e-8.
 //
 // One wavefront owns a row of Q or of K, and a workgroup of eight rows shares the weight of the norm across heads in LDS (fp32,
-// it is as many bytes as the row is read and written: from L2 for every row, 32760 rows of 40 + 40 heads took
-// 283 us). A wave takes one row and ends: the loads of a next one would stand behind the stores of this one in
+// it is as many bytes as the row is read and written). 32760 rows of 40 + 40 heads of 128: 258 us, 5.2 of the 5.5 TB/s
+// of a large copy; with the weight from L2 for every row 283. A wave takes one row and ends: the loads of a next one would stand behind the stores of this one in
 // the order that a wave waits for them.
 //
 // A lane holds runs of 8 channels (16 bytes), neighbouring lanes neighbouring runs, so that every instruction moves whole
@@ -25,7 +25,8 @@
 //
 // The largest norm of a request's K rows: the workgroup's largest is compared with what is there already and
 // exchanged only if it is larger, since atomics on these few addresses are served one after another for all the
-// XCDs (a maximum does not depend on their order).
+// XCDs (a maximum does not depend on their order): 70 us without, 84 with it at 7800 rows of 40 + 40 heads, and 99 with four
+// rows a workgroup; 260 and 264 at 32760.
 #include "wanmi_common.h"
 
 namespace wanmi {
@@ -87,12 +88,12 @@ __device__ __forceinline__ void raise_max(float* at, float n) {
   if (bits > __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(p, bits);
 }
 
-constexpr int kRowWaves = 8;
-
-// NU: units of 16 channels per lane, heads * D / 16 / 64 rounded up; kWhole: every lane has all of them.
-template <int NU, bool kHalves, bool kWhole>
-__global__ __launch_bounds__(64 * kRowWaves) __attribute__((amdgpu_waves_per_eu(NU <= 3 || (NU <= 5 && (kWhole || !kHalves)) ? 4 : 2))) void qk_axes_kernel(QKAxesArgs a) {
+// NU: units of 16 channels per lane, heads * D / 16 / 64 rounded up; kWhole: every lane has all of them. kAlone: the
+// rows share neither a weight nor maxima.
+template <int NU, bool kHalves, bool kWhole, bool kAlone>
+__global__ __launch_bounds__(kAlone ? 256 : 512) __attribute__((amdgpu_waves_per_eu(kAlone ? (NU == 2 && kHalves && kWhole ? 5 : 6) : NU <= 3 || (NU <= 5 && (kWhole || !kHalves)) ? 4 : 2))) void qk_axes_kernel(QKAxesArgs a) {
   extern __shared__ __attribute__((aligned(1024))) float gam[];  // [run slot][half][lane] x 4 floats; then the heads' maxima
+  constexpr int kRowWaves = kAlone ? 4 : 8;
   __shared__ float tab[kRowWaves][2][kMaxPairs];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -110,6 +111,7 @@ __global__ __launch_bounds__(64 * kRowWaves) __attribute__((amdgpu_waves_per_eu(
   const auto chan = [&](int i) { return kHalves && (i & 1) ? c1 : c0; };
   const auto head = [&](int i) { return h0 + (kHalves ? i >> 1 : i) * step; };
   const auto has = [&](int i) { return kWhole || head(i) < p.heads; };
+  const auto past = [&](int i) { return !kWhole && (kHalves ? i >> 1 : i) * step >= p.heads; };  // no lane has run i (few heads beside many)
 
   const int64_t from = min(row, a.T - 1);  // (the loads do not wait to know whether the row has a request)
   u32x4 x[kRuns];
@@ -132,7 +134,7 @@ __global__ __launch_bounds__(64 * kRowWaves) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
       for (int j = 0; j < 8; ++j) own[r][j] = p.gamma ? p.gamma[chan(r) + j] : 1.0f;
   }
-  const bool across = a.norm == WANMI_QKNORM_ACROSS_HEADS && p.gamma;
+  const bool across = !kAlone && a.norm == WANMI_QKNORM_ACROSS_HEADS && p.gamma;
   if (across) {
     const u32x4 rg = buffer_rsrc(p.gamma, 4u * (uint32_t)(p.heads * D));  // heads past the end: zeros, not used
     const uint32_t base = lds_addr(gam);
@@ -142,7 +144,7 @@ __global__ __launch_bounds__(64 * kRowWaves) __attribute__((amdgpu_waves_per_eu(
         lds_dma_b128(rg, (uint32_t)((head(k >> 1) * D + chan(k >> 1) + 4 * (k & 1)) * 4), base + k * 1024);
   }
   float* maxima = gam + (a.norm == WANMI_QKNORM_ACROSS_HEADS ? 2 * kRuns * 256 : 0);
-  const bool bound = a.kmax && blockIdx.y == 1;
+  const bool bound = !kAlone && a.kmax && blockIdx.y == 1;
   if (bound)
     for (int h = threadIdx.x; h < p.heads; h += 64 * kRowWaves) maxima[h] = 0.0f;
   float* tc = tab[wave][0];
@@ -196,6 +198,7 @@ __global__ __launch_bounds__(64 * kRowWaves) __attribute__((amdgpu_waves_per_eu(
     }
 #pragma unroll
     for (int i = 0; i < kRuns; i += kHalves ? 2 : 1) {
+      if (past(i)) break;
       constexpr int kN = kHalves ? 2 : 1;  // runs taken together
       float v[kN][8];
 #pragma unroll
@@ -282,36 +285,42 @@ __global__ __launch_bounds__(256) void qk_axes_zero_kernel(float* p, int64_t n) 
 }
 
 // One instantiation for Q and K: the larger part's.
-template <int NU, bool kHalves>
+template <int NU, bool kHalves, bool kAlone>
 void launch_qk_axes(const QKAxesArgs& a, hipStream_t s) {
+  constexpr int kRowWaves = kAlone ? 4 : 8;
   const dim3 grid((unsigned)((a.T + kRowWaves - 1) / kRowWaves), a.part[1].heads ? 2u : 1u);
   const int per_head = 1 << a.unit_shift;
   const bool whole = a.part[0].heads * per_head == 64 * NU && (!a.part[1].heads || a.part[1].heads * per_head == 64 * NU);
-  const int bytes = (a.norm == WANMI_QKNORM_ACROSS_HEADS ? 4096 * NU : 0) + (a.kmax ? 4 * a.part[1].heads : 0);
+  const int bytes = kAlone ? 0 : (a.norm == WANMI_QKNORM_ACROSS_HEADS ? 4096 * NU : 0) + (a.kmax ? 4 * a.part[1].heads : 0);
   // (16 units, more than 8192 channels: past the 64 KB that a launch has by itself, with the angles)
   if (NU == 16) {
     static int allowed[64] = {0};
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64 || !allowed[dev]) {
-      for (const void* f : {reinterpret_cast<const void*>(&qk_axes_kernel<NU, kHalves, true>), reinterpret_cast<const void*>(&qk_axes_kernel<NU, kHalves, false>)})
+      for (const void* f : {reinterpret_cast<const void*>(&qk_axes_kernel<NU, kHalves, true, kAlone>), reinterpret_cast<const void*>(&qk_axes_kernel<NU, kHalves, false, kAlone>)})
         if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024) != hipSuccess) return;  // (the error is the launch's)
       if (dev >= 0 && dev < 64) allowed[dev] = 1;
     }
   }
-  if (whole) hipLaunchKernelGGL((qk_axes_kernel<NU, kHalves, true>), grid, dim3(64 * kRowWaves), bytes, s, a);
-  else hipLaunchKernelGGL((qk_axes_kernel<NU, kHalves, false>), grid, dim3(64 * kRowWaves), bytes, s, a);
+  if (whole) hipLaunchKernelGGL((qk_axes_kernel<NU, kHalves, true, kAlone>), grid, dim3(64 * kRowWaves), bytes, s, a);
+  else hipLaunchKernelGGL((qk_axes_kernel<NU, kHalves, false, kAlone>), grid, dim3(64 * kRowWaves), bytes, s, a);
 }
 
 template <bool kHalves>
 void launch_qk_axes(const QKAxesArgs& a, int nu, hipStream_t s) {
-  if (nu <= 1) launch_qk_axes<1, kHalves>(a, s);
-  else if (nu <= 2) launch_qk_axes<2, kHalves>(a, s);
-  else if (nu <= 3) launch_qk_axes<3, kHalves>(a, s);
-  else if (nu <= 4) launch_qk_axes<4, kHalves>(a, s);
-  else if (nu <= 5) launch_qk_axes<5, kHalves>(a, s);
-  else if (nu <= 6) launch_qk_axes<6, kHalves>(a, s);
-  else if (nu <= 8) launch_qk_axes<8, kHalves>(a, s);
-  else launch_qk_axes<16, kHalves>(a, s);
+  // Short rows that share nothing: many small workgroups (7799 rows of 32 + 4 heads of 64,
+  // halves: 22.7 us; as eight rows a workgroup in the kernel that can share, with its registers, 25.9).
+  const bool alone = !a.kmax && (a.norm != WANMI_QKNORM_ACROSS_HEADS || (!a.part[0].gamma && !a.part[1].gamma));
+  if (nu <= 1 && alone) launch_qk_axes<1, kHalves, true>(a, s);
+  else if (nu <= 2 && alone) launch_qk_axes<2, kHalves, true>(a, s);
+  else if (nu <= 1) launch_qk_axes<1, kHalves, false>(a, s);
+  else if (nu <= 2) launch_qk_axes<2, kHalves, false>(a, s);
+  else if (nu <= 3) launch_qk_axes<3, kHalves, false>(a, s);
+  else if (nu <= 4) launch_qk_axes<4, kHalves, false>(a, s);
+  else if (nu <= 5) launch_qk_axes<5, kHalves, false>(a, s);
+  else if (nu <= 6) launch_qk_axes<6, kHalves, false>(a, s);
+  else if (nu <= 8) launch_qk_axes<8, kHalves, false>(a, s);
+  else launch_qk_axes<16, kHalves, false>(a, s);
 }
 
 }  // namespace

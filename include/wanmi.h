@@ -362,7 +362,7 @@ int wanmi_dmajor_to_mx(const void* x, int64_t B, int heads, int64_t S, int64_t b
  * fp32 [H]; gate, mul, add fp32: one row of H per request, ld_* elements apart (multiples of 4), or ld_* 0: one
  * row for every request; out and scales as wanmi_adaln_quant's. q = request_ids[t] (int32; NULL: every row is request 0). A row whose id is not in
  * [0, requests) is not computed; its outputs are left as they are, or zeroed with zero_rest. residual_out may
- * be `residual`, out `hidden`, row for row. H as for wanmi_adaln_quant. Both norms use eps.
+ * be `residual`, out `hidden`, row for row. H as for wanmi_adaln_quant, T at most 2^26 - 8. Both norms use eps.
  * Stands beside wanmi_adaln_quant (one request, no norm before the gate); no reference counterpart.
  */
 int wanmi_adaln_sandwich(const void* hidden, int64_t ld_hidden, const void* residual, int64_t ld_residual,
@@ -387,7 +387,7 @@ int wanmi_adaln_sandwich(const void* hidden, int64_t ld_hidden, const void* resi
  * from its first one on (even, their sum a multiple of 16, at most head_dim; channels behind it are not turned), and the
  * angle per unit of position of every pair. rope_pairs: WANMI_ROTATE_* over those channels.
  * gamma: fp32 [heads * head_dim] or [head_dim] as `norm` says, or NULL (ones).
- * head_dim 32, 64, 128 or 256, heads * head_dim at most 16384. request_ids, requests, zero_rest as in
+ * head_dim 32, 64, 128 or 256, heads * head_dim at most 16384, T at most 2^26 - 8. request_ids, requests, zero_rest as in
  * wanmi_adaln_sandwich. k_maxnorm (optional, fp32 [requests, k_heads]): a bound on ||k_out|| of each request's
  * rows: the largest norm before the rounding, times 1 + 2^-8 (0 where a request has no rows). NaN where a row is NaN.
  * Stands beside wanmi_qk_rmsnorm_rope (one sequence, tables of one grid); no reference counterpart.
@@ -411,7 +411,7 @@ int wanmi_qk_norm_rope_axes(const void* q, int64_t q_token_stride, int64_t q_hea
  * e = adapter_ids[q], q = request_ids[t] (NULL: q = t, an id per row). e outside [0, adapters): the row keeps its base.
  * q outside [0, requests): the row is not computed, its output left as it is or zeroed with zero_rest. base and
  * out: bf16 [T, N], rows ldb / ldo elements apart; out may be base, row for row. rank a multiple of 16, at most
- * 1024 (shorter adapters are padded with zeros); K a multiple of 32, N of 8. `workspace`: device
+ * 1024 (shorter adapters are padded with zeros); K a multiple of 32, N of 8; T below 2^28. `workspace`: device
  * memory of wanmi_lora_workspace bytes, for this call alone (two launches on `stream` use it).
  * Stands beside wanmi_mxfp8_gemm, whose activation and output it takes; no reference counterpart.
  */

@@ -186,3 +186,17 @@ def test_c_entry_points_refuse_before_any_launch(pkg):
         assert lora(**kw) == arg, kw
     assert lora(T=0, p=None) == 0
     assert lib.wanmi_lora_workspace(0, 96, 1, 16) == 0 and lib.wanmi_lora_workspace(4, 96, 2, 32) >= 4 * 4 * 64
+
+
+def test_more_rows_than_a_launch_holds(pkg):
+    """A launch has fewer than 2^32 lanes: more rows are an argument error, not a failed launch."""
+    lib = pkg._lib.load()
+    arg = pkg._lib.WANMI_ERR_ARG
+    dims, freqs, widths = (ctypes.c_int * 1)(16), (ctypes.c_double * 8)(), (ctypes.c_int64 * 1)(64)
+    for T in (1 << 26, (1 << 26) - 7):
+        assert lib.wanmi_adaln_sandwich(16, 64, 16, 64, None, None, 0, None, 0, None, 0, None, 1, 1.0, T, 64, 1e-6, 2, 1, 0, 1, 16, 16, None, None) == arg
+        assert lib.wanmi_qk_norm_rope_axes(16, 64, 64, 1, None, 16, 64, 64, None, 0, 0, 0, None, None, 0, 0, T, 64, 16, 0, 1, dims, freqs, 0, 0, 1e-6,
+                                           None, 1, 1, None, None) == arg
+    assert lib.wanmi_lora_add(16, None, None, 96, 16, 16, None, 16, None, 1 << 28, 1, 1 << 28, 96, 64, 16, 1, widths, 16, 64, 16, 64, 1, 16, 1 << 62, None) == arg
+    assert lib.wanmi_qk_norm_rope_axes(16, 64, 64, 1, None, 16, 64, 64, 16, 64, 64, 2, None, 16, 64, 64, 0, 64, 16, 0, 1, dims, freqs, 0, 0, 1e-6,
+                                       16, 1 << 30, 1, 16, None) == arg

@@ -560,7 +560,8 @@ extern "C" int wanmi_adaln_sandwich(const void* hidden, int64_t ld_hidden, const
                                     uint8_t* scales, void* stream) {
   using namespace wanmi;
   clear_error();
-  WANMI_REQUIRE(T >= 0 && T < (1LL << 32), WANMI_ERR_ARG, "wanmi_adaln_sandwich: T=%lld must be in [0, 2^32)", (long long)T);
+  // (a wave a row: a launch has fewer than 2^32 lanes)
+  WANMI_REQUIRE(T >= 0 && T <= (1LL << 26) - 8, WANMI_ERR_ARG, "wanmi_adaln_sandwich: T=%lld must be in [0, 2^26 - 8]", (long long)T);
   WANMI_REQUIRE(H > 0 && H % 32 == 0, WANMI_ERR_ARG, "wanmi_adaln_sandwich: H=%lld must be a positive multiple of 32",
                 (long long)H);
   WANMI_REQUIRE(H <= 16384, WANMI_ERR_UNSUPPORTED, "wanmi_adaln_sandwich: H=%lld exceeds 16384", (long long)H);

@@ -871,7 +871,7 @@ extern "C" int wanmi_lora_add(const void* x, const uint8_t* x_scales, const floa
   using namespace wanmi;
   clear_error();
   const char* const f = "wanmi_lora_add";
-  WANMI_REQUIRE(T >= 0 && T < (1LL << 31), WANMI_ERR_ARG, "%s: T=%lld must be in [0, 2^31)", f, (long long)T);
+  WANMI_REQUIRE(T >= 0 && T < (1LL << 28), WANMI_ERR_ARG, "%s: T=%lld must be in [0, 2^28)", f, (long long)T);
   WANMI_REQUIRE(K > 0 && K % 32 == 0 && K < (1LL << 24), WANMI_ERR_ARG, "%s: K=%lld must be a positive multiple of 32 below 2^24", f, (long long)K);
   WANMI_REQUIRE(N > 0 && N % 8 == 0 && N < (1LL << 24), WANMI_ERR_ARG, "%s: N=%lld must be a positive multiple of 8 below 2^24", f, (long long)N);
   WANMI_REQUIRE(rank > 0 && rank % 16 == 0 && rank <= 1024, WANMI_ERR_ARG, "%s: rank=%d must be a multiple of 16, at most 1024 (pad with zeros)", f, rank);

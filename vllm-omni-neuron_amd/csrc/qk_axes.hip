@@ -338,7 +338,8 @@ extern "C" int wanmi_qk_norm_rope_axes(const void* q, int64_t q_token_stride, in
   using namespace wanmi;
   clear_error();
   const char* const f = "wanmi_qk_norm_rope_axes";
-  WANMI_REQUIRE(T >= 0 && T < (1LL << 32), WANMI_ERR_ARG, "%s: T=%lld must be in [0, 2^32)", f, (long long)T);
+  // (a wave a row: a launch has fewer than 2^32 lanes)
+  WANMI_REQUIRE(T >= 0 && T <= (1LL << 26) - 8, WANMI_ERR_ARG, "%s: T=%lld must be in [0, 2^26 - 8]", f, (long long)T);
   WANMI_REQUIRE(head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256, WANMI_ERR_UNSUPPORTED,
                 "%s: head_dim=%d must be 32, 64, 128 or 256", f, head_dim);
   WANMI_REQUIRE(rope_pairs == WANMI_ROTATE_INTERLEAVED || rope_pairs == WANMI_ROTATE_HALVES, WANMI_ERR_ARG,
@@ -367,6 +368,7 @@ extern "C" int wanmi_qk_norm_rope_axes(const void* q, int64_t q_token_stride, in
   hipStream_t s = (hipStream_t)stream;
   if (k_maxnorm) {
     const int64_t n = requests * k_heads;
+    WANMI_REQUIRE(n < (1LL << 31), WANMI_ERR_ARG, "%s: %lld requests of %d heads are too many", f, (long long)requests, k_heads);
     hipLaunchKernelGGL(qk_axes_zero_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, k_maxnorm, n);
     const int st = check_launch(f);
     if (st != WANMI_OK) return st;

@@ -204,3 +204,30 @@ def test_the_norm_alone(pkg, dev, norm):
     for x, gamma, got in ((q, gq, oq), (k, gk, ok)):
         want, bound, _ = ref.rope_axes(x, torch.zeros(20, 0), (), 1.0, "halves", norm, gamma, EPS)
         ref.within(got, want, bound)
+
+
+def test_bases_as_tensors_are_read_at_every_call(pkg, dev):
+    q, k, pos, _, _ = (None if t is None else t.to(dev) for t in _inputs(40, 4, 2, 128, "none", 23))
+    theta, eps = torch.tensor(10000.0), torch.tensor(EPS)
+    for base in (10000.0, 500.0):
+        theta.fill_(base)
+        for pair in ((theta, EPS), (base, eps)):
+            got = pkg.qk_norm_rope_axes(q, k, pos, theta=pair[0], eps=pair[1])
+            assert all(torch.equal(a, b) for a, b in zip(got, pkg.qk_norm_rope_axes(q, k, pos, theta=base)))
+
+
+@pytest.mark.parametrize("T,hq,hk,D,axes", [(1, 1, 1, 32, (16, 16)), (301, 32, 4, 64, (8, 12, 12)), (301, 32, 32, 64, (32, 16, 16)), (77, 16, 16, 64, (16,)),
+                                            (1030, 16, 1, 128, (44, 42, 42)), (65, 5, 16, 128, (64, 16)), (130, 8, 3, 256, (16, 0, 96)), (9, 3, 64, 32, (16,))])
+@pytest.mark.parametrize("norm", ["none", "rms_norm"])
+@pytest.mark.parametrize("pairs", ["interleaved", "halves"])
+def test_without_the_bound(pkg, dev, pairs, norm, T, hq, hk, D, axes):
+    """Short rows that share neither a weight nor maxima."""
+    q, k, pos, gq, gk = _inputs(T, hq, hk, D, norm, T + hq, axes=len(axes))
+    ids = torch.randint(-1, 3, (T,), generator=torch.Generator().manual_seed(T), dtype=torch.int32)
+    to = lambda v: None if v is None else v.to(dev)  # noqa: E731
+    got = pkg.qk_norm_rope_axes(to(q), to(k), to(pos), axes=axes, rope_pairs=pairs, norm=norm, q_gamma=to(gq), k_gamma=to(gk), eps=EPS, request_ids=to(ids))
+    live = ids >= 0
+    for x, gamma, y in zip((q, k), (gq, gk), got):
+        want, bound, _ = ref.rope_axes(x, pos, axes, 10000.0, pairs, norm, gamma, EPS)
+        ref.within(y[live.to(dev)], want[live], bound[live], "q or k")
+        assert not y[~live.to(dev)].any()

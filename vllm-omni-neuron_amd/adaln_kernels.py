@@ -269,7 +269,7 @@ def _sandwich_plain(hidden, residual, mul, add, eps, post_norm, post_weight, gat
     here); None if any is not."""
     try:
         T, H = shape = hidden.shape
-        if H & 31 or not 0 < H <= _MAX_HIDDEN or not eps >= 0:
+        if H & 31 or not 0 < H <= _MAX_HIDDEN or type(eps) not in (float, int) or not eps >= 0:
             return None
         norms, dev = _lib.NORM, hidden.get_device()
         n_post, n_pre, n_quant = norms[post_norm], norms[norm_type], _lib.QUANT[quant]  # (norm_type None: the full checks)

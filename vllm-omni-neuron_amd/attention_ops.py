@@ -218,6 +218,9 @@ def _qk_axes_plain(q, k, positions, axes, theta, rope_pairs, norm, q_gamma, k_ga
         T, qh, D = q.shape
         kh = k.shape[1]
         turn, kind, dev = _ROTATE[rope_pairs], _QK_NORM[norm], q.get_device()
+        # (numbers of Python's own: the frequencies are kept by their value, and a tensor's may change)
+        if type(theta) not in (float, int) or type(eps) not in (float, int):
+            return None
         if D not in (32, 64, 128, 256) or not _axes_fit(axes, D) or not 0 < theta < math.inf or not eps >= 0:
             return None
         if not 0 < qh * D <= 16384 or not 0 < kh * D <= 16384 or k.shape != (T, kh, D) or k.get_device() != dev or requests is not None:

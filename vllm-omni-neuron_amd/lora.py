@@ -37,7 +37,7 @@ def _workspace(T: int, K: int, parts: int, rank: int) -> int:
 def _fits(slices: tuple, N: int) -> bool:
     """Whether :func:`_check_slices` takes these widths as they are."""
     try:
-        return _check_slices(slices, N) == slices
+        return all(type(w) is int for w in slices) and _check_slices(slices, N) == slices
     except (TypeError, ValueError):
         return False
 

@@ -120,3 +120,18 @@ def test_a_forward_changes_none_of_its_inputs(pkg, dev):
     again = pkg.packed_block_forward(ws[0], h, temb, packed, pos, crosses[0])
     assert torch.equal(first, again)
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before, (h, temb, pos, packed.request_ids)))
+
+
+def test_requests_without_rows_and_a_batch_without_any(pkg, dev):
+    ws, _, _, h, temb, crosses = _setup(pkg, dev, blocks=1)
+    grids = [(0, 5, 7), (2, 5, 7), (1, 0, 3)]
+    packed = pkg.PackedRequests.from_lengths([0, 70, 0], 72, dev)
+    got = pkg.packed_dit_forward(ws, h[:72], temb[:3], packed, packed.grid_positions(grids), [crosses[0][:3]])
+    alone = pkg.PackedRequests.from_lengths([70], 72, dev)
+    want = pkg.packed_dit_forward(ws, h[:72], temb[1:2], alone, alone.grid_positions(grids[1:2]), [crosses[0][1:2]])
+    assert torch.equal(got, want)
+    none = pkg.PackedRequests.from_lengths([0, 0], 0, dev)
+    empty = pkg.packed_dit_forward(ws, h[:0], temb[:2], none, none.grid_positions(grids[::2]), [crosses[0][:2]])
+    assert empty.shape == (0, DIM)
+    idle = pkg.PackedRequests.from_lengths([0], 5, dev)
+    assert not pkg.packed_dit_forward(ws, h[-5:], temb[:1], idle, idle.grid_positions(grids[:1]), [crosses[0][:1]]).any()

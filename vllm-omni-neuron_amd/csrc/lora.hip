@@ -764,7 +764,10 @@ LoraPlan lora_plan(int64_t T, int64_t K, int64_t R, int64_t adapters, bool plain
     const int64_t wgs = (T + rows - 1) / rows * ((R + p.nr - 1) / p.nr);
     const int64_t pairs = K / 128;  // a split holds whole pairs of steps (a stage of MX codes)
     int64_t n = resident / wgs;
-    if (n > pairs / 4) n = pairs / 4;
+    // A split shortens shrink and lengthens expand, which adds them up (rank 128, 1024 rows, K = 13824: 84 us with 6 splits,
+    // 170 with 27; rank 32, 4096 rows, K = 5120: 32 with 4, 39 with 10). At few rows shrink takes about 0.57 us more
+    // for a pair of steps and expand 1.3 for a split at rank 32, 1.7 and 5 at 128: least where n^2 is 0.34 to 0.44 of the pairs.
+    while (n > 1 && 5 * n * n > 2 * pairs) --n;
     if (n < 1) n = 1;
     const int64_t per = (pairs + n - 1) / n;
     p.splits = (int)((pairs + per - 1) / per);

@@ -231,3 +231,21 @@ def test_without_the_bound(pkg, dev, pairs, norm, T, hq, hk, D, axes):
         want, bound, _ = ref.rope_axes(x, pos, axes, 10000.0, pairs, norm, gamma, EPS)
         ref.within(y[live.to(dev)], want[live], bound[live], "q or k")
         assert not y[~live.to(dev)].any()
+
+
+@pytest.mark.parametrize("norm", ["none", "rms_norm_across_heads"])
+def test_a_batch_of_no_requests(pkg, dev, norm):
+    """``requests=0``: every row belongs to none, with the bound as without it."""
+    T, hq, hk = 70, 4, 2
+    q, k, pos, gq, gk = (None if t is None else t.to(dev) for t in _inputs(T, hq, hk, 128, norm, 29))
+    kw = dict(norm=norm, q_gamma=gq, k_gamma=gk, request_ids=torch.zeros(T, dtype=torch.int32, device=dev), requests=0)
+    for want_max in (False, True):
+        for _ in range(4):  # what the allocator hands out next holds no zeros
+            old = [torch.full_like(t, float("nan")) for t in (q, k)]
+            del old
+            oq, ok, *rest = pkg.qk_norm_rope_axes(q, k, pos, want_max=want_max, **kw)
+            assert not oq.any() and not ok.any()
+            assert not want_max or rest[0].shape == (0, hk)
+    q_out = torch.full_like(q, 5.0)
+    _, ok, kmax = pkg.qk_norm_rope_axes(q, k, pos, want_max=True, q_out=q_out, **kw)
+    assert bool((q_out == 5.0).all()) and not ok.any() and kmax.shape == (0, hk)

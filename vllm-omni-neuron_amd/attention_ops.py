@@ -325,14 +325,12 @@ def _qk_axes_checked(q, k, positions, axes, theta, rope_pairs, norm, q_gamma, k_
             views[i] = (*views[i][:3], out.stride(0), out.stride(1))
         outs.append(out)
     kmax = torch.empty((n, k.shape[1]), dtype=torch.float32, device=dev) if want_max else None
-    if kmax is not None and n == 0:
-        return (*outs, kmax)
     p = _lib.ptr
     dims, freqs = _axis_arrays(axes, theta)
     (qts, qhs, qh, qots, qohs), (kts, khs, kh, kots, kohs) = views
     _lib.call("wanmi_qk_norm_rope_axes", q.get_device(), p(q), qts, qhs, qh, p(q_gamma), p(outs[0]), qots, qohs, p(k), kts, khs, kh, p(k_gamma),
               p(outs[1]), kots, kohs, T, D, p(positions), int(floats), len(axes), dims, freqs,
-              _ROTATE[rope_pairs], _QK_NORM[norm], float(eps), p(request_ids), n, int(zero_rest), p(kmax))
+              _ROTATE[rope_pairs], _QK_NORM[norm], float(eps), p(request_ids), n, int(zero_rest), p(kmax) if n else None)
     return (*outs, kmax) if want_max else tuple(outs)
 
 

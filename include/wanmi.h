@@ -409,7 +409,8 @@ int wanmi_qk_norm_rope_axes(const void* q, int64_t q_token_stride, int64_t q_hea
  * [adapters, N, rank]; the columns of a fused projection fall into `parts` runs of part_widths (HOST array; multiples
  * of 64 unless there is one), p(n) is the run of column n. adapter_scales fp32 [adapters] or NULL.
  * e = adapter_ids[q], q = request_ids[t] (NULL: q = t, an id per row). e outside [0, adapters): the row keeps its base.
- * q outside [0, requests): the row is not computed, its output left as it is or zeroed with zero_rest. base and
+ * q outside [0, requests): the row is not computed, its output left as it is or zeroed with zero_rest (requests 0 with
+ * request_ids: no row is, and adapter_ids may be NULL). base and
  * out: bf16 [T, N], rows ldb / ldo elements apart; out may be base, row for row. rank a multiple of 16, at most
  * 1024 (shorter adapters are padded with zeros); K a multiple of 32, N of 8; T below 2^28. `workspace`: device
  * memory of wanmi_lora_workspace bytes, for this call alone (two launches on `stream` use it).

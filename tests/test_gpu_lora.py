@@ -261,3 +261,16 @@ def test_graph_replays_with_other_adapters_and_two_graphs(pkg, dev):
         want = call()
         torch.cuda.synchronize()
         assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("T", [9, 1100])
+def test_a_batch_of_no_requests(pkg, dev, T):
+    """No adapter ids at all: every row belongs to no request."""
+    base, x, a, b, scales = (t.to(dev) for t in _inputs(T, 128, (64,), 2, 16, 37))
+    none = torch.empty(0, dtype=torch.int32, device=dev)
+    for ids in (torch.full((T,), -1, dtype=torch.int32, device=dev), torch.zeros(T, dtype=torch.int32, device=dev)):
+        out = pkg.lora_add(base, x, a, b, none, scales=scales, request_ids=ids)
+        assert out.shape == base.shape and not out.any()
+        given = torch.full_like(base, 3.0)
+        pkg.lora_add(base, x, a, b, none, scales=scales, request_ids=ids, out=given)
+        assert bool((given == 3.0).all())

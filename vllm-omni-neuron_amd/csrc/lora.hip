@@ -891,7 +891,8 @@ extern "C" int wanmi_lora_add(const void* x, const uint8_t* x_scales, const floa
   }
   WANMI_REQUIRE(end == N, WANMI_ERR_ARG, "%s: the parts hold %lld of %lld columns", f, (long long)end, (long long)N);
   if (T == 0) return WANMI_OK;
-  WANMI_REQUIRE(x && A && B && adapter_ids && base && out && workspace, WANMI_ERR_ARG, "%s: null pointer", f);
+  // (without requests there is no row that has an adapter id)
+  WANMI_REQUIRE(x && A && B && (adapter_ids || (request_ids && requests == 0)) && base && out && workspace, WANMI_ERR_ARG, "%s: null pointer", f);
   WANMI_REQUIRE(ldx >= K && ldx % (x_scales ? 16 : 8) == 0, WANMI_ERR_ARG, "%s: x rows must be 16-byte aligned", f);
   WANMI_REQUIRE(ldb >= N && ldb % 8 == 0 && ldo >= N && ldo % 8 == 0, WANMI_ERR_ARG,
                 "%s: the row strides of base and out must be multiples of 8 of at least N", f);

@@ -274,3 +274,21 @@ def test_a_batch_of_no_requests(pkg, dev, T):
         given = torch.full_like(base, 3.0)
         pkg.lora_add(base, x, a, b, none, scales=scales, request_ids=ids, out=given)
         assert bool((given == 3.0).all())
+
+
+@pytest.mark.parametrize("zero_rest", [0, 1])
+@pytest.mark.parametrize("T,rank", [(9, 16), (1100, 16), (1100, 144)])
+def test_more_rows_than_requests_without_request_ids(pkg, dev, T, rank, zero_rest):
+    """The C entry point without request_ids: row t is request t, and the rows behind the last request read no adapter id."""
+    R, K, N = T - 5, 128, 64
+    base, x, a, b, scales = (t.to(dev) for t in _inputs(T, K, (N,), 2, rank, 41))
+    ids = (torch.arange(T, device=dev) % 3 - 1).int()  # (ids behind the last request, too: what they say is not used)
+    want = pkg.lora_add(base, x, a, b, ids, scales=scales)
+    out = torch.full_like(base, 3.0)
+    lib = pkg._lib.load()
+    size = lib.wanmi_lora_workspace(T, K, 1, rank)
+    work = torch.empty(size, dtype=torch.uint8, device=dev)
+    p = lambda t: t.data_ptr()  # noqa: E731
+    pkg._lib.call("wanmi_lora_add", 0, p(x), None, None, K, p(a), p(b), p(scales), p(ids), None, R, 2, T, K, N, rank, 1, pkg.lora._widths((N,)), p(base), N,
+                  p(out), N, zero_rest, p(work), size)
+    assert torch.equal(out[:R], want[:R]) and bool((out[R:] == (0.0 if zero_rest else 3.0)).all())

@@ -60,13 +60,9 @@ struct LoraArgs {
 // The adapter of row t: -1 none (the row keeps its base), -2 no request (the row is not computed).
 __device__ __forceinline__ int row_adapter(const LoraArgs& a, int64_t t) {
   if (t >= a.T) return -2;
-  int64_t at = t;
-  if (a.request_ids) {
-    const int q = a.request_ids[t];
-    if ((uint32_t)q >= (uint32_t)a.requests) return -2;
-    at = q;
-  }
-  const int e = a.adapter_ids[at];
+  const int q = a.request_ids ? a.request_ids[t] : (int)t;
+  if ((uint32_t)q >= (uint32_t)a.requests) return -2;  // (adapter_ids ends there)
+  const int e = a.adapter_ids[q];
   return (uint32_t)e < (uint32_t)a.adapters ? e : -1;
 }
 

@@ -249,3 +249,11 @@ def test_a_batch_of_no_requests(pkg, dev, norm):
     q_out = torch.full_like(q, 5.0)
     _, ok, kmax = pkg.qk_norm_rope_axes(q, k, pos, want_max=True, q_out=q_out, **kw)
     assert bool((q_out == 5.0).all()) and not ok.any() and kmax.shape == (0, hk)
+
+
+@pytest.mark.parametrize("norm", ["rms_norm", "rms_norm_across_heads"])
+def test_rows_whose_mean_square_is_subnormal(pkg, dev, norm):
+    """Without eps, rows of 2^-64 normalize like any others: their mean square is held to 2^-150, 2^-22 of itself."""
+    q, k, pos, gq, gk = _inputs(33, 5, 3, 128, norm, 31)
+    tiny = lambda x: (x.float() * 2.0**-64).to(torch.bfloat16)  # noqa: E731
+    _check(pkg, dev, tiny(q), tiny(k), pos, gq, gk, norm=norm, eps=0.0)

@@ -244,3 +244,14 @@ def test_without_a_residual_or_without_a_second_output(pkg, dev, T, H):
     ro = torch.full_like(full, 2.0)
     pkg.adaln_sandwich(to(h), to(res), norm_type=None, residual_out=ro, **kw)
     assert torch.equal(ro[: T - 2], full[: T - 2]) and bool((ro[T - 2 :] == 2.0).all())
+
+
+@pytest.mark.parametrize("T", [5, 600])
+@pytest.mark.parametrize("norm", ["layer_norm", "rms_norm"])
+def test_rows_whose_variance_is_subnormal(pkg, dev, norm, T):
+    """Without eps, rows of 3 x 2^-66 normalize like any others: their mean square (2^-129) is held to 2^-150, 2^-21 of itself."""
+    ids = ref.packed_ids([T])
+    h, res, w, gate, mul, add = _inputs(T, 512, 1, 71)
+    tiny = (h.float() * 2.0**-66).to(torch.bfloat16)
+    _check(pkg, dev, tiny, res, w, gate, mul, add, ids, post=norm, eps=0.0)
+    _check(pkg, dev, torch.zeros_like(h), tiny, None, None, mul, add, ids, post="none", norm=norm, eps=0.0)

@@ -190,12 +190,15 @@ __device__ __forceinline__ int max_with_lane_xor32(int x) {
 }
 
 // 1 / sqrt(x) for x >= 0 in fp32: the hardware's estimate (within 1 ulp, infinite for 0 and 0 for infinity), one Newton
-// step where that is finite and not zero. A workgroup whose threads all need the root of their row spends a
-// fourth of the time on it that the fp64 division and root take.
+// step where that is finite and not zero. The estimate takes subnormal x for 0 (a mean square of values of 2^-64, without
+// eps): those are scaled by 2^64 before and the root by 2^32 after it, exactly. A workgroup whose threads all need the
+// root of their row spends a fourth of the time on it that the fp64 division and root take.
 __device__ __forceinline__ float rsqrt_f32(float x) {
-  const float y = __builtin_amdgcn_rsqf(x);
-  const float z = y * fmaf(-0.5f * x * y, y, 1.5f);
-  return y > 0.0f && y < INFINITY ? z : y;
+  const bool small = x < 0x1p-126f;
+  const float s = small ? x * 0x1p64f : x;
+  const float y = __builtin_amdgcn_rsqf(s);
+  const float z = y * fmaf(-0.5f * s * y, y, 1.5f);
+  return (y > 0.0f && y < INFINITY ? z : y) * (small ? 0x1p32f : 1.0f);
 }
 
 // s_waitcnt immediates (gfx9 encoding: vmcnt[3:0] | expcnt[6:4] | lgkmcnt[11:8] | vmcnt[5:4] << 14)

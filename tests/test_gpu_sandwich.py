@@ -255,3 +255,22 @@ def test_rows_whose_variance_is_subnormal(pkg, dev, norm, T):
     tiny = (h.float() * 2.0**-66).to(torch.bfloat16)
     _check(pkg, dev, tiny, res, w, gate, mul, add, ids, post=norm, eps=0.0)
     _check(pkg, dev, torch.zeros_like(h), tiny, None, None, mul, add, ids, post="none", norm=norm, eps=0.0)
+
+
+@pytest.mark.parametrize("T", [6, 700])
+def test_one_row_of_vectors_serves_one_request(pkg, dev, T):
+    """Vectors ``[1, H]`` are those of request 0: a row with another id belongs to none. Beside vectors of several
+    requests, and as ``[H]``, they serve every one."""
+    H = 96
+    ids = (torch.arange(T) % 3 - 1).to(torch.int32)  # -1, 0, 1
+    h, res, w, gate, mul, add = _inputs(T, H, 1, 73)
+    _check(pkg, dev, h, res, w, gate, mul, add, torch.where(ids == 0, ids, -1))
+    to = lambda v: v.to(dev)  # noqa: E731
+    kw = dict(eps=EPS, post_weight=to(w), request_ids=to(ids))
+    mine = (ids == 0).to(dev)
+    r, y = pkg.adaln_sandwich(to(h), to(res), to(mul), to(add), gate=to(gate), **kw)
+    assert not r[~mine].any() and not y[~mine].any() and bool(r[mine].any(1).all())
+    every = pkg.adaln_sandwich(to(h), to(res), to(mul)[0], to(add)[0], gate=to(gate)[0], **kw)
+    assert torch.equal(every[0][mine], r[mine]) and torch.equal(every[1][mine], y[mine])
+    mixed = pkg.adaln_sandwich(to(h), to(res), to(mul).expand(2, H).contiguous(), to(add), gate=to(gate), **kw)
+    assert all(torch.equal(a, b) for a, b in zip(every, mixed)) and bool(every[0][(ids == 1).to(dev)].any(1).all())

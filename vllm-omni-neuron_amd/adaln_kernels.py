@@ -180,8 +180,8 @@ def adaln_modulate(
 
 
 def _request_vector(vec: torch.Tensor | None, name: str, H: int, requests: int | None):
-    """fp32 ``[H]`` (or ``[1, H]``: for every request) or ``[R, H]`` (one row per request) -> (elements between
-    requests, requests so far)."""
+    """fp32 ``[H]`` (for every request) or ``[R, H]`` (one row per request; ``[1, H]`` beside vectors of several: for every
+    one) -> (elements between requests, requests so far)."""
     if vec is None:
         return 0, requests
     _lib.expect(vec, name, dtype=torch.float32, contiguous=False, row_contiguous=True)
@@ -189,9 +189,11 @@ def _request_vector(vec: torch.Tensor | None, name: str, H: int, requests: int |
         raise ValueError(f"{name} must be [{H}] or [requests, {H}], got {list(vec.shape)}")
     if vec.data_ptr() % 16:
         raise ValueError(f"{name} must be 16-byte aligned")
-    if vec.dim() == 1 or vec.shape[0] == 1:
+    if vec.dim() == 1:
         return 0, requests
-    if requests is not None and vec.shape[0] != requests:
+    if vec.shape[0] == 1:
+        return 0, 1 if requests is None else requests
+    if requests not in (None, 1, vec.shape[0]):
         raise ValueError(f"{name} has {vec.shape[0]} rows, the other vectors {requests}")
     if vec.stride(0) < H or vec.stride(0) % 4:
         raise ValueError(f"{name} rows must lie a multiple of 4 elements of at least {H} apart")
@@ -233,7 +235,8 @@ def adaln_sandwich(
 
     ``hidden`` (the sub-layer's output) and ``residual``: bf16 ``[T, H]``, any row stride; ``post_weight`` fp32
     ``[H]``; ``gate`` / ``mul`` / ``add`` fp32 ``[H]`` for every request, or ``[R, H]``, one row per request (rows
-    may be strided: a slice ``mod[:, i]`` of a ``[R, 6, H]`` modulation is taken as it is). ``post_norm`` and
+    may be strided: a slice ``mod[:, i]`` of a ``[R, 6, H]`` modulation is taken as it is; ``[1, H]`` beside vectors of
+    several requests serves them all). ``post_norm`` and
     ``norm_type`` are ``"layer_norm"``, ``"rms_norm"`` or ``"none"``, both with ``eps``. ``quant`` as in
     :func:`adaln_modulate`.
 
@@ -330,7 +333,7 @@ def _sandwich_checked(hidden, residual, mul, add, eps, post_norm, post_weight, g
     ld_mul, requests = _request_vector(mul, "mul", H, requests)
     ld_add, requests = _request_vector(add, "add", H, requests)
     _lib.request_rows(request_ids, T)
-    if request_ids is None and requests is not None:
+    if request_ids is None and requests not in (None, 1):
         raise ValueError("vectors of several requests need request_ids")
     if not eps >= 0:
         raise ValueError(f"eps must be non-negative, got {eps}")

@@ -200,3 +200,33 @@ def test_more_rows_than_a_launch_holds(pkg):
     assert lib.wanmi_lora_add(16, None, None, 96, 16, 16, None, 16, None, 1 << 28, 1, 1 << 28, 96, 64, 16, 1, widths, 16, 64, 16, 64, 1, 16, 1 << 62, None) == arg
     assert lib.wanmi_qk_norm_rope_axes(16, 64, 64, 1, None, 16, 64, 64, 16, 64, 64, 2, None, 16, 64, 64, 0, 64, 16, 0, 1, dims, freqs, 0, 0, 1e-6,
                                        16, 1 << 30, 1, 16, None) == arg
+
+
+def _over(t, dtype, *shape):
+    """A tensor of this type and shape over the first bytes of ``t``."""
+    raw = t.view(-1).view(torch.uint8)
+    n = torch.empty((), dtype=dtype).element_size()
+    for s in shape:
+        n *= s
+    return raw[:n].view(dtype).view(shape)
+
+
+def test_sandwich_outputs_over_the_other_inputs(pkg):
+    """What every row still reads: the vectors and the ids; and the scales of the codes, over anything."""
+    big = {name: f(2 * T, H) for name in ("mul", "add", "gate", "post_weight", "request_ids")}
+    arg = dict(mul=big["mul"][:2], add=big["add"][:2], gate=big["gate"][:2], post_weight=big["post_weight"][0], request_ids=_over(big["request_ids"], torch.int32, T))
+    for name in big:
+        over = _over(big[name], BF, T, H)
+        for kw in (dict(out=over), dict(residual_out=over)):
+            args = dict(arg)
+            with pytest.raises(ValueError, match="overlaps|may not be"):
+                pkg.adaln_sandwich(z(T, H), z(T, H), args.pop("mul"), args.pop("add"), eps=1e-6, **args, **kw)
+    codes = z(T, H, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    kw = dict(eps=1e-6, quant="mx", request_ids=arg["request_ids"], gate=arg["gate"])
+    hidden, residual, ro = z(T, H), z(T, H), z(T, H)
+    for t in (big["gate"], big["request_ids"], hidden, residual, ro, codes):
+        scales = _over(t, torch.uint8, T, H // 32)
+        with pytest.raises(ValueError, match="overlaps|may not be|share memory"):
+            pkg.adaln_sandwich(hidden, residual, residual_out=ro, out=pkg.MXTensor(codes, scales), **kw)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):  # apart from each other: accepted, but for the device
+        pkg.adaln_sandwich(hidden, residual, residual_out=residual, out=pkg.MXTensor(codes, z(T, H // 32, dtype=torch.uint8)), **kw)

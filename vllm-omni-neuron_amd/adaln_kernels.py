@@ -347,11 +347,15 @@ def _sandwich_checked(hidden, residual, mul, add, eps, post_norm, post_weight, g
         if codes.data_ptr() % 16:
             raise ValueError("out must be 16-byte aligned")
         _lib.refuse_overlap(codes, "out", hidden, residual)
+        _lib.refuse_input(codes, "out", post_weight, gate, mul, add, request_ids)
+        if scales is not None:
+            _lib.refuse_input(scales, "out.scales", hidden, residual, post_weight, gate, mul, add, request_ids, codes, residual_out)
     if residual_out is not None:
         _lib.expect(residual_out, "residual_out", dtype=torch.bfloat16, shape=(T, H))
         if residual_out.data_ptr() % 16:
             raise ValueError("residual_out must be 16-byte aligned")
         _lib.refuse_overlap(residual_out, "residual_out", hidden, residual)
+        _lib.refuse_input(residual_out, "residual_out", post_weight, gate, mul, add, request_ids)
         if out is not None and _shares(codes, residual_out):
             raise ValueError("out and residual_out share memory")
     _lib.require_gpu(hidden, residual, post_weight, gate, mul, add, request_ids, residual_out, codes, scales,

@@ -230,3 +230,15 @@ def test_sandwich_outputs_over_the_other_inputs(pkg):
             pkg.adaln_sandwich(hidden, residual, residual_out=ro, out=pkg.MXTensor(codes, scales), **kw)
     with pytest.raises(RuntimeError, match="no CPU fallback"):  # apart from each other: accepted, but for the device
         pkg.adaln_sandwich(hidden, residual, residual_out=residual, out=pkg.MXTensor(codes, z(T, H // 32, dtype=torch.uint8)), **kw)
+
+
+def test_lora_outputs_over_the_other_inputs(pkg):
+    """The ids and scales that the rows of other workgroups still read."""
+    buf = {name: f(T, 128) for name in ("scales", "adapter_ids", "request_ids")}
+    arg = dict(scales=_over(buf["scales"], torch.float32, 2), adapter_ids=_over(buf["adapter_ids"], torch.int32, T),
+               request_ids=_over(buf["request_ids"], torch.int32, T))
+    for name in buf:
+        with pytest.raises(ValueError, match="overlaps|may not be"):
+            _lora(pkg, out=_over(buf[name], BF, T, 128), **arg)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        _lora(pkg, out=z(T, 128), **arg)

@@ -191,19 +191,26 @@ def plain_ptr(t: torch.Tensor | None, dtype: torch.dtype, shape, dev: int):
     return p if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == dev and not p & 15 else -1
 
 
+def _span(t: torch.Tensor) -> int:
+    """Bytes from a tensor's first element to the end of its last."""
+    if t.is_contiguous():
+        return t.nbytes
+    return t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) if t.numel() else 0
+
+
 def refuse_overlap(out: torch.Tensor, what: str, *inputs: torch.Tensor | None) -> None:
     """An output may be an input, element for element, or share no byte with it: anything between would be read after
     it is written. Views of one buffer whose rows are equally far apart are told apart by their columns."""
+    a0 = out.data_ptr()
+    a1 = a0 + _span(out)
     for t in inputs:
-        if t is None or not t.numel() or not out.numel():
+        if t is None:
+            continue
+        b0 = t.data_ptr()
+        if b0 >= a1 or b0 + _span(t) <= a0 or not t.numel() or not out.numel():
             continue
         size, tsize = out.element_size(), t.element_size()
-        a0, b0 = out.data_ptr(), t.data_ptr()
         if a0 == b0 and size == tsize and out.shape == t.shape and out.stride() == t.stride():
-            continue
-        a1 = a0 + size * (1 + sum((n - 1) * s for n, s in zip(out.shape, out.stride())))
-        b1 = b0 + tsize * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-        if a1 <= b0 or b1 <= a0:
             continue
         if out.dim() > 1 and t.dim() > 1 and out.stride(0) * size == t.stride(0) * tsize:
             pitch = out.stride(0) * size
@@ -218,7 +225,7 @@ def refuse_overlap(out: torch.Tensor, what: str, *inputs: torch.Tensor | None) -
 def refuse_input(out: torch.Tensor, what: str, *inputs: torch.Tensor | None) -> None:
     """An output that shares memory with an input which other rows still read, even element for element."""
     for t in inputs:
-        if t is not None and t.numel() and out.numel() and t.data_ptr() == out.data_ptr():
+        if t is not None and t.data_ptr() == out.data_ptr() and t.numel() and out.numel():
             raise ValueError(f"{what} may not be that input")
     refuse_overlap(out, what, *inputs)
 

@@ -179,7 +179,7 @@ def _add_checked(base, x, a, b, adapter_ids, scales, slices, request_ids, out):
         if (T > 1 and (out.stride(0) < N or out.stride(0) % 8)) or out.data_ptr() % 16:
             raise ValueError("out rows must be 16-byte aligned")
         _lib.refuse_overlap(out, "out", base)
-        _lib.refuse_input(out, "out", codes, x_scales, a, b)
+        _lib.refuse_input(out, "out", codes, x_scales, row_scale, a, b, scales, adapter_ids, request_ids)
     _lib.require_gpu(base, codes, x_scales, row_scale, a, b, scales, adapter_ids, request_ids, out, what="lora_add")
     zero_rest = out is None
     if out is None:

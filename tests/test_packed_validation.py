@@ -242,3 +242,16 @@ def test_lora_outputs_over_the_other_inputs(pkg):
             _lora(pkg, out=_over(buf[name], BF, T, 128), **arg)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         _lora(pkg, out=z(T, 128), **arg)
+
+
+def test_qk_axes_outputs_over_the_other_inputs(pkg):
+    """The positions, ids and weights that the rows of other workgroups still read, for either output."""
+    buf = {name: f(T, 256) for name in ("positions", "request_ids", "q_gamma", "k_gamma")}
+    arg = dict(positions=_over(buf["positions"], torch.int32, T, 2), request_ids=_over(buf["request_ids"], torch.int32, T), requests=2,
+               q_gamma=_over(buf["q_gamma"], torch.float32, 64), k_gamma=_over(buf["k_gamma"], torch.float32, 64), norm="rms_norm")
+    for name in buf:
+        for out in (dict(q_out=_over(buf[name], BF, T, 4, 64)), dict(k_out=_over(buf[name], BF, T, 2, 64))):
+            with pytest.raises(ValueError, match="overlaps|may not be"):
+                _qk(pkg, **arg, **out)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        _qk(pkg, q_out=z(T, 4, 64), k_out=z(T, 2, 64), **arg)

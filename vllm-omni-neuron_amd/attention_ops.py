@@ -290,6 +290,7 @@ def _qk_axes_checked(q, k, positions, axes, theta, rope_pairs, norm, q_gamma, k_
                 raise ValueError(f"{name}_out must be {list(x.shape)}, got {list(out.shape)}")
             _separate(out, f"{name}_out")
             _lib.refuse_overlap(out, f"{name}_out", q, k)
+            _lib.refuse_input(out, f"{name}_out", positions, q_gamma, k_gamma, request_ids)
             if name == "k" and q_out is not None:
                 _lib.refuse_overlap(out, "k_out", q_out)
                 if out.data_ptr() == q_out.data_ptr() and out.numel():

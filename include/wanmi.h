@@ -386,7 +386,7 @@ int wanmi_adaln_sandwich(const void* hidden, int64_t ld_hidden, const void* resi
  * axis_dims [axes] and freqs [sum(axis_dims) / 2] are HOST arrays (no axes: positions and both NULL): the axes' channels, which fill the head
  * from its first one on (even, their sum a multiple of 16, at most head_dim; channels behind it are not turned), and the
  * angle per unit of position of every pair. rope_pairs: WANMI_ROTATE_* over those channels.
- * gamma: fp32 [heads * head_dim] or [head_dim] as `norm` says, or NULL (ones).
+ * gamma: fp32 [heads * head_dim] (16-byte aligned) or [head_dim] as `norm` says, or NULL (ones).
  * head_dim 32, 64, 128 or 256, heads * head_dim at most 16384, T at most 2^26 - 8. request_ids, requests, zero_rest as in
  * wanmi_adaln_sandwich. k_maxnorm (optional, fp32 [requests, k_heads]): a bound on ||k_out|| of each request's
  * rows: the largest norm before the rounding, times 1 + 2^-8 (0 where a request has no rows). NaN where a row is NaN.

@@ -257,3 +257,13 @@ def test_rows_whose_mean_square_is_subnormal(pkg, dev, norm):
     q, k, pos, gq, gk = _inputs(33, 5, 3, 128, norm, 31)
     tiny = lambda x: (x.float() * 2.0**-64).to(torch.bfloat16)  # noqa: E731
     _check(pkg, dev, tiny(q), tiny(k), pos, gq, gk, norm=norm, eps=0.0)
+
+
+@pytest.mark.parametrize("pairs", ["interleaved", "halves"])
+def test_a_weight_of_one_head_at_an_odd_float(pkg, dev, pairs):
+    q, k, pos, gq, gk = (t.to(dev) for t in _inputs(20, 3, 2, 128, "rms_norm", 37))
+    want = pkg.qk_norm_rope_axes(q, k, pos, rope_pairs=pairs, norm="rms_norm", q_gamma=gq, k_gamma=gk)
+    buf = torch.zeros(300, device=dev)
+    buf[1:129], buf[150:278] = gq, gk
+    got = pkg.qk_norm_rope_axes(q, k, pos, rope_pairs=pairs, norm="rms_norm", q_gamma=buf[1:129], k_gamma=buf[150:278])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -255,3 +255,16 @@ def test_qk_axes_outputs_over_the_other_inputs(pkg):
                 _qk(pkg, **arg, **out)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         _qk(pkg, q_out=z(T, 4, 64), k_out=z(T, 2, 64), **arg)
+
+
+def test_qk_axes_weights_across_heads_at_an_odd_float(pkg):
+    """They are read 16 bytes a lane; a weight of one head may lie anywhere."""
+    for kw, what in ((dict(q_gamma=f(257)[1:]), "q_gamma"), (dict(q_gamma=f(256), k_gamma=f(130)[2:]), "k_gamma")):
+        with pytest.raises(ValueError, match=f"{what} must be 16-byte aligned"):
+            _qk(pkg, norm="rms_norm_across_heads", **kw)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        _qk(pkg, norm="rms_norm", q_gamma=f(65)[1:])
+    lib, dims, freqs = pkg._lib.load(), (ctypes.c_int * 1)(16), (ctypes.c_double * 8)()
+    for gq, gk in ((20, None), (None, 24), (32, 36)):
+        assert lib.wanmi_qk_norm_rope_axes(16, 64, 64, 1, gq, 16, 64, 64, 16, 64, 64, 1, gk, 16, 64, 64, 4, 64, 16, 0, 1, dims, freqs, 0, 2, 1e-6,
+                                           None, 1, 1, None, None) == pkg._lib.WANMI_ERR_ARG

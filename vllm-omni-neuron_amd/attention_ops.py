@@ -189,7 +189,7 @@ def qk_norm_rope_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.
     2i and 2i+1) or ``"halves"`` (i and i + half of the turned channels).
 
     ``norm``: ``"none"``, ``"rms_norm"`` (each head, weight fp32 ``[D]``) or ``"rms_norm_across_heads"`` (the whole row,
-    weight fp32 ``[heads * D]``); a weight left out is ones. Norm and rotation are fp32, rounded once
+    weight fp32 ``[heads * D]``, 16-byte aligned); a weight left out is ones. Norm and rotation are fp32, rounded once
     (:func:`qk_rmsnorm_rope_` rounds between them, as its reference does).
 
     Returns ``(q_out, k_out)``; ``q_out`` / ``k_out`` may be given, and may be ``q`` and ``k`` themselves. With
@@ -283,6 +283,8 @@ def _qk_axes_checked(q, k, positions, axes, theta, rope_pairs, norm, q_gamma, k_
             if norm == "none":
                 raise ValueError(f"{name}_gamma without a norm")
             _lib.expect(gamma, f"{name}_gamma", dtype=torch.float32, shape=(D if norm == "rms_norm" else heads * D,))
+            if norm == "rms_norm_across_heads" and gamma.data_ptr() % 16:
+                raise ValueError(f"{name}_gamma must be 16-byte aligned")
         ots = ohs = 0
         if out is not None:
             ots, ohs, _ = _heads_view(out, f"{name}_out", T, D)

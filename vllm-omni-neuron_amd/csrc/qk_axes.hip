@@ -382,6 +382,10 @@ extern "C" int wanmi_qk_norm_rope_axes(const void* q, int64_t q_token_stride, in
     WANMI_REQUIRE(v >= 0 && v % 8 == 0, WANMI_ERR_ARG, "%s: strides must be multiples of 8 elements, got %lld", f, (long long)v);
   for (const void* p : {q, (const void*)q_out, k, (const void*)k_out})
     WANMI_REQUIRE(((uintptr_t)p % 16) == 0, WANMI_ERR_ARG, "%s: tensors must be 16-byte aligned", f);
+  // (read 16 bytes a lane, straight into LDS; a head's own weight is read by the element)
+  for (const float* p : {q_gamma, k_gamma})
+    WANMI_REQUIRE(norm != WANMI_QKNORM_ACROSS_HEADS || ((uintptr_t)p % 16) == 0, WANMI_ERR_ARG,
+                  "%s: the weights of a norm across heads must be 16-byte aligned", f);
   a.part[0] = {static_cast<const uint16_t*>(q), q_token_stride, q_head_stride, static_cast<uint16_t*>(q_out),
                q_out_token_stride, q_out_head_stride, q_gamma, q_heads};
   a.part[1] = {static_cast<const uint16_t*>(k), k_token_stride, k_head_stride, static_cast<uint16_t*>(k_out),

@@ -268,3 +268,11 @@ def test_qk_axes_weights_across_heads_at_an_odd_float(pkg):
     for gq, gk in ((20, None), (None, 24), (32, 36)):
         assert lib.wanmi_qk_norm_rope_axes(16, 64, 64, 1, gq, 16, 64, 64, 16, 64, 64, 1, gk, 16, 64, 64, 4, 64, 16, 0, 1, dims, freqs, 0, 2, 1e-6,
                                            None, 1, 1, None, None) == pkg._lib.WANMI_ERR_ARG
+
+
+@pytest.mark.parametrize("name", ["mul", "add", "gate"])
+def test_sandwich_vectors_without_dimensions(pkg, name):
+    args = dict(mul=None, add=None, gate=None)
+    args[name] = torch.tensor(1.0)
+    with pytest.raises(ValueError, match=name):
+        pkg.adaln_sandwich(z(T, H), z(T, H), args["mul"], args["add"], gate=args["gate"], eps=1e-6)

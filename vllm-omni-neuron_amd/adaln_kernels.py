@@ -293,7 +293,7 @@ def _sandwich_plain(hidden, residual, mul, add, eps, post_norm, post_weight, gat
         pg, lg = _request_ptr(gate, vs, dev)
         pm, lm = _request_ptr(mul, vs, dev)
         pa, la = _request_ptr(add, vs, dev)
-    except (AttributeError, KeyError, TypeError, ValueError):
+    except (AttributeError, IndexError, KeyError, TypeError, ValueError):
         return None
     if dev < 0 or T == 0 or -1 in (ph, pr, pw, pi, pg, pm, pa):
         return None

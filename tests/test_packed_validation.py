@@ -276,3 +276,16 @@ def test_sandwich_vectors_without_dimensions(pkg, name):
     args[name] = torch.tensor(1.0)
     with pytest.raises(ValueError, match=name):
         pkg.adaln_sandwich(z(T, H), z(T, H), args["mul"], args["add"], gate=args["gate"], eps=1e-6)
+
+
+def test_packed_forward_refuses_what_does_not_fit(pkg):
+    packed = pkg.PackedRequests.from_lengths([2, 3], 6, "cpu")
+    args = dict(h=z(6, 128), temb=f(2, 6, 128), packed=packed, positions=torch.zeros(6, 3, dtype=torch.int32), crosses=[[None, None]])
+    none = pkg.packed_block.BlockAdapters()
+    for kw, match in ((dict(h=z(5, 128)), "do not fit"), (dict(positions=torch.zeros(6, 2, dtype=torch.int32)), "do not fit"), (dict(temb=f(1, 6, 128)), "crosses"),
+                      (dict(crosses=[[None]]), "crosses"), (dict(crosses=[]), "crosses"), (dict(adapter_ids=ids(3)), "adapter_ids"),
+                      (dict(adapters=[none, none], adapter_ids=ids(2)), "adapters")):
+        with pytest.raises(ValueError, match=match):
+            pkg.packed_dit_forward([None], **{**args, **kw}, tables=f(1, 6, 128))
+    with pytest.raises(ValueError, match="1 entries for 2 blocks"):
+        pkg.packed_dit_forward([None] * 2, **{**args, "crosses": [[None] * 2] * 2}, adapters=[none], tables=f(2, 6, 128))

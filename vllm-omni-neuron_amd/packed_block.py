@@ -166,6 +166,8 @@ def packed_dit_forward(blocks, h: torch.Tensor, temb: torch.Tensor, packed: Pack
         raise ValueError(f"h {list(h.shape)} and positions {list(positions.shape)} do not fit {packed.rows} rows")
     if tuple(temb.shape) != (count, 6, dim) or len(crosses) != len(blocks) or any(len(c) != count for c in crosses):
         raise ValueError(f"temb and every block's crosses need one entry for each of {count} requests")
+    if adapters and len(adapters) != len(blocks):
+        raise ValueError(f"adapters: {len(adapters)} entries for {len(blocks)} blocks (None where a block has none)")
     if adapter_ids is not None and tuple(adapter_ids.shape) != (count,):
         raise ValueError(f"adapter_ids must be [{count}], got {list(adapter_ids.shape)}")
     if tables is None:

@@ -274,3 +274,75 @@ def test_one_row_of_vectors_serves_one_request(pkg, dev, T):
     assert torch.equal(every[0][mine], r[mine]) and torch.equal(every[1][mine], y[mine])
     mixed = pkg.adaln_sandwich(to(h), to(res), to(mul).expand(2, H).contiguous(), to(add), gate=to(gate), **kw)
     assert all(torch.equal(a, b) for a, b in zip(every, mixed)) and bool(every[0][(ids == 1).to(dev)].any(1).all())
+
+
+@pytest.mark.parametrize("post,norm", [("rms_norm", "layer_norm"), ("layer_norm", "rms_norm"), ("none", "none"), ("layer_norm", "layer_norm")])
+@pytest.mark.parametrize("H", [32, 512, 544, 1024, 1056, 1536, 2048, 2080, 2592, 3040, 3104, 3616, 4096, 4128, 4608, 4640, 5088])
+def test_many_rows_of_every_length(pkg, dev, H, post, norm):
+    """More rows than two for every CU, in rows of one to ten pieces of 512 with whole and ragged last ones; requests
+    that end inside a workgroup's eight rows, and rows of none between them."""
+    ids = ref.packed_ids([1, 300, 0, 205, 83], 9)
+    ids[[40, 41, 320]] = -1
+    h, res, w, gate, mul, add = _inputs(len(ids), H, 5, H + 1, shift=0.5)
+    _check(pkg, dev, h, res, w, gate, mul, add, ids, alpha=-0.5, post=post, norm=norm)
+
+
+@pytest.mark.parametrize("H", [96, 1536, 2592, 4640, 5120, 5152])
+def test_many_quantized_rows_are_those_of_the_bf16_output(pkg, dev, H):
+    T, live = 611, 607
+    ids = ref.packed_ids([200, 407], 4).to(dev)
+    h, res, w, gate, mul, add = (t.to(dev) for t in _inputs(T, H, 2, H))
+    kw = dict(eps=EPS, post_norm="none", gate=gate, request_ids=ids)
+    r, y = pkg.adaln_sandwich(h, res, mul, add, **kw)
+    for quant in ("mx", "row"):
+        r2, q = pkg.adaln_sandwich(h, res, mul, add, quant=quant, **kw)
+        want = pkg.adaln_modulate(y, eps=EPS, norm_type="none", quant=quant)
+        assert torch.equal(r, r2)
+        for got, full in zip(q if quant == "mx" else (q,), want if quant == "mx" else (want,)):
+            got, full = got.view(torch.uint8), full.view(torch.uint8)
+            assert torch.equal(got[:live], full[:live]) and not got[live:].any()
+
+
+@pytest.mark.parametrize("H", [1536, 4640, 5120, 13824])
+def test_many_rows_in_place_strided_and_sliced_modulation(pkg, dev, H):
+    T, R = 700, 3
+    g = torch.Generator(device=dev).manual_seed(15)
+    wide = torch.randn(T, 2 * H + 64, device=dev, generator=g).to(torch.bfloat16)
+    h, res = wide[:, :H], wide[:, H + 32 : 2 * H + 32]
+    mod = torch.randn(R, 6, H, device=dev, generator=g)
+    ids = (torch.arange(T, device=dev) * (R + 1) // T - 1).to(torch.int32)
+    kw = dict(eps=EPS, request_ids=ids)
+    want = pkg.adaln_sandwich(h.contiguous(), res.contiguous(), mod[:, 1].contiguous(), mod[:, 0].contiguous(), gate=mod[:, 2].contiguous(), **kw)
+    got = pkg.adaln_sandwich(h, res, mod[:, 1], mod[:, 0], gate=mod[:, 2], **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    h2, r2 = h.contiguous(), res.contiguous()
+    pkg.adaln_sandwich(h2, r2, mod[:, 1], mod[:, 0], gate=mod[:, 2], residual_out=r2, out=h2, **kw)
+    live = ids >= 0
+    assert torch.equal(r2[live], want[0][live]) and torch.equal(h2[live], want[1][live])
+    assert torch.equal(r2[~live], res[~live]) and torch.equal(h2[~live], h[~live])
+    # the sum over hidden, the second output over the residual
+    h2, r2 = h.contiguous(), res.contiguous()
+    pkg.adaln_sandwich(h2, r2, mod[:, 1], mod[:, 0], gate=mod[:, 2], residual_out=h2, out=r2, **kw)
+    assert torch.equal(h2[live], want[0][live]) and torch.equal(r2[live], want[1][live])
+
+
+@pytest.mark.parametrize("T,H", [(600, 5152), (1100, 8192), (1030, 13824), (601, 16384)])
+def test_many_rows_longer_than_a_wave_holds(pkg, dev, T, H):
+    """A workgroup goes through several rows: requests change between them, and some belong to none."""
+    ids = torch.randint(-1, 3, (T,), generator=torch.Generator().manual_seed(T), dtype=torch.int32)
+    h, res, w, gate, mul, add = _inputs(T, H, 3, 81)
+    _check(pkg, dev, h, res, w, gate, mul, add, ids, post="layer_norm")
+
+
+def test_a_workgroup_of_more_rows_than_it_looks_up_at_once(pkg, dev):
+    """17000 rows of 5152: more than 64 to each of 256 workgroups. Every row as in a batch of 250."""
+    T, H = 17000, 5152
+    g = torch.Generator(device=dev).manual_seed(83)
+    h, res = (torch.randn(T, H, device=dev, generator=g).to(torch.bfloat16) for _ in range(2))
+    gate, mul, add = (torch.randn(4, H, device=dev, generator=g) for _ in range(3))
+    ids = torch.randint(-1, 4, (T,), device=dev, generator=g, dtype=torch.int32)
+    r, y = pkg.adaln_sandwich(h, res, mul, add, eps=EPS, gate=gate, quant="mx", request_ids=ids)
+    for at in range(0, T, 250):
+        s = slice(at, at + 250)
+        r2, y2 = pkg.adaln_sandwich(h[s], res[s], mul, add, eps=EPS, gate=gate, quant="mx", request_ids=ids[s].clone())
+        assert torch.equal(r[s], r2) and torch.equal(y.codes.view(torch.uint8)[s], y2.codes.view(torch.uint8)) and torch.equal(y.scales[s], y2.scales)

@@ -267,3 +267,16 @@ def test_a_weight_of_one_head_at_an_odd_float(pkg, dev, pairs):
     buf[1:129], buf[150:278] = gq, gk
     got = pkg.qk_norm_rope_axes(q, k, pos, rope_pairs=pairs, norm="rms_norm", q_gamma=buf[1:129], k_gamma=buf[150:278])
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("hq,hk,D", [(23, 20, 128), (22, 3, 128), (32, 32, 128), (31, 29, 128), (64, 16, 64), (36, 40, 128), (40, 40, 128), (48, 48, 128),
+                                     (45, 6, 128), (64, 64, 128), (60, 8, 128), (30, 32, 256), (1, 60, 128), (65, 3, 128), (128, 128, 128), (512, 400, 32)])
+@pytest.mark.parametrize("pairs", ["interleaved", "halves"])
+@pytest.mark.parametrize("norm", ["rms_norm", "rms_norm_across_heads"])
+def test_rows_of_every_width(pkg, dev, hq, hk, D, pairs, norm):
+    """Up to 16384 channels in both layouts of the pairs, Q and K of equal and of unequal widths; requests that meet inside
+    a workgroup's eight rows."""
+    axes = {32: (8, 8), 64: (8, 12, 12), 128: (44, 42, 42), 256: (64, 96, 80)}[D]
+    ids = ref.packed_ids([5, 9, 0, 18], 3)
+    ids[20] = -1
+    _check(pkg, dev, *_inputs(35, hq, hk, D, norm, hq + hk, axes=len(axes)), ids=ids, axes=axes, pairs=pairs, norm=norm)

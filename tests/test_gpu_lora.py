@@ -292,3 +292,17 @@ def test_more_rows_than_requests_without_request_ids(pkg, dev, T, rank, zero_res
     pkg._lib.call("wanmi_lora_add", 0, p(x), None, None, K, p(a), p(b), p(scales), p(ids), None, R, 2, T, K, N, rank, 1, pkg.lora._widths((N,)), p(base), N,
                   p(out), N, zero_rest, p(work), size)
     assert torch.equal(out[:R], want[:R]) and bool((out[R:] == (0.0 if zero_rest else 3.0)).all())
+
+
+@pytest.mark.parametrize("kind", ["bf16", "mx", "row"])
+@pytest.mark.parametrize("K,slices,r", [
+    (1664, (256,), 16),  # 13 pairs of steps of K in two splits, the second one shorter
+    (2944, (192,), 32), (2944, (64, 128), 64), (2944, (136,), 128),  # 23 pairs in three, the last one shorter
+    (5120, (256,), 32), (5120, (128, 64, 64), 64), (5120, (320,), 128),  # 40 pairs in four
+    (13824, (64,), 32), (13824, (128,), 96), (13824, (72,), 128), (13824, (64,), 160),  # 108 pairs in six
+])
+def test_many_rows_in_several_splits_of_k(pkg, dev, kind, K, slices, r):
+    ids = ref.packed_ids([500, 0, 413, 200], 5)
+    base, x, a, b, scales = _inputs(len(ids), K, slices, 3, r, K + r)
+    adapters = torch.tensor([1, 0, -1, 2], dtype=torch.int32)
+    _check(pkg, dev, base, x, a, b, scales, slices, adapters, ids, kind=kind)

@@ -289,3 +289,15 @@ def test_packed_forward_refuses_what_does_not_fit(pkg):
             pkg.packed_dit_forward([None], **{**args, **kw}, tables=f(1, 6, 128))
     with pytest.raises(ValueError, match="1 entries for 2 blocks"):
         pkg.packed_dit_forward([None] * 2, **{**args, "crosses": [[None] * 2] * 2}, adapters=[none], tables=f(2, 6, 128))
+
+
+def test_qk_axes_refuses_before_it_clears_the_bounds(pkg):
+    """With a bound asked for, too: null pointers, strides and alignment are argument errors, no launch."""
+    lib, dims, freqs = pkg._lib.load(), (ctypes.c_int * 1)(16), (ctypes.c_double * 8)()
+
+    def qk(q=16, k=16, ts=64, pos=16, gq=None):
+        return lib.wanmi_qk_norm_rope_axes(q, ts, 64, 1, gq, 16, 64, 64, k, 64, 64, 1, None, 16, 64, 64, 4, 64, pos, 0, 1, dims, freqs, 0, 2, 1e-6,
+                                           None, 1, 1, 16, None)
+
+    for kw in (dict(q=None), dict(k=None), dict(ts=4), dict(ts=-64), dict(q=8), dict(pos=None), dict(gq=20)):
+        assert qk(**kw) == pkg._lib.WANMI_ERR_ARG, kw

@@ -365,15 +365,15 @@ extern "C" int wanmi_qk_norm_rope_axes(const void* q, int64_t q_token_stride, in
   const int most = 16384;
   WANMI_REQUIRE((int64_t)q_heads * head_dim <= most && (int64_t)k_heads * head_dim <= most, WANMI_ERR_UNSUPPORTED,
                 "%s: heads * head_dim exceeds %d", f, most);
+  const int64_t bounds = k_maxnorm ? requests * k_heads : 0;
+  WANMI_REQUIRE(bounds < (1LL << 31), WANMI_ERR_ARG, "%s: %lld requests of %d heads are too many", f, (long long)requests, k_heads);
   hipStream_t s = (hipStream_t)stream;
-  if (k_maxnorm) {
-    const int64_t n = requests * k_heads;
-    WANMI_REQUIRE(n < (1LL << 31), WANMI_ERR_ARG, "%s: %lld requests of %d heads are too many", f, (long long)requests, k_heads);
-    hipLaunchKernelGGL(qk_axes_zero_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, k_maxnorm, n);
-    const int st = check_launch(f);
-    if (st != WANMI_OK) return st;
-  }
-  if (T == 0) return WANMI_OK;
+  const auto clear_bounds = [&]() {
+    if (!bounds) return (int)WANMI_OK;
+    hipLaunchKernelGGL(qk_axes_zero_kernel, dim3((unsigned)((bounds + 255) / 256)), dim3(256), 0, s, k_maxnorm, bounds);
+    return check_launch(f);
+  };
+  if (T == 0) return clear_bounds();
   WANMI_REQUIRE(q && (positions || !rot) && q_out && (!k_heads || (k && k_out)), WANMI_ERR_ARG, "%s: null pointer", f);
   const int64_t strides[8] = {q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride,
                               k_heads ? k_token_stride : 0, k_heads ? k_head_stride : 0, k_heads ? k_out_token_stride : 0,
@@ -403,6 +403,8 @@ extern "C" int wanmi_qk_norm_rope_axes(const void* q, int64_t q_token_stride, in
   a.zero_rest = zero_rest;
   a.eps = eps;
   a.kmax = k_maxnorm;
+  const int cleared = clear_bounds();
+  if (cleared != WANMI_OK) return cleared;
   const int units = (k_heads > q_heads ? k_heads : q_heads) * (head_dim / 16);
   const int nu = (units + 63) / 64;
   if (rope_pairs == WANMI_ROTATE_HALVES) launch_qk_axes<true>(a, nu, s);

@@ -403,7 +403,8 @@ int wanmi_qk_norm_rope_axes(const void* q, int64_t q_token_stride, int64_t q_hea
 /*
  * Low-rank adapters of many requests beside a shared projection:
  *   out[t, n] = bf16(base[t, n] + sum_j B[e][n, j] u[t, p(n) rank + j]),
- *   u[t, i] = adapter_scales[e] * row_scale[t] * sum_k A[e][i, k] x[t, k]           (fp32)
+ *   u[t, i] = adapter_scales[e] * row_scale[t] * sum_k A[e][i, k] x[t, k]
+ * Both sums in fp32; u, fp32 as well, enters the second one as two bf16 values (to 2^-16 of itself).
  * x: bf16 [T, K], rows ldx elements apart, or with x_scales (e8m0 [T, K/32]) e4m3fn codes, rows ldx bytes apart
  * (16-byte aligned rows); row_scale fp32 [T] or NULL. A: bf16 [adapters, parts * rank, K]; B: bf16
  * [adapters, N, rank]; the columns of a fused projection fall into `parts` runs of part_widths (HOST array; multiples
@@ -422,7 +423,7 @@ int wanmi_lora_add(const void* x, const uint8_t* x_scales, const float* row_scal
                    const void* base, int64_t ldb, void* out, int64_t ldo, int zero_rest, void* workspace,
                    int64_t workspace_bytes, void* stream);
 
-/* Bytes of workspace that wanmi_lora_add needs for these sizes on the current device (0 where there is nothing to compute). */
+/* Bytes of workspace that wanmi_lora_add needs for these sizes, on any device (0 where there is nothing to compute). */
 int64_t wanmi_lora_workspace(int64_t T, int64_t K, int parts, int rank);
 
 /*

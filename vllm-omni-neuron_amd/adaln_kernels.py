@@ -241,9 +241,10 @@ def adaln_sandwich(
     :func:`adaln_modulate`.
 
     ``request_ids`` int32 ``[T]`` names each row's request q (None: every row is request 0). A row whose id is
-    negative, or at least R, belongs to none: it is not computed, and its rows of ``residual_out`` and ``out`` are left
+    negative, or at least R where a vector has R rows, belongs to none: it is not computed, and its rows of ``residual_out`` and ``out`` are left
     as they are where the caller gave them, zeros where they are allocated here. ``residual_out`` may be
-    ``residual`` and ``out`` (contiguous; an :class:`MXTensor` for ``quant="mx"``) may be ``hidden``.
+    ``residual`` and ``out`` (contiguous; an :class:`MXTensor` for ``quant="mx"``) may be ``hidden``; no output may
+    share memory with anything else.
     """
     if out is None and residual_out is None:
         r = _sandwich_plain(hidden, residual, mul, add, eps, post_norm, post_weight, gate, residual_scale, norm_type, quant,

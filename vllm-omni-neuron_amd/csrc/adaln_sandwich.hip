@@ -20,7 +20,8 @@
 // vectors of its rows' request into LDS while the rows are under way (where the eight rows belong to several requests, each
 // wave reads its own from L2). A wave takes one row and ends: in a loop, the loads of the next row stand
 // behind the stores of this one in the order that a wave waits for them, and 32760 rows took 343 us instead of 257
-// (5.2 TB/s of the 5.5 that a large copy reaches here).
+// (5.2 TB/s of the 5.5 that a large copy reaches here; with MX codes 226 to 231, ROW 237 to 247, without and with a norm
+// before the gate).
 //
 // Few rows: a workgroup owns a row, a thread 8 columns of it (kNC runs of them), so that all of its waves share the
 // row's latency: 5.5 us for 7 rows where a wavefront each takes 12.
@@ -532,7 +533,7 @@ void launch_few(const SandwichArgs& a, hipStream_t s) {
 }
 
 template <int NCH>
-int launch_many(SandwichArgs a, int cus, hipStream_t s) {
+int launch_many(const SandwichArgs& a, hipStream_t s) {
   constexpr int bytes = 8192 * NCH;  // four fp32 vectors of whole chunks
   static int allowed[64] = {0};
   int dev = 0;
@@ -617,7 +618,10 @@ extern "C" int wanmi_adaln_sandwich(const void* hidden, int64_t ld_hidden, const
   const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
   const int nch = (int)((H + 511) / 512);
   if (T <= 2 * cus || nch > 10) {
-    // few rows, or more of a row than a wave's registers hold
+    // few rows, or more of a row than a wave's registers hold. A workgroup / a wave a row, us: 5120 columns 256 rows 6.4 /
+    // 15.8, 512 11.2 / 17.1, 640 16.3 / 17.7, 1024 17.3 / 20.0, 1560 26.3 / 17.1, 4096 46 / 34; 1536 columns 512 rows 5.2 / 6.4,
+    // 1024 6.5 / 6.7, 1560 9.0 / 7.4, 4096 15.2 / 13.0 (the bf16 form; MX codes cross at the same places). Past 5120 columns
+    // there is the first alone: 7800 rows of 8192 116 us, of 13824 344 (8 bytes a column at 5.5 TB/s: 93 and 157).
     const int waves = H <= 8192 ? nch : (nch + 1) / 2;
     const int64_t resident = (int64_t)cus * (waves <= 10 ? 20 / waves : 1);
     a.rows_each = (T + resident - 1) / resident;
@@ -626,15 +630,15 @@ extern "C" int wanmi_adaln_sandwich(const void* hidden, int64_t ld_hidden, const
     return check_launch("wanmi_adaln_sandwich");
   }
   switch (nch) {
-    case 1: return launch_many<1>(a, cus, s);
-    case 2: return launch_many<2>(a, cus, s);
-    case 3: return launch_many<3>(a, cus, s);
-    case 4: return launch_many<4>(a, cus, s);
-    case 5: return launch_many<5>(a, cus, s);
-    case 6: return launch_many<6>(a, cus, s);
-    case 7: return launch_many<7>(a, cus, s);
-    case 8: return launch_many<8>(a, cus, s);
-    case 9: return launch_many<9>(a, cus, s);
-    default: return launch_many<10>(a, cus, s);
+    case 1: return launch_many<1>(a, s);
+    case 2: return launch_many<2>(a, s);
+    case 3: return launch_many<3>(a, s);
+    case 4: return launch_many<4>(a, s);
+    case 5: return launch_many<5>(a, s);
+    case 6: return launch_many<6>(a, s);
+    case 7: return launch_many<7>(a, s);
+    case 8: return launch_many<8>(a, s);
+    case 9: return launch_many<9>(a, s);
+    default: return launch_many<10>(a, s);
   }
 }

@@ -569,7 +569,7 @@ __global__ __launch_bounds__(256, 2) void lora_expand_many_kernel(LoraArgs a) {
   const int v0 = row_adapter(a, t0 + lane), v1 = row_adapter(a, t0 + 64 + lane);
   int e = next_adapter(v0, v1, -1);
   // u of the wave's rows (two groups of 16) as the MFMA's operand: high and low halves. The splits of K are added two at a time
-  // with all of their loads under way (one by one, each a memory latency, 4096 rows x 5120 columns of ten splits took 38 us instead of 32).
+  // with all of their loads under way (4096 rows x 5120 columns, rank 32, four splits: 38.5 us a call, one by one 39.0).
   bf16x8 uh[2][kKS], ul[2][kKS];
   {
     float f[2][kKS][8];
@@ -742,7 +742,19 @@ __global__ __launch_bounds__(256, 2) void lora_expand_many_kernel(LoraArgs a) {
 }
 
 // Which kernels a call takes. Many rows take the large tiles: below 1024 rows there are too few of them
-// to fill the chip, and K that is no multiple of 128 is left to the other, as are rows past its 32-bit offsets.
+// to fill the chip. Whole calls in us, N = 5120, small tiles / large tiles, MX:
+//   rows                                          512         1024        2048        4096
+//   K =  5120, rank  16,  1 adapter            10.9 / 16.8 15.2 / 20.1 19.8 / 23.2 30.1 / 28.8
+//   K =  5120, rank  32,  8 adapters           16.3 / 21.8 21.2 / 23.4 29.7 / 25.5 42.7 / 32.4
+//   K =  5120, rank  64,  4 adapters           19.4 / 26.1 28.7 / 31.2 37.6 / 33.8 56.0 / 40.5
+//   K = 13824, rank 128,  1 adapter            29.1 / 70.3 42.0 / 82.0 66.6 / 86.1 118  / 111
+// So from 1024 rows to the crossing (2048, at one adapter 3000 to 4000) the small tiles would do as well or better,
+// most of all at rank 128; the bound is the number of rows alone.
+// K that is no multiple of 128 is left to the small tiles, as are rows past the large ones' 32-bit offsets: their
+// rows of A come from L2 again for every 32 rows. 32760 rows, MX, K = 5088 against 5120: rank 16 221 / 186 us, 32 243 /
+// 188, 64 275 / 194, 128 349 / 225 (4096 rows: 29 / 29, 34 / 32, 44 / 39, 66 / 78; K = 1504 against 1536 at 32760: 166 / 159 to
+// 214 / 190).
+// The chip's 256 CUs are constants here: the caller sizes the workspace by the same plan, on whichever device is current.
 struct LoraPlan {
   bool big;
   int nr;  // ranks of a workgroup (big)

@@ -95,7 +95,9 @@ def lora_add(base: torch.Tensor, x, a: torch.Tensor, b: torch.Tensor, adapter_id
     is negative (or not below R) belongs to no request and is not computed: left as it is in a given ``out``, zeros
     in one allocated here. ``out`` may be ``base``.
 
-    The sums are fp32 throughout, with one rounding to bf16 at the end.
+    Both sums are fp32, and the output is rounded once; between them ``u = scales[e] * (x[t] @ a[e].T)`` enters the
+    second product as two bf16 values, to 2^-16 of itself. From 1024 rows on, K that is a multiple of 128 is faster than K
+    that is not (1.2 to 1.8 times at 32760 rows and K about 5000). A ROW-packed ``x`` is unpacked by a launch of its own first.
     """
     if out is None and (slices is None or type(slices) is tuple):
         done = _add_plain(base, x, a, b, adapter_ids, scales, slices, request_ids)

@@ -1,7 +1,10 @@
 """The Wan2.2 DiT blocks over a packed batch: several requests of different sizes, timesteps and adapters at once.
 
 The rows of all requests lie one behind the other in one ``[rows, dim]`` tensor (:class:`PackedRequests`), so that a
-weight is read once for all of them and small requests fill the chip together. Per request differ the modulation
+weight is read once for all of them and small requests fill the chip together: a block of dim 5120 on 16 requests of
+16 tokens takes 0.82 ms and 3.95 one request after another, 8 of 390 tokens 1.50 and 2.47, 4 of 1560 2.12 and 2.62, 2 of 7800
+6.22 and 6.42. Attention runs request by request, and one request alone is faster through :func:`.block.dit_forward`
+(7800 tokens: 3.30 here, 3.22 there). Per request differ the modulation
 (one row of the timestep embedding each), the grid (positions given per token), the text context and the
 low-rank adapters. A block is that of :mod:`.block` with each request's own
 
@@ -25,7 +28,7 @@ import torch
 
 from . import attention_ops as ops
 from .adaln_kernels import adaln_sandwich
-from .block import HEAD_DIM, BlockWeights, CrossKV, modulation
+from .block import HEAD_DIM, BlockWeights, modulation
 from .common_types import MXTensor
 from .lora import lora_add
 from .row_mx_kernels import mxfp8_linear
@@ -80,7 +83,11 @@ class Adapters(NamedTuple):
 
 
 class BlockAdapters(NamedTuple):
-    """Adapters of a block's projections (None: that projection has none). ``qkv`` in three slices of ``dim`` columns."""
+    """Adapters of a block's projections (None: that projection has none). ``qkv`` in three slices of ``dim`` columns.
+
+    The FFN's up projection takes none: its GELU and quantization are in the GEMM's epilogue. Nor do the text's K and V,
+    which :func:`.block.project_cross_kv` projects once per generation: an adapter of theirs can be merged into the
+    weights that it is given, request by request."""
 
     qkv: Adapters | None = None
     o: Adapters | None = None
@@ -187,5 +194,5 @@ def packed_dit_forward(blocks, h: torch.Tensor, temb: torch.Tensor, packed: Pack
 def packed_block_forward(w: BlockWeights, h: torch.Tensor, temb: torch.Tensor, packed: PackedRequests, positions: torch.Tensor,
                          crosses, eps: float = 1e-6, adapters: BlockAdapters | None = None,
                          adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
-    """One block over a packed batch (:func:`packed_dit_forward` with one block); ``crosses``: one :class:`.CrossKV` per request."""
+    """One block over a packed batch (:func:`packed_dit_forward` with one block); ``crosses``: one :class:`.block.CrossKV` per request."""
     return packed_dit_forward([w], h, temb, packed, positions, [crosses], eps, None if adapters is None else [adapters], adapter_ids)

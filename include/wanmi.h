@@ -427,6 +427,36 @@ int wanmi_lora_add(const void* x, const uint8_t* x_scales, const float* row_scal
 int64_t wanmi_lora_workspace(int64_t T, int64_t K, int parts, int rank);
 
 /*
+ * Attention of packed rows over packed texts: the rows [q_offsets[r], q_offsets[r + 1]) of q over the keys and values
+ * [k_offsets[r], k_offsets[r + 1]), request by request, in one launch:
+ *   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - max)          (no keys: zeros)
+ * q: bf16, element (i, h, d) at i * q_ss + h * q_hs + d; k, v likewise with k_heads heads (heads a multiple of k_heads, query
+ * head h reads key head h / (heads / k_heads)); strides multiples of 8 below 2^22, 16-byte aligned tensors. head_dim 64 or 128.
+ * q_offsets, k_offsets: int32 [requests + 1] on the device, ascending from 0, held inside [0, T] and [0, Tk] (below 2^28).
+ * out: bf16 [T, heads * head_dim], rows o_ss elements apart (a multiple of 16), may be q element for element; with out_scales (uint8
+ * [T, heads * head_dim / 32]) e4m3fn codes and e8m0 scales as wanmi_mxfp8_gemm reads them. Rows behind the last request
+ * are left, or zeroed with zero_rest. scale positive. Sums and the softmax in fp32, p enters the second product as bf16.
+ * Stands beside wanmi_attention_const_max (one sequence, a bound in place of the maximum); no reference counterpart.
+ */
+int wanmi_packed_cross_attention(const void* q, int64_t q_ss, int64_t q_hs, const void* k, int64_t k_ss, int64_t k_hs,
+                                 const void* v, int64_t v_ss, int64_t v_hs, const int32_t* q_offsets, const int32_t* k_offsets,
+                                 int64_t requests, int64_t T, int64_t Tk, int64_t heads, int64_t k_heads, int head_dim, float scale,
+                                 void* out, int64_t o_ss, uint8_t* out_scales, int zero_rest, void* stream);
+
+/*
+ * Self-attention of packed prompts with a learned bias by buckets of relative distance:
+ *   p_j = exp(scale q_i.k_j + table[bucket(j - i), h] - max)               over the tokens j of row i's prompt
+ * q, k, v, offsets, out, zero_rest as above (as many key heads as heads; no codes). table: fp32 or (table_bf16) bf16
+ * [buckets, heads]. starts: HOST array, the smallest distance of each of the `side` buckets of one direction (at most 128), ascending
+ * from 0 to at most 1024. both: buckets [0, side) are for j <= i, [side, 2 side) for j > i; else [0, side) for j <= i, and j > i
+ * takes bucket 0. No reference counterpart.
+ */
+int wanmi_relative_bias_attention(const void* q, int64_t q_ss, int64_t q_hs, const void* k, int64_t k_ss, int64_t k_hs,
+                                  const void* v, int64_t v_ss, int64_t v_hs, const int32_t* offsets, int64_t requests, int64_t T,
+                                  int64_t heads, int head_dim, float scale, const void* table, int table_bf16, const int* starts,
+                                  int side, int both, void* out, int64_t o_ss, int zero_rest, void* stream);
+
+/*
  * Streaming device-to-device copy of `bytes` (a multiple of 16; src and dst 16-byte aligned, not
  * overlapping) on `stream`: 16-byte loads, eight per thread in flight before its non-temporal
  * stores, one 32 KiB chunk per workgroup. Measurement infrastructure with no counterpart in the

@@ -34,6 +34,7 @@ from .attention_ops import (  # noqa: F401
     row_mx_qkv_proj,
     wan_cp_self_attention,
 )
+from .packed_attention import packed_cross_attention, relative_bias_attention  # noqa: F401
 attention_ops.register_torch_ops()
 from . import block  # noqa: F401
 from . import comfy_fp8_checkpoint  # noqa: F401

@@ -77,6 +77,10 @@ _SIGNATURES = {
     "wanmi_lora_add": [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _vp, _vp, _i64,
                        _vp, _i64, _i32, _vp, _i64, _vp],
     "wanmi_lora_workspace": [_i64, _i64, _i32, _i32],
+    "wanmi_packed_cross_attention": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                                     _i32, _f32, _vp, _i64, _vp, _i32, _vp],
+    "wanmi_relative_bias_attention": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _f32, _vp,
+                                      _i32, _vp, _i32, _i32, _vp, _i64, _i32, _vp],
 }
 
 _LIB = None

@@ -1,0 +1,504 @@
+// Attention of packed rows over packed texts for gfx950, bf16 MFMA with fp32 softmax and sums.
+//
+//   o_i = sum_j exp(s q_i.k_j + b(j - i) - m_i) v_j / sum_j exp(s q_i.k_j + b(j - i) - m_i)
+//
+// The queries of request r are rows [q_off[r], q_off[r + 1]) of the batch, its keys and values rows [k_off[r],
+// k_off[r + 1]) of the texts: all requests in one launch, nothing padded between them. b is absent (cross-attention) or a
+// learned bias of the head for the bucket of the distance j - i (a text encoder's self-attention). A request without
+// keys gives zeros. The offsets are read on the GPU and held inside the tensors, so that no offset reads or writes
+// out of bounds; ascending ones that start at 0 are the caller's part.
+//
+// A workgroup of four waves takes one head of one tile of a request's rows: 128 rows, 32 per wave, all waves over the same
+// keys (kSplit 1), or 32 rows with the keys shared out over the waves and their parts joined through LDS at the end
+// (kSplit 4: few rows per request). K and V pass through LDS in tiles of 64 (128) keys, loaded straight into it while the
+// tile before is computed. S^T = K Q^T puts a row's scores into one lane (and lane ^ 32), so that the softmax is lane-local, and
+// its P^T is the operand of O^T = V^T P^T as it stands. V stays [key][d] in LDS; its columns are read by the transposing LDS read
+// (ds_read_b64_tr_b16: 16 lanes read four keys x 16 d and get one d's four keys each).
+//
+// The maximum m of a row is one that its running maximum may exceed by 2^8 before sums and outputs are rescaled: P then reaches
+// 2^8 instead of 1, which costs bf16 and fp32 no precision, and nearly every tile after the first goes without a rescale.
+#include "wanmi_common.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace wanmi {
+
+constexpr int kMaxSide = 128;         // bias buckets of one direction
+constexpr int kMaxSaturation = 1024;  // the distance from which on a direction's last bucket holds
+constexpr float kSlack = 8.0f;        // log2 units
+
+struct PackedAttnArgs {
+  const uint16_t* q;  // row i, head h at q + i * q_ss + h * q_hs
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t q_ss, q_hs, k_ss, k_hs, v_ss, v_hs;
+  const int* q_off;  // [requests + 1]
+  const int* k_off;
+  int requests;
+  int T, Tk;
+  int heads, group;   // query heads, and how many of them share a key head
+  float scale_log2;   // s log2(e)
+  void* out;          // bf16 [T, heads * D], or e4m3 codes
+  int64_t o_ss;
+  uint8_t* out_scales;  // MX: [T, heads * D / 32]
+  int zero_rest;        // rows behind the last request: written as zeros, or left
+  int tiles, per_xcd;   // tiles of rows (an upper bound), workgroups per XCD
+};
+
+struct BiasArgs {
+  const void* table;  // [buckets, heads], fp32 or bf16
+  int bf16;
+  int side;           // buckets of one direction
+  int both;           // buckets for later keys follow those for earlier ones; else every later key takes bucket 0
+  int start[kMaxSide];  // smallest distance of each bucket
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float max_lane_xor32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// LDS tiles of K and V: rows of D bf16, 16-byte chunk c of a key's row in slot c ^ f(key). K is read 16 keys to a cycle,
+// one chunk of each; V four keys to a cycle, 64 bytes of each: f spreads both over all banks.
+template <int D>
+__device__ __forceinline__ int k_slot(int key) {
+  return D == 128 ? key & 15 : (key & 7) ^ ((key >> 3) & 1);
+}
+template <int D>
+__device__ __forceinline__ int v_slot(int key) {
+  return D == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2;
+}
+
+// The tile `t` of the launch: its request, rows and keys. Every wave finds it for itself, 64 requests at a time. The rows behind the last
+// request are one more request, without keys. False: no rows.
+template <int kRows>
+__device__ __forceinline__ bool find_tile(const PackedAttnArgs& a, int t, int& row0, int& rows, int& in_request, int& k0, int& keys) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int c = 0; c <= a.requests; c += 64) {
+    const int r = min(c + lane, a.requests);
+    const int lo = min(max(a.q_off[r], 0), a.T);
+    int hi = r < a.requests ? min(max(a.q_off[r + 1], 0), a.T) : a.zero_rest ? a.T : lo;
+    if (c + lane > a.requests) hi = lo;
+    int sum = max(hi - lo + kRows - 1, 0) / kRows;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int s = __shfl_up(sum, o, 64);
+      sum += lane >= o ? s : 0;
+    }
+    sum += before;
+    const uint64_t hit = __ballot(sum > t);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      const int first = __builtin_amdgcn_readfirstlane(l ? __shfl(sum, l - 1, 64) : before);
+      const int at = __builtin_amdgcn_readfirstlane(__shfl(lo, l, 64)), end = __builtin_amdgcn_readfirstlane(__shfl(hi, l, 64));
+      in_request = (t - first) * kRows;
+      if (in_request < 0 || in_request >= end - at) return false;
+      row0 = at + in_request;
+      rows = min(kRows, end - row0);
+      const int q = c + l;
+      k0 = keys = 0;
+      if (q < a.requests) {
+        k0 = min(max(a.k_off[q], 0), a.Tk);
+        keys = max(min(max(a.k_off[q + 1], 0), a.Tk) - k0, 0);
+      }
+      k0 = __builtin_amdgcn_readfirstlane(k0);
+      keys = __builtin_amdgcn_readfirstlane(keys);
+      return true;
+    }
+    before = __builtin_amdgcn_readfirstlane(__shfl(sum, 63, 64));
+  }
+  return false;
+}
+
+// 16 outputs of a lane (d = 8 g + 4 hq + q of a block of 32) as bf16 pairs; kMx: as four words of codes and the block's
+// scale byte. The block's other half is lane ^ 32's.
+__device__ __forceinline__ int mx_codes(const uint32_t (&pp)[8], uint32_t (&codes)[4]) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 mag = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) mag = __builtin_elementwise_max(mag, __builtin_bit_cast(u16x2, pp[i] & 0x7FFF7FFFu));
+  const int e = max_with_lane_xor32((int)(max(mag[0], mag[1]) >> 7));
+  const int sx = max(e - 7, 0);
+  const float sc = __uint_as_float((uint32_t)sx << 23);
+#pragma unroll
+  for (int g = 0; g < 4; ++g) codes[g] = cvt_e4m3x4_scaled(pp[2 * g], pp[2 * g + 1], sc);
+  return sx;
+}
+
+template <int D, bool kBias, int kSplit, bool kMx>
+__global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs a, BiasArgs bias) {
+  constexpr int kRows = 128 / kSplit;              // rows of a workgroup
+  constexpr int kHalves = kSplit == 1 ? 2 : 1;     // 32-key halves of a wave's part of a tile
+  constexpr int kKeys = kSplit == 1 ? 64 : 128;    // keys of a tile
+  constexpr int kRowB = 2 * D;                     // bytes
+  constexpr int kChunks = D / 8;
+  constexpr int kTile = kKeys * kRowB;             // of K, and as much of V
+  constexpr int kLoads = kTile / 4096;             // per wave, of each
+  constexpr int kRing = 2;
+  constexpr int kJoin = kSplit == 1 ? 0 : kSplit * 32 * (D * 4 + 8);
+  constexpr int kLds = kRing * 2 * kTile > kJoin ? kRing * 2 * kTile : kJoin;
+  constexpr int kBiasLds = kBias ? 2 * (kMaxSaturation + 63) + 2 : 1;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
+  __shared__ float sbias[kBiasLds];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, hq = lane >> 5;
+  // XCD x takes a contiguous run of (head, tile): the tiles of a head read the same keys
+  const int in_xcd = blockIdx.x >> 3;
+  const int work = (int)(blockIdx.x & 7) * a.per_xcd + in_xcd;
+  if (in_xcd >= a.per_xcd || work >= a.tiles * a.heads) return;
+  const int head = work / a.tiles;
+  int row0, rows, in_request, k0, keys;
+  if (!find_tile<kRows>(a, work - head * a.tiles, row0, rows, in_request, k0, keys)) return;
+
+  // ---- loads of a tile of keys: four rows (D = 64: eight) to an instruction ----
+  const int khead = head / a.group;
+  const uint16_t* kb = a.k + (int64_t)k0 * a.k_ss + (int64_t)khead * a.k_hs;
+  const uint16_t* vb = a.v + (int64_t)k0 * a.v_ss + (int64_t)khead * a.v_hs;
+  const int lrow = lane / kChunks, lslot = lane % kChunks;
+  constexpr int kPer = 64 / kChunks;  // rows of an instruction
+  const int tiles = (keys + kKeys - 1) / kKeys;
+  auto load_tile = [&](int t) {
+    const int left = min(keys - t * kKeys, kKeys);  // > 0
+    const u32x4 rk = buffer_rsrc(kb + (int64_t)t * kKeys * a.k_ss, (uint32_t)(((left - 1) * a.k_ss + D) * 2));
+    const u32x4 rv = buffer_rsrc(vb + (int64_t)t * kKeys * a.v_ss, (uint32_t)(((left - 1) * a.v_ss + D) * 2));
+    const uint32_t to = lds_addr(lds) + (uint32_t)((t % kRing) * 2 * kTile);
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int r = (wave * kLoads + j) * kPer;  // the instruction's first row; keys past the text read as zeros
+      const int key = r + lrow;
+      lds_dma_b128(rk, (uint32_t)key * (uint32_t)(a.k_ss * 2) + (uint32_t)((lslot ^ k_slot<D>(key)) << 4), to + r * kRowB);
+      lds_dma_b128(rv, (uint32_t)key * (uint32_t)(a.v_ss * 2) + (uint32_t)((lslot ^ v_slot<D>(key)) << 4), to + kTile + r * kRowB);
+    }
+  };
+  if (tiles > 0) load_tile(0);
+
+  // ---- the wave's 32 queries as MFMA operands: lane holds d = 16 t + 8 hq .. + 7 of query col ----
+  const int qw = kSplit == 1 ? wave * 32 : 0;  // the wave's first row in the tile
+  bf16x8 qf[D / 16];
+  {
+    const int r = min(qw + col, rows - 1);  // rows behind the tile's repeat its last and are not written
+    const uint16_t* pq = a.q + (int64_t)(row0 + r) * a.q_ss + (int64_t)head * a.q_hs + 8 * hq;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) qf[t] = *reinterpret_cast<const bf16x8*>(pq + 16 * t);
+  }
+
+  // ---- the head's bias over the distances -(sat + 63) .. sat + 63, in log2 units ----
+  [[maybe_unused]] int sat = 0;
+  [[maybe_unused]] float far_lo = 0.0f, far_hi = 0.0f;
+  if constexpr (kBias) {
+    sat = bias.start[bias.side - 1];
+    for (int i = threadIdx.x; i < 2 * (sat + 63) + 1; i += 256) {
+      const int d = i - (sat + 63), n = abs(d);
+      int b = 0;
+      for (int j = 1; j < bias.side; ++j) b += n >= bias.start[j];
+      if (d > 0) b = bias.both ? b + bias.side : 0;
+      const int at = b * a.heads + head;
+      const float x = bias.bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t*>(bias.table)[at]) : reinterpret_cast<const float*>(bias.table)[at];
+      sbias[i] = x * 1.4426950408889634f;
+    }
+    __syncthreads();
+    far_lo = sbias[0];
+    far_hi = sbias[2 * (sat + 63)];
+  }
+
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
+  float m = -INFINITY, sum = 0.0f;
+  const float c = a.scale_log2;
+  const bf16x2_t ones = {(__bf16)1.0f, (__bf16)1.0f};
+
+  for (int t = 0; t < tiles; ++t) {
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    __syncthreads();  // the tile is in LDS, and every wave is done with the one before it
+    if (t + 1 < tiles) load_tile(t + 1);
+    const uint8_t* tk = lds + (t % kRing) * 2 * kTile;
+    const uint8_t* tv = tk + kTile;
+    const int half0 = kSplit == 1 ? 0 : wave;  // the wave's first half
+    const int left = keys - t * kKeys - 32 * half0;  // keys from there on
+    if (kSplit > 1 && left <= 0) continue;
+
+    f32x16 s[kHalves];
+#pragma unroll
+    for (int i = 0; i < kHalves; ++i) {
+      const int key = 32 * (half0 + i) + col;
+      const uint8_t* row = tk + key * kRowB;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[i][r] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(row + (((2 * d + hq) ^ k_slot<D>(key)) << 4));
+        s[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[d], s[i], 0, 0, 0);
+      }
+    }
+    // register r of half i: key 32 i + 8 (r >> 2) + 4 hq + (r & 3)
+#pragma unroll
+    for (int i = 0; i < kHalves; ++i) {
+      if constexpr (kBias) {
+        const int d0 = t * kKeys + 32 * (half0 + i) - (in_request + qw);  // first key - first query
+        if (d0 - 31 >= sat || d0 + 31 <= -sat) {
+          const float b = d0 > 0 ? far_hi : far_lo;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[i][r] = fmaf(s[i][r], c, b);
+        } else {
+          const float* pb = sbias + (sat + 63 + d0 + 4 * hq - col);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[i][r] = fmaf(s[i][r], c, pb[8 * (r >> 2) + (r & 3)]);
+        }
+      }
+    }
+    if (left < 32 * kHalves) {
+#pragma unroll
+      for (int i = 0; i < kHalves; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * i + 8 * (r >> 2) + 4 * hq + (r & 3) >= left) s[i][r] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 0; i < kHalves; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[i][r]);
+    mx = max_lane_xor32(mx);
+    if constexpr (!kBias) mx *= c;
+    if (__any(mx > m + kSlack)) {
+      const float mn = fmaxf(m, mx);
+      const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      sum *= f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] *= f;
+    }
+    const float off = m == -INFINITY ? 0.0f : m;  // no key above -inf yet: every P is 0
+#pragma unroll
+    for (int i = 0; i < kHalves; ++i) {
+      bf16x8 pf[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float s0 = s[i][8 * u + 2 * j], s1 = s[i][8 * u + 2 * j + 1];
+          const float p0 = __builtin_amdgcn_exp2f(kBias ? s0 - off : fmaf(s0, c, -off));
+          const float p1 = __builtin_amdgcn_exp2f(kBias ? s1 - off : fmaf(s1, c, -off));
+          w[j] = pack_bf16x2(p0, p1);
+          sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w[j]), ones, sum, false);  // the P that multiplies V
+        }
+        pf[u] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        // lane's keys: 16 u + 4 hq .. + 3 and 8 further, of d = 32 i + col; it reads four d of key + (lane & 15) / 4
+        const int key = 32 * (half0 + i) + 16 * u + 4 * hq + ((lane & 15) >> 2);
+        const int ch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        const uint8_t* p0 = tv + key * kRowB + 8 * (lane & 1);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) {
+          const int at = ((4 * dt + ch) ^ v_slot<D>(key)) << 4;  // v_slot(key + 8) is the same
+          typedef __attribute__((address_space(3))) s16x4* lds4;
+          const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p0 + at));
+          const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p0 + 8 * kRowB + at));
+          const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+          acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[u], acc[dt], 0, 0, 0);
+        }
+      }
+    }
+  }
+  sum = add_lane_xor32(sum);
+  __syncthreads();  // LDS is free
+
+  if constexpr (kSplit == 1) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no keys: zeros; NaN stays
+    uint8_t* stage = lds + wave * (32 * kRowB);
+    const int live = min(rows - qw, 32);  // rows of the wave
+    [[maybe_unused]] uint32_t sbytes = 0;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) {
+      uint32_t pp[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pp[i] = pack_bf16x2(acc[dt][2 * i] * inv, acc[dt][2 * i + 1] * inv);
+      if constexpr (kMx) {
+        uint32_t codes[4];
+        sbytes |= (uint32_t)mx_codes(pp, codes) << (8 * dt);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {  // codes 32 dt + 8 g + 4 hq .. + 3
+          const int chunk = 2 * dt + (g >> 1);
+          *reinterpret_cast<uint32_t*>(stage + col * D + ((chunk ^ ((col >> 1) & (D / 16 - 1))) << 4) + 8 * (g & 1) + 4 * hq) = codes[g];
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<uint2*>(stage + col * kRowB + (((4 * dt + g) ^ (col & (kChunks - 1))) << 4) + 8 * hq) = make_uint2(pp[2 * g], pp[2 * g + 1]);
+      }
+    }
+    // (a wave's LDS operations complete in order: no barrier before its own rows are read back)
+    if constexpr (kMx) {
+      uint8_t* po = reinterpret_cast<uint8_t*>(a.out) + (int64_t)(row0 + qw) * a.o_ss + head * D;
+      constexpr int kPerRow = D / 16, kStep = 64 / kPerRow;
+#pragma unroll
+      for (int it = 0; it < 32 / kStep; ++it) {
+        const int r = it * kStep + lane / kPerRow, chunk = lane % kPerRow;
+        const u32x4 x = *reinterpret_cast<const u32x4*>(stage + r * D + ((chunk ^ ((r >> 1) & (D / 16 - 1))) << 4));
+        if (r < live) store_b128_guarded(x, po + (int64_t)r * a.o_ss + chunk * 16);
+      }
+      if (hq == 0 && col < live) {
+        uint8_t* ps = a.out_scales + (int64_t)(row0 + qw + col) * (a.heads * (D / 32)) + head * (D / 32);
+        if constexpr (D == 128) *reinterpret_cast<uint32_t*>(ps) = sbytes;
+        else *reinterpret_cast<uint16_t*>(ps) = (uint16_t)sbytes;
+      }
+    } else {
+      uint16_t* po = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(row0 + qw) * a.o_ss + head * D;
+#pragma unroll
+      for (int it = 0; it < 32 / kPer; ++it) {
+        const int r = it * kPer + lrow;
+        const u32x4 x = *reinterpret_cast<const u32x4*>(stage + r * kRowB + ((lslot ^ (r & (kChunks - 1))) << 4));
+        if (r < live) store_b128_guarded(x, po + (int64_t)r * a.o_ss + lslot * 8);
+      }
+    }
+  } else {
+    // ---- join the waves' parts: [wave][d][row] sums of P V, then [wave][row] maxima and sums ----
+    float* parts = reinterpret_cast<float*>(lds);
+    float* stats = parts + kSplit * 32 * D;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) parts[(wave * D + 32 * dt + 8 * (r >> 2) + 4 * hq + (r & 3)) * 32 + col] = acc[dt][r];
+    if (hq == 0) {
+      stats[wave * 64 + col] = m;
+      stats[wave * 64 + 32 + col] = sum;
+    }
+    __syncthreads();
+    if (wave >= D / 32) return;
+    float mw[kSplit], mm = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kSplit; ++w) mm = fmaxf(mm, mw[w] = stats[w * 64 + col]);
+#pragma unroll
+    for (int w = 0; w < kSplit; ++w) {
+      mw[w] = mw[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw[w] - mm);
+      const float part = stats[w * 64 + 32 + col];
+      total += part == 0.0f ? 0.0f : mw[w] * part;
+    }
+    // a NaN maximum is no maximum, but its sum is NaN
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    float o[16];  // d = 32 wave + 8 g + 4 hq + q of row col
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int d = 32 * wave + 8 * (r >> 2) + 4 * hq + (r & 3);
+      float x = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kSplit; ++w) x = fmaf(mw[w], parts[(w * D + d) * 32 + col], x);
+      o[r] = x * inv;
+    }
+    uint32_t pp[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) pp[i] = pack_bf16x2(o[2 * i], o[2 * i + 1]);
+    const int64_t row = row0 + col;
+    if constexpr (kMx) {
+      uint32_t codes[4];
+      const int sx = mx_codes(pp, codes);
+      if (col < rows) {
+        uint8_t* po = reinterpret_cast<uint8_t*>(a.out) + row * a.o_ss + head * D + 32 * wave + 4 * hq;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) *reinterpret_cast<uint32_t*>(po + 8 * g) = codes[g];
+        if (hq == 0) a.out_scales[row * (a.heads * (D / 32)) + head * (D / 32) + wave] = (uint8_t)sx;
+      }
+    } else if (col < rows) {
+      uint16_t* po = reinterpret_cast<uint16_t*>(a.out) + row * a.o_ss + head * D + 32 * wave + 4 * hq;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) *reinterpret_cast<uint2*>(po + 8 * g) = make_uint2(pp[2 * g], pp[2 * g + 1]);
+    }
+  }
+}
+
+template <int D, bool kBias, int kSplit>
+static int launch(PackedAttnArgs a, const BiasArgs& b, hipStream_t stream, const char* what) {
+  constexpr int kRows = 128 / kSplit;
+  // every request ends in at most one part of a tile, and so do the rows behind the last
+  const int64_t tiles = a.T / kRows + a.requests + 1;
+  const int64_t per = (tiles * a.heads + 7) / 8;
+  WANMI_REQUIRE(tiles * a.heads < (1LL << 30), WANMI_ERR_ARG, "%s: %lld tiles of rows times %d heads are too many", what, (long long)tiles, a.heads);
+  a.tiles = (int)tiles;
+  a.per_xcd = (int)per;
+  if constexpr (!kBias) {
+    if (a.out_scales) {
+      hipLaunchKernelGGL((packed_attention_kernel<D, kBias, kSplit, true>), dim3((unsigned)(8 * per)), dim3(256), 0, stream, a, b);
+      return check_launch(what);
+    }
+  }
+  hipLaunchKernelGGL((packed_attention_kernel<D, kBias, kSplit, false>), dim3((unsigned)(8 * per)), dim3(256), 0, stream, a, b);
+  return check_launch(what);
+}
+
+template <bool kBias>
+static int dispatch(const PackedAttnArgs& a, const BiasArgs& b, int head_dim, hipStream_t stream, const char* what) {
+  // few rows per request: a tile of 32 rows whose keys the waves share out
+  const bool few = a.T <= (int64_t)32 * a.requests;
+  if (head_dim == 64) return few ? launch<64, kBias, 4>(a, b, stream, what) : launch<64, kBias, 1>(a, b, stream, what);
+  return few ? launch<128, kBias, 4>(a, b, stream, what) : launch<128, kBias, 1>(a, b, stream, what);
+}
+
+// What both entry points check: sizes, strides and alignment that the kernel's 16-byte accesses and 32-bit offsets need.
+static int check_args(const PackedAttnArgs& a, int64_t T, int64_t Tk, int64_t requests, int64_t heads, int64_t k_heads, int head_dim, const char* what) {
+  WANMI_REQUIRE(head_dim == 64 || head_dim == 128, WANMI_ERR_UNSUPPORTED, "%s: head_dim %d is not 64 or 128", what, head_dim);
+  WANMI_REQUIRE(T >= 0 && T < (1LL << 28) && Tk >= 0 && Tk < (1LL << 28), WANMI_ERR_ARG, "%s: %lld rows, %lld keys: at most 2^28 - 1", what, (long long)T, (long long)Tk);
+  WANMI_REQUIRE(requests >= 0 && requests < (1 << 20), WANMI_ERR_ARG, "%s: %lld requests: at most 2^20 - 1", what, (long long)requests);
+  WANMI_REQUIRE(heads > 0 && k_heads > 0 && heads % k_heads == 0 && heads <= 1024, WANMI_ERR_ARG, "%s: %lld heads (at most 1024) over %lld key heads", what, (long long)heads, (long long)k_heads);
+  WANMI_REQUIRE(std::isfinite(a.scale_log2) && a.scale_log2 > 0.0f, WANMI_ERR_ARG, "%s: the scale must be positive and finite", what);
+  const int64_t strides[6] = {a.q_ss, a.q_hs, a.k_ss, a.k_hs, a.v_ss, a.v_hs};
+  for (int64_t s : strides)
+    WANMI_REQUIRE(s >= 0 && s % 8 == 0 && s < (1 << 22), WANMI_ERR_ARG, "%s: stride %lld must be a multiple of 8 below 2^22", what, (long long)s);
+  if (T == 0) return WANMI_OK;
+  WANMI_REQUIRE(a.q && a.out && a.q_off && a.k_off && (Tk == 0 || (a.k && a.v)), WANMI_ERR_ARG, "%s: null pointer", what);
+  WANMI_REQUIRE(((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) % 16 == 0, WANMI_ERR_ARG, "%s: q, k, v and out must be 16-byte aligned", what);
+  WANMI_REQUIRE(T == 1 || a.q_ss >= head_dim, WANMI_ERR_ARG, "%s: rows of q overlap", what);
+  WANMI_REQUIRE(Tk <= 1 || (a.k_ss >= head_dim && a.v_ss >= head_dim), WANMI_ERR_ARG, "%s: rows of k or v overlap", what);
+  WANMI_REQUIRE(a.o_ss % 16 == 0 && a.o_ss >= heads * head_dim, WANMI_ERR_ARG, "%s: the output's row stride must be a multiple of 16 of at least %lld", what, (long long)(heads * head_dim));
+  return WANMI_OK;
+}
+
+}  // namespace wanmi
+
+extern "C" int wanmi_packed_cross_attention(const void* q, int64_t q_ss, int64_t q_hs, const void* k, int64_t k_ss, int64_t k_hs,
+                                            const void* v, int64_t v_ss, int64_t v_hs, const int* q_offsets, const int* k_offsets,
+                                            int64_t requests, int64_t T, int64_t Tk, int64_t heads, int64_t k_heads, int head_dim,
+                                            float scale, void* out, int64_t o_ss, uint8_t* out_scales, int zero_rest, void* stream) {
+  using namespace wanmi;
+  clear_error();
+  PackedAttnArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, q_ss, q_hs, k_ss, k_hs, v_ss, v_hs, q_offsets, k_offsets, (int)requests,
+                   (int)T, (int)Tk, (int)heads, (int)(k_heads > 0 ? heads / k_heads : 1), scale * 1.4426950408889634f, out, o_ss, out_scales, zero_rest, 0, 0};
+  const int st = check_args(a, T, Tk, requests, heads, k_heads, head_dim, "wanmi_packed_cross_attention");
+  if (st != WANMI_OK || T == 0) return st;
+  return dispatch<false>(a, BiasArgs{}, head_dim, (hipStream_t)stream, "wanmi_packed_cross_attention");
+}
+
+extern "C" int wanmi_relative_bias_attention(const void* q, int64_t q_ss, int64_t q_hs, const void* k, int64_t k_ss, int64_t k_hs,
+                                             const void* v, int64_t v_ss, int64_t v_hs, const int* offsets, int64_t requests, int64_t T,
+                                             int64_t heads, int head_dim, float scale, const void* table, int table_bf16,
+                                             const int* starts, int side, int both, void* out, int64_t o_ss, int zero_rest, void* stream) {
+  using namespace wanmi;
+  clear_error();
+  const char* what = "wanmi_relative_bias_attention";
+  PackedAttnArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, q_ss, q_hs, k_ss, k_hs, v_ss, v_hs, offsets, offsets, (int)requests,
+                   (int)T, (int)T, (int)heads, 1, scale * 1.4426950408889634f, out, o_ss, nullptr, zero_rest, 0, 0};
+  const int st = check_args(a, T, T, requests, heads, heads, head_dim, what);
+  if (st != WANMI_OK) return st;
+  WANMI_REQUIRE(side >= 1 && side <= kMaxSide && starts, WANMI_ERR_ARG, "%s: %d buckets of one direction, at most %d", what, side, kMaxSide);
+  BiasArgs b{table, table_bf16, side, both, {0}};
+  for (int i = 0; i < side; ++i) {
+    WANMI_REQUIRE(starts[i] >= (i ? starts[i - 1] : 0) && starts[i] <= kMaxSaturation, WANMI_ERR_ARG,
+                  "%s: the buckets' first distances must ascend from 0 to at most %d", what, kMaxSaturation);
+    b.start[i] = starts[i];
+  }
+  if (T == 0) return WANMI_OK;
+  WANMI_REQUIRE(table, WANMI_ERR_ARG, "%s: null pointer", what);
+  return dispatch<true>(a, b, head_dim, (hipStream_t)stream, what);
+}

@@ -1,0 +1,176 @@
+"""Attention over packed rows on gfx950: the text side of a batch of requests.
+
+:func:`packed_cross_attention` lets the rows of every request look at its own text, whatever its length, in one launch.
+:func:`relative_bias_attention` is the self-attention of the text encoder in front of it, over packed prompts, with a learned
+bias by buckets of relative distance. Where a request's rows and keys begin and end is read from GPU tensors of offsets, so
+that a captured HIP graph may be replayed with other lengths. The reference serves one request per forward and
+has no counterpart.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+
+import torch
+
+from . import _lib
+from .common_types import MXTensor
+
+_MAX_SIDE, _MAX_SATURATION = 128, 1024
+
+
+@functools.lru_cache(maxsize=64)
+def _bucket_starts(buckets: int, max_distance: int, bidirectional: bool):
+    """The smallest distance of each bucket of one direction: the first half hold one distance each, the
+    others grow by equal ratios up to ``max_distance``. The borders are ``first * (max_distance / first)^(i / steps)`` rounded up,
+    found in whole numbers: some of them are whole, where a logarithm in floating point may fall on either side."""
+    if buckets < (4 if bidirectional else 2) or (bidirectional and buckets % 2):
+        raise ValueError(f"{buckets} buckets: at least 2 a direction, an even number for both")
+    side = buckets // 2 if bidirectional else buckets
+    first = side // 2
+    if side > _MAX_SIDE or max_distance <= first:
+        raise ValueError(f"{side} buckets of one direction (at most {_MAX_SIDE}) up to distance {max_distance}, which must exceed {first}")
+    steps = side - first
+    starts = list(range(first))
+    n = first
+    for i in range(steps):
+        while n**steps * first**i < max_distance**i * first**steps:
+            n += 1
+        starts.append(n)
+    if starts[-1] > _MAX_SATURATION:
+        raise ValueError(f"the last bucket of {side} up to {max_distance} starts at {starts[-1]}: at most {_MAX_SATURATION}")
+    return (ctypes.c_int * side)(*starts)
+
+
+def _rows(t, what: str, heads: int | None, head_dim: int | None) -> None:
+    _lib.expect(t, what, dtype=torch.bfloat16, shape=(None, heads, head_dim), contiguous=False, row_contiguous=True)
+
+
+def _strides(t) -> tuple:
+    """Row and head strides; those of a dimension of one element, which nothing reads, as a contiguous tensor has them."""
+    T, H, D = t.shape
+    return (t.stride(0) if T > 1 else H * D), (t.stride(1) if H > 1 else D)
+
+
+def _check(q, k, v, scale, out, quant, what: str) -> float:
+    _rows(q, "q", None, None)
+    T, heads, head_dim = q.shape
+    _rows(k, "k", None, head_dim)
+    _rows(v, "v", k.shape[1], head_dim)
+    if v.shape[0] != k.shape[0]:
+        raise ValueError(f"k holds {k.shape[0]} rows, v {v.shape[0]}")
+    if head_dim not in (64, 128):
+        raise NotImplementedError(f"{what}: head_dim {head_dim}: 64 or 128")
+    if heads < 1 or k.shape[1] < 1 or heads % k.shape[1]:
+        raise ValueError(f"{heads} query heads over {k.shape[1]} key heads")
+    scale = head_dim**-0.5 if scale is None else float(scale)
+    if not (0.0 < scale < math.inf):
+        raise ValueError(f"scale {scale} must be positive and finite")
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        ss, hs = _strides(t)
+        if ss % 8 or hs % 8 or t.data_ptr() % 16:
+            raise ValueError(f"{name}'s rows and heads must be 16-byte aligned")
+        if (t.shape[0] > 1 and ss < head_dim) or (t.shape[1] > 1 and hs < head_dim):
+            raise ValueError(f"{name}'s rows or heads overlap")
+    if quant not in ("none", "mx"):
+        raise ValueError(f"unknown quant {quant!r}")
+    if out is not None:
+        if quant != "none":
+            raise ValueError("out takes bf16: quant must be 'none'")
+        _lib.expect(out, "out", dtype=torch.bfloat16, shape=(T, heads, head_dim), contiguous=False, row_contiguous=True)
+        ss, hs = _strides(out)
+        if ss % 16 or (heads > 1 and hs != head_dim) or ss < heads * head_dim or out.data_ptr() % 16:
+            raise ValueError("out must have its heads side by side and 16-byte aligned rows, a multiple of 16 elements apart")
+        # a tile reads its rows of q before it writes them, and nobody else reads them
+        _lib.refuse_overlap(out, "out", q)
+        _lib.refuse_input(out, "out", k, v)
+    return scale
+
+
+def _offsets(t, what: str, n: int | None = None) -> int:
+    _lib.expect(t, what, dtype=torch.int32, shape=(n,))
+    if t.shape[0] < 1:
+        raise ValueError(f"{what} needs one entry more than there are requests")
+    return t.shape[0] - 1
+
+
+def packed_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor,
+                           *, scale: float | None = None, quant: str = "none", out: torch.Tensor | None = None):
+    """Each request's rows of ``q`` over its own rows of ``k`` and ``v``: ``softmax(scale * q k^T) v`` per head, all requests in one launch.
+
+    ``q`` bf16 ``[T, heads, D]``, ``k`` and ``v`` bf16 ``[Tk, k_heads, D]`` with D 64 or 128, ``heads`` a multiple of ``k_heads`` (query
+    head h reads key head ``h // (heads // k_heads)``); rows and heads may be strided (column blocks of a fused
+    projection). ``q_offsets`` and ``k_offsets`` int32 ``[R + 1]`` on the GPU, ascending from 0: request r has the rows
+    ``q_offsets[r]`` to ``q_offsets[r + 1]`` and the keys ``k_offsets[r]`` to ``k_offsets[r + 1]``
+    (:meth:`.PackedRequests.offsets`). ``scale``: ``D ** -0.5`` if None.
+
+    Returns bf16 ``[T, heads, D]``, or with ``quant="mx"`` an :class:`MXTensor` ``[T, heads * D]`` as the MX projections read it.
+    The rows of a request without keys are zeros. Rows behind the last request are zeros too in an output allocated here and
+    left as they are in a given ``out``, which may be ``q``. Offsets are held inside the tensors: wrong ones give wrong
+    rows, and no access out of bounds. The softmax has a running maximum (no bound on scores is needed) and fp32 sums; its weights enter the
+    second product as bf16.
+    """
+    scale = _check(q, k, v, scale, out, quant, "packed_cross_attention")
+    requests = _offsets(q_offsets, "q_offsets")
+    _offsets(k_offsets, "k_offsets", requests + 1)
+    _lib.require_gpu(q, k, v, q_offsets, k_offsets, out, what="packed_cross_attention")
+    T, heads, head_dim = q.shape
+    zero_rest = out is None
+    scales = None
+    if quant == "mx":
+        out = torch.empty((T, heads * head_dim), dtype=torch.float8_e4m3fn, device=q.device)
+        scales = torch.empty((T, heads * head_dim // 32), dtype=torch.uint8, device=q.device)
+        ldo = heads * head_dim
+    else:
+        if out is None:
+            out = torch.empty((T, heads, head_dim), dtype=torch.bfloat16, device=q.device)
+        else:
+            _lib.refuse_input(out, "out", q_offsets, k_offsets)
+        ldo = _strides(out)[0]
+    if T:
+        p = _lib.ptr
+        _lib.call("wanmi_packed_cross_attention", q.get_device(), p(q), *_strides(q), p(k), *_strides(k), p(v), *_strides(v), p(q_offsets),
+                  p(k_offsets), requests, T, k.shape[0], heads, k.shape[1], head_dim, scale, p(out), ldo, p(scales), int(zero_rest))
+    return out if scales is None else MXTensor(out, scales)
+
+
+def relative_bias_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, offsets: torch.Tensor, *,
+                            max_distance: int = 128, bidirectional: bool = True, scale: float = 1.0,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """Self-attention of packed prompts with a learned bias by buckets of relative distance: per head
+    ``softmax(scale * q_i k_j + table[bucket(j - i), h]) v_j`` over the tokens j of row i's own prompt.
+
+    ``q``, ``k``, ``v`` bf16 ``[T, heads, D]``, D 64 or 128 (rows and heads may be strided); ``table`` fp32 or bf16 ``[buckets, heads]``, the
+    weight of the embedding that holds the bias; ``offsets`` int32 ``[R + 1]`` on the GPU, ascending from 0: prompt r is the rows
+    ``offsets[r]`` to ``offsets[r + 1]``. ``scale`` 1: such an encoder's scores are not scaled.
+
+    Half of a direction's buckets hold one distance each, the others grow by equal ratios up to ``max_distance``, and the last
+    holds everything beyond. ``bidirectional``: the first half of the table is for keys at or before the query, the second for those
+    after it. Otherwise every bucket is for the keys before, and all later ones take bucket 0 (they are not masked).
+
+    Returns bf16 ``[T, heads, D]``. Rows behind the last prompt are zeros in an output allocated here and left as they are in a
+    given ``out``, which may be ``q``. Inference only: no gradient.
+    """
+    scale = _check(q, k, v, scale, out, "none", "relative_bias_attention")
+    T, heads, head_dim = q.shape
+    if k.shape[1] != heads or k.shape[0] != T:
+        raise ValueError(f"k and v {list(k.shape)} must have the rows and heads of q {list(q.shape)}")
+    if not isinstance(table, torch.Tensor) or table.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("table must be an fp32 or bf16 tensor [buckets, heads]")
+    _lib.expect(table, "table", dtype=table.dtype, shape=(None, heads))
+    starts = _bucket_starts(table.shape[0], int(max_distance), bool(bidirectional))
+    requests = _offsets(offsets, "offsets")
+    _lib.require_gpu(q, k, v, table, offsets, out, what="relative_bias_attention")
+    zero_rest = out is None
+    if out is None:
+        out = torch.empty((T, heads, head_dim), dtype=torch.bfloat16, device=q.device)
+    else:
+        _lib.refuse_input(out, "out", table, offsets)
+    if T:
+        p = _lib.ptr
+        _lib.call("wanmi_relative_bias_attention", q.get_device(), p(q), *_strides(q), p(k), *_strides(k), p(v), *_strides(v), p(offsets), requests,
+                  T, heads, head_dim, scale, p(table), int(table.dtype is torch.bfloat16), starts, len(starts), int(bool(bidirectional)),
+                  p(out), _strides(out)[0], int(zero_rest))
+    return out

@@ -62,6 +62,10 @@ class PackedRequests(NamedTuple):
             yield at, at + n
             at += n
 
+    def offsets(self) -> torch.Tensor:
+        """int32 ``[requests + 1]``: each request's first row, and the row behind the last one's."""
+        return torch.tensor([0, *(end for _, end in self.spans())], dtype=torch.int32, device=self.request_ids.device)
+
     def grid_positions(self, grids) -> torch.Tensor:
         """int32 ``[rows, 3]``: frame, row and column of every token in its request's latent grid ``(F, H, W)``, raster order
         (zeros for rows of no request)."""

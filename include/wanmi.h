@@ -457,6 +457,30 @@ int wanmi_relative_bias_attention(const void* q, int64_t q_ss, int64_t q_hs, con
                                   int side, int both, void* out, int64_t o_ss, int zero_rest, void* stream);
 
 /*
+ * bf16 rows to e4m3fn codes with one fp32 scale for each 128 of a row: scale = max(amax, 2^-100) / 448, codes = x / scale to the nearest.
+ * x: [M, ldx] (ldx a multiple of 8, K of 16); codes: [M, K]; the scale of block b of row m at m * s_row + b * s_blk. A block with an
+ * infinity or a NaN is NaN throughout. No reference counterpart.
+ */
+int wanmi_fp8_block_quantize(const void* x, int64_t ldx, int64_t M, int64_t K, uint8_t* codes, float* scales, int64_t s_row,
+                             int64_t s_blk, void* stream);
+
+/*
+ * Product with an 8-bit weight that has one fp32 scale per block of 128 x 128:
+ *   out[m, n] = bf16(act(sum_b xs[m, b] ws[n / 128, b] sum_{k in block b} x[m, k] w[n, k] + bias[n]))
+ * x: e4m3fn codes [M, ldx] (ldx a multiple of 16) with x_scales, block b of row m at m * xs_row + b * xs_blk; or, x_scales NULL, bf16 [M, ldx]
+ * (ldx a multiple of 8) that is quantized first as wanmi_fp8_block_quantize does it. w: e4m3fn [N, K]; w_scales: fp32
+ * [ceil(N / 128), ceil(K / 128)]; bias: fp32 [N] or NULL; gelu: the tanh form, or none. out: bf16 [M, ldo] (ldo a multiple of 8). K a multiple
+ * of 16, N of 8; ldx below 2^23. `workspace`: wanmi_fp8_block_workspace bytes of device memory for this call alone.
+ * Stands beside wanmi_mxfp8_gemm (power-of-two scales per 32); no reference counterpart.
+ */
+int wanmi_fp8_block_linear(const void* x, const float* x_scales, int64_t ldx, int64_t xs_row, int64_t xs_blk, const uint8_t* w,
+                           const float* w_scales, const float* bias, int64_t M, int64_t N, int64_t K, int gelu, void* out,
+                           int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that wanmi_fp8_block_linear needs for these sizes (0 for few rows). */
+int64_t wanmi_fp8_block_workspace(int64_t M, int64_t K, int is_bf16);
+
+/*
  * Streaming device-to-device copy of `bytes` (a multiple of 16; src and dst 16-byte aligned, not
  * overlapping) on `stream`: 16-byte loads, eight per thread in flight before its non-temporal
  * stores, one 32 KiB chunk per workgroup. Measurement infrastructure with no counterpart in the

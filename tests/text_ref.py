@@ -60,3 +60,53 @@ def attention_bound(size, out, score_size, terms):
     eps = 2.0**-8
     drift = math.expm1(2 * (terms + 4) * 2.0**-24 * score_size) + 2.0**-15
     return size * (2 * eps + drift) * (1 + eps) + out.abs() * eps + 1e-30
+
+
+def row_blocks(x):
+    """bf16 [M, K] (CPU) -> e4m3 codes and fp32 scales [M, ceil(K / 128)]."""
+    M, K = x.shape
+    y = torch.nn.functional.pad(x.float(), (0, -K % 128)).view(M, -1, 128)
+    scale = y.abs().amax(-1).clamp_min(2.0**-100) / 448.0
+    return (y / scale[..., None]).view(M, -1)[:, :K].contiguous().to(torch.float8_e4m3fn), scale
+
+
+def spread(scales, rows, K):
+    """Block scales at every element: [M, kb] (rows None) or [nb, kb]."""
+    s = scales.double().repeat_interleave(128, 1)[:, :K]
+    return s if rows is None else s.repeat_interleave(128, 0)[:rows]
+
+
+def block_linear(codes, scales, w_codes, w_scales, bias, gelu):
+    """fp64 [M, N], the most an output may be off, and the rms it may be off.
+
+    The product of 128 codes is one matrix instruction. It adds them in groups of eight consecutive ones, in which every product is cut
+    toward zero at 2^-13 of the power of two of the largest, and the sixteen groups in fp32 (seen on MI355X with powers of two: in a
+    group 2^16 + 2^3 is exact, 2^16 + 2^2 is 2^16, whether the 2^16 is cancelled by a third product or not; in two groups both are
+    exact). So a group is off by less than 7 2^-13 of its largest product, which is at most the product of the two largest magnitudes;
+    the sums of the groups, the factor and the sum over kb blocks are 16 + 2 + kb fp32 operations, each off by 2^-23 at most of
+    the sum of magnitudes (cut or rounded). The signs of what is cut are those of the products: uniform in [0, 2^-13) and independent it
+    has the mean square 2^-26 / 3, seven of them in a group."""
+    M, K = codes.shape
+    N = w_codes.shape[0]
+    x = codes.double() * spread(scales, None, K)
+    w = w_codes.double() * spread(w_scales, N, K)
+    y = x @ w.t()
+    xg, wg = x.abs().view(M, K // 8, 8).amax(-1), w.abs().view(N, K // 8, 8).amax(-1)
+    rest = (x.abs() @ w.abs().t()) * (18 + scales.shape[1]) * 2.0**-23
+    off = (xg @ wg.t()) * 7 * 2.0**-13 + rest
+    rms = ((xg.square() @ wg.square().t()) * (7 / 3) * 2.0**-26).sqrt() + rest
+    if bias is not None:
+        y = y + bias.double()
+        off, rms = off + y.abs() * 2.0**-23, rms + y.abs() * 2.0**-23
+    if gelu:  # its slope is at most 1.13; its own fp32 evaluation: exp2's argument, at most 64 here, rounded to 2^-24 of itself
+        y = 0.5 * y * (1 + torch.tanh(math.sqrt(2 / math.pi) * (y + 0.044715 * y.pow(3))))
+        own = y.abs() * 2.0**-17 + 2.0**-40
+        off, rms = 1.13 * off + own, 1.13 * rms + own
+    return y, off * (1 + 2.0**-8) + y.abs() * 2.0**-8 + 1e-38, rms + y.abs() * 2.0**-8 + 1e-38
+
+
+def check_block_linear(got, want, bound, rms):
+    err = (got.double().cpu() - want).abs()
+    bad = err > bound
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist(), float(err.max()))
+    assert float(err.square().mean().sqrt()) <= float(rms.square().mean().sqrt())

@@ -22,6 +22,13 @@ from .row_mx_kernels import (  # noqa: F401
     row_mx_mlp,
     row_quantize_packed,
 )
+from .fp8_block import (  # noqa: F401
+    FP8BlockTensor,
+    FP8BlockWeight,
+    fp8_block_linear,
+    quantize_fp8_blocks,
+    quantize_weight_fp8_blocks,
+)
 from .lora import lora_add, stack_adapters  # noqa: F401
 from . import rope  # noqa: F401
 from .rope import WanRotaryPosEmbed, rope_tables  # noqa: F401

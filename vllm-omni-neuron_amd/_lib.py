@@ -81,6 +81,9 @@ _SIGNATURES = {
                                      _i32, _f32, _vp, _i64, _vp, _i32, _vp],
     "wanmi_relative_bias_attention": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _f32, _vp,
                                       _i32, _vp, _i32, _i32, _vp, _i64, _i32, _vp],
+    "wanmi_fp8_block_quantize": [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp],
+    "wanmi_fp8_block_linear": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp],
+    "wanmi_fp8_block_workspace": [_i64, _i64, _i32],
 }
 
 _LIB = None
@@ -107,6 +110,7 @@ def load() -> ctypes.CDLL:
         fn.restype = _i32
     lib.wanmi_last_error.restype = ctypes.c_char_p
     lib.wanmi_lora_workspace.restype = _i64
+    lib.wanmi_fp8_block_workspace.restype = _i64
     _LIB = lib
     return lib
 

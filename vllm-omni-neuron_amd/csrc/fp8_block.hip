@@ -1,0 +1,427 @@
+// Products with 8-bit weights that have one fp32 scale per block of 128 x 128, for gfx950.
+//
+//   y[m, n] = act( sum_b sa[m, b] sw[n / 128, b] sum_{k in block b} a[m, k] w[n, k] + bias[n] )
+//
+// a and w are e4m3 codes, b the blocks of 128 along k. The scales are any fp32 numbers, not powers of two, so the hardware's block
+// scales cannot apply them: each block's inner product is one 16 x 16 x 128 MFMA from zero, and its result enters the fp32
+// accumulator by a multiply-add with sa * sw (sw is the same for a wave's whole tile, and with the weight as the MFMA's first operand a lane's
+// four results belong to one row m, so a block costs one factor per fragment). A multiply-add per result is half the time
+// that its MFMA takes on the matrix pipe, and runs beside the other wave's MFMAs.
+//
+// Activations come as codes with scales, or as bf16 that is quantized on the way: amax of each 128 of a row (at least 2^-100) / 448
+// is the scale, x / scale rounded to nearest the code.
+#include "wanmi_common.h"
+#include "gemm_plan.h"
+
+#include <algorithm>
+
+namespace wanmi {
+
+constexpr int kBlock = 128;
+
+struct Fp8Args {
+  const uint8_t* a;       // [M, lda] codes
+  int64_t lda;
+  const float* a_scales;  // block b of row m at m * as_row + b * as_blk
+  int64_t as_row, as_blk;
+  const uint16_t* x;      // bf16 [M, lda] in place of codes and scales (few rows)
+  const uint8_t* w;       // [N, K]
+  const float* w_scales;  // [ceil(N / 128), KB]
+  const float* bias;      // [N] or null
+  uint16_t* out;          // bf16 [M, ldo]
+  int64_t ldo;
+  int M, N, K, KB;
+  int gelu;
+  int tiles_m, tiles_n;
+};
+
+// As the MXFP8 GEMM's: gelu_tanh(x) = x / (1 + 2^(x (k0 + k1 x^2))).
+__device__ __forceinline__ float gelu_tanh_f32(float x) {
+  const float e = __builtin_amdgcn_exp2f(x * (-2.302208198144325f + -0.1029432395800235f * (x * x)));
+  return x * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Quantization
+// ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t max_magnitude(uint32_t best, uint32_t pair) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, best), __builtin_bit_cast(u16x2_t, pair & 0x7FFF7FFFu)));
+}
+// The scale of a block from its largest magnitude (bf16 bits; those of infinities and NaN are the largest, and then every code of the block is NaN).
+__device__ __forceinline__ float block_scale(uint32_t best) {
+  const uint32_t top = max(best >> 16, best & 0xFFFFu);
+  const float amax = bf16_to_f32((uint16_t)top);
+  return (amax < 0x1p-100f ? 0x1p-100f : amax) / 448.0f;
+}
+// x / scale rounded as the division rounds it: with y the rounded reciprocal, q + (x - q scale) y rounds correctly for q = x y (Markstein);
+// nothing here underflows that could reach a code (scales are 2^-109 or more).
+__device__ __forceinline__ float quotient(float x, float scale, float y) {
+  const float q = x * y;
+  return fmaf(fmaf(-q, scale, x), y, q);
+}
+__device__ __forceinline__ uint32_t four_codes(uint32_t p01, uint32_t p23, float scale, float y) {
+  return cvt_e4m3x4(quotient(bf16_lo(p01), scale, y), quotient(bf16_hi(p01), scale, y), quotient(bf16_lo(p23), scale, y),
+                    quotient(bf16_hi(p23), scale, y));
+}
+
+// A wave takes four blocks of a row, 16 lanes x 8 values each. K is a multiple of 16: a lane's 8 values are all inside or all behind.
+__global__ __launch_bounds__(256) void fp8_block_quantize_kernel(const uint16_t* __restrict__ x, int64_t ldx, int M, int K, int KB,
+                                                                uint8_t* __restrict__ codes, float* __restrict__ scales,
+                                                                int64_t s_row, int64_t s_blk) {
+  const int lane = threadIdx.x & 63;
+  const int groups = (KB + 3) / 4;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t m = id / groups;
+  if (m >= M) return;
+  const int b = (int)(id - m * groups) * 4 + (lane >> 4);
+  const int k = b * kBlock + 8 * (lane & 15);
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if (k < K) v = *reinterpret_cast<const u32x4*>(x + m * ldx + k);
+  uint32_t best = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) best = max_magnitude(best, v[i]);
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) best = max_magnitude(best, (uint32_t)__shfl_xor((int)best, o, 64));
+  const float scale = block_scale(best), y = 1.0f / scale;
+  if (k < K) *reinterpret_cast<uint2*>(codes + m * K + k) = make_uint2(four_codes(v[0], v[1], scale, y), four_codes(v[2], v[3], scale, y));
+  if (b < KB && (lane & 15) == 0) scales[m * s_row + b * s_blk] = scale;
+}
+
+// scales [M, KB] of any strides -> [KB, M]
+__global__ __launch_bounds__(256) void fp8_scales_kernel(const float* __restrict__ in, int64_t s_row, int64_t s_blk, int M, int KB, float* __restrict__ out) {
+  const int m = blockIdx.x * 64 + (threadIdx.x & 63);
+  if (m >= M) return;
+  for (int b = threadIdx.x >> 6; b < KB; b += 4) out[(int64_t)b * M + m] = in[m * s_row + b * s_blk];
+}
+
+// ------------------------------------------------------------------------------------------------
+// Many rows: tiles of kTn features x kTm rows, both operands through LDS in stages of 128 along k.
+// ------------------------------------------------------------------------------------------------
+// LDS offset of 16-byte chunk c of row r: as the MXFP8 GEMM's, sixteen rows' equal chunks on distinct banks.
+__device__ __forceinline__ int fp8_slot(int row) { return (row & 7) ^ ((row >> 3) & 1); }
+
+template <int kTn, int kTm, int kWn, int kWm>  // the tile and how many waves along each side
+__global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Args g) {
+  constexpr int kWaves = kWn * kWm;
+  constexpr int kFn = kTn / kWn / 16, kFm = kTm / kWm / 16;  // fragments of a wave
+  constexpr int kStage = (kTn + kTm) * kBlock;
+  constexpr int kLoads = (kTn + kTm) / 8 / kWaves;           // per wave and stage
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, q = lane >> 4;
+  const TileAt at = tile_at(blockIdx.x, g.tiles_m, g.tiles_n, kGroupM * TM / kTm);
+  const int m0 = at.tm * kTm, n0 = at.tn * kTn;
+  const int mw = (wave % kWm) * 16 * kFm, nw = (wave / kWm) * 16 * kFn;  // the wave's first row and feature
+
+  const int mv = min(kTm, g.M - m0), nv = min(kTn, g.N - n0);
+  const u32x4 rw = buffer_rsrc(g.w + (int64_t)n0 * g.K, (uint32_t)nv * (uint32_t)g.K);
+  const u32x4 ra = buffer_rsrc(g.a + (int64_t)m0 * g.lda, (uint32_t)((mv - 1) * g.lda + g.K));
+  // rows 8 p + (lane >> 3) of the stage's kTn + kTm rows; slot lane & 7 takes the chunk whose slot that is
+  const int lrow = lane >> 3;
+  const uint32_t ce = (uint32_t)(((lane & 7) ^ lrow) << 4), co = ce ^ 16u;
+  auto load = [&](int kt) {
+    const uint32_t k0 = (uint32_t)kt * kBlock;
+    const uint32_t to = lds_addr(lds) + (uint32_t)(kt & 1) * kStage;
+    const bool ie = k0 + ce < (uint32_t)g.K, io = k0 + co < (uint32_t)g.K;  // chunks behind K read as zeros
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int p = wave * kLoads + i;
+      const bool odd = i & 1;
+      const uint32_t chunk = (odd ? co : ce) + k0;
+      const bool in = odd ? io : ie;
+      if (p < kTn / 8) {
+        const uint32_t off = (uint32_t)(8 * p + lrow) * (uint32_t)g.K + chunk;
+        lds_dma_b128(rw, in ? off : 0xFFFFFFF0u, to + p * 1024);
+      } else {
+        const uint32_t off = (uint32_t)(8 * p - kTn + lrow) * (uint32_t)g.lda + chunk;
+        lds_dma_b128(ra, in ? off : 0xFFFFFFF0u, to + p * 1024);
+      }
+    }
+  };
+  const float* ps = g.a_scales + m0 + mw + c;  // (as_row is 1)
+  int mo[kFm];
+#pragma unroll
+  for (int j = 0; j < kFm; ++j) mo[j] = min(16 * j, g.M - 1 - (m0 + mw + c));  // rows past M: the last one's (maybe before this one)
+  const float* pw = g.w_scales + (int64_t)(min(n0 + nw, g.N - 1) / kBlock) * g.KB;
+  float sa[kFm], sw;
+  auto load_scales = [&](int kt) {
+#pragma unroll
+    for (int j = 0; j < kFm; ++j) sa[j] = ps[(int64_t)kt * g.as_blk + mo[j]];
+    sw = pw[kt];
+  };
+
+  f32x4 acc[kFn][kFm];
+#pragma unroll
+  for (int i = 0; i < kFn; ++i)
+#pragma unroll
+    for (int j = 0; j < kFm; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  load_scales(0);
+  load(0);
+  for (int kt = 0; kt < g.KB; ++kt) {
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    __syncthreads();  // the stage is in LDS, and every wave is done with the one before it
+    float s[kFm];
+#pragma unroll
+    for (int j = 0; j < kFm; ++j) s[j] = sa[j] * sw;
+    if (kt + 1 < g.KB) {
+      load_scales(kt + 1);
+      load(kt + 1);
+    }
+    const uint8_t* tw = lds + (kt & 1) * kStage + (nw + c) * kBlock;
+    const uint8_t* ta = lds + (kt & 1) * kStage + (kTn + mw + c) * kBlock;
+    // lane's bytes of a row: chunks q and 4 + q (in both operands, so the order of k is of no account)
+    const int o0 = (q ^ fp8_slot(c)) << 4, o1 = ((4 + q) ^ fp8_slot(c)) << 4;
+    auto fragment = [&](const uint8_t* p) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(p + o0), y = *reinterpret_cast<const u32x4*>(p + o1);
+      return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+    };
+    i32x8 fa[kFm];
+#pragma unroll
+    for (int j = 0; j < kFm; ++j) fa[j] = fragment(ta + 16 * j * kBlock);
+#pragma unroll
+    for (int i = 0; i < kFn; ++i) {
+      const i32x8 fw = fragment(tw + 16 * i * kBlock);
+#pragma unroll
+      for (int j = 0; j < kFm; ++j) {
+        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        const f32x4 p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, fa[j], zero, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(p[r], s[j], acc[i][j][r]);
+      }
+    }
+  }
+  __syncthreads();  // LDS is free
+
+  // ---- epilogue: lane holds features nw + 16 i + 4 q .. + 3 of row mw + 16 j + c; rows are staged in LDS and stored whole ----
+  constexpr int kRow = 32 * kFn;  // bytes of a wave's row
+  constexpr int kCh = kRow / 16;  // chunks
+  static_assert(kWaves * 16 * kFm * kRow <= 2 * kStage, "staging fits the ring");
+  uint8_t* stage = lds + wave * (16 * kFm * kRow);
+#pragma unroll
+  for (int i = 0; i < kFn; ++i) {
+    f32x4 b = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int n = n0 + nw + 16 * i + 4 * q;
+    if (g.bias && n < g.N) b = *reinterpret_cast<const f32x4*>(g.bias + n);
+#pragma unroll
+    for (int j = 0; j < kFm; ++j) {
+      float y[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        y[r] = acc[i][j][r] + b[r];
+        if (g.gelu) y[r] = gelu_tanh_f32(y[r]);
+      }
+      *reinterpret_cast<uint2*>(stage + (16 * j + c) * kRow + (((2 * i + (q >> 1)) ^ (c & (kCh - 1))) << 4) + 8 * (q & 1)) =
+          make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+    }
+  }
+  constexpr int kPer = 64 / kCh;  // rows of a store
+  const int ch = lane % kCh;
+  const int n = n0 + nw + 8 * ch;
+#pragma unroll
+  for (int it = 0; it < 16 * kFm / kPer; ++it) {
+    const int r = it * kPer + lane / kCh;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(stage + r * kRow + ((ch ^ (r & (kCh - 1))) << 4));
+    const int m = m0 + mw + r;
+    if (m < g.M && n < g.N) store_b128_guarded(v, g.out + (int64_t)m * g.ldo + n);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Few rows: a workgroup of eight waves takes 16 features and all rows, the waves share out the blocks of k. The weight goes straight
+// into registers, all of a wave's loads under way together: what counts is to read it once, at the memory's rate.
+// ------------------------------------------------------------------------------------------------
+constexpr int kFewWaves = 8;
+constexpr int kFewAhead = 4;  // blocks whose weight is under way in a wave
+
+template <int kFm, bool kQuantize>
+__global__ __launch_bounds__(64 * kFewWaves) void fp8_block_few_kernel(Fp8Args g) {
+  __shared__ f32x4 red[kFewWaves][kFm][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = lane & 15, q = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const uint8_t* pw = g.w + (int64_t)min(n0 + c, g.N - 1) * g.K + 32 * q;
+  const float* psw = g.w_scales + (int64_t)(n0 / kBlock) * g.KB;
+  int row[kFm];
+#pragma unroll
+  for (int j = 0; j < kFm; ++j) row[j] = min(16 * j + c, g.M - 1);
+  f32x4 acc[kFm];
+#pragma unroll
+  for (int j = 0; j < kFm; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const u32x4 none = {0u, 0u, 0u, 0u};
+
+  for (int b0 = wave; b0 < g.KB; b0 += kFewWaves * kFewAhead) {
+    u32x4 w[kFewAhead][2];
+#pragma unroll
+    for (int u = 0; u < kFewAhead; ++u) {
+      const int k = (b0 + kFewWaves * u) * kBlock + 32 * q;  // K is a multiple of 16
+      w[u][0] = k < g.K ? *reinterpret_cast<const u32x4*>(pw + (k - 32 * q)) : none;
+      w[u][1] = k + 16 < g.K ? *reinterpret_cast<const u32x4*>(pw + (k - 32 * q) + 16) : none;
+    }
+#pragma unroll
+    for (int u = 0; u < kFewAhead; ++u) {
+      const int b = b0 + kFewWaves * u;
+      if (b >= g.KB) break;
+      const int k = b * kBlock + 32 * q;
+      const i32x8 fw = {(int)w[u][0][0], (int)w[u][0][1], (int)w[u][0][2], (int)w[u][0][3], (int)w[u][1][0], (int)w[u][1][1], (int)w[u][1][2], (int)w[u][1][3]};
+      const float sw = psw[b];
+#pragma unroll
+      for (int j = 0; j < kFm; ++j) {
+        i32x8 fa;
+        float s;
+        if constexpr (kQuantize) {
+          const u32x4* px = reinterpret_cast<const u32x4*>(g.x + row[j] * g.lda + k);
+          u32x4 v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = k + 16 * (i >> 1) < g.K ? px[i] : none;
+          uint32_t best = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) best = max_magnitude(best, v[i][e]);
+          best = max_magnitude(best, (uint32_t)__shfl_xor((int)best, 16, 64));
+          best = max_magnitude(best, (uint32_t)__shfl_xor((int)best, 32, 64));
+          s = block_scale(best);
+          const float y = 1.0f / s;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) fa[i] = (int)four_codes(v[i >> 1][2 * (i & 1)], v[i >> 1][2 * (i & 1) + 1], s, y);
+        } else {
+          const u32x4* pa = reinterpret_cast<const u32x4*>(g.a + row[j] * g.lda + k);
+          const u32x4 lo = k < g.K ? pa[0] : none, hi = k + 16 < g.K ? pa[1] : none;
+          fa = i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+          s = g.a_scales[row[j] * g.as_row + b * g.as_blk];
+        }
+        s *= sw;
+        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        const f32x4 p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, fa, zero, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(p[r], s, acc[j][r]);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kFm; ++j) red[wave][j][lane] = acc[j];
+  __syncthreads();
+  if (wave >= kFm) return;  // wave j adds the parts of fragment j, in the waves' order
+  f32x4 y = red[0][wave][lane];
+#pragma unroll
+  for (int w = 1; w < kFewWaves; ++w) y += red[w][wave][lane];
+  const int m = 16 * wave + c, n = n0 + 4 * q;
+  if (m >= g.M || n >= g.N) return;
+  if (g.bias) y += *reinterpret_cast<const f32x4*>(g.bias + n);
+  if (g.gelu) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = gelu_tanh_f32(y[r]);
+  }
+  *reinterpret_cast<uint2*>(g.out + (int64_t)m * g.ldo + n) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+}
+
+constexpr int kFewRows = 64;      // at most: beyond, tiles
+constexpr int kFewQuantize = 16;  // at most, quantizing in every workgroup: beyond, once before
+
+static void launch_quantize(const uint16_t* x, int64_t ldx, int M, int K, uint8_t* codes, float* scales, int64_t s_row, int64_t s_blk, hipStream_t st) {
+  const int KB = (K + kBlock - 1) / kBlock;
+  const int64_t waves = (int64_t)M * ((KB + 3) / 4);
+  hipLaunchKernelGGL(fp8_block_quantize_kernel, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, x, ldx, M, K, KB, codes, scales, s_row, s_blk);
+}
+
+template <int kTn, int kTm, int kWn, int kWm>
+static void launch_tiles(Fp8Args g, hipStream_t st) {
+  g.tiles_m = (g.M + kTm - 1) / kTm;
+  g.tiles_n = (g.N + kTn - 1) / kTn;
+  hipLaunchKernelGGL((fp8_block_gemm_kernel<kTn, kTm, kWn, kWm>), dim3((unsigned)(g.tiles_m * g.tiles_n)), dim3(64 * kWn * kWm), 0, st, g);
+}
+
+template <int kFm>
+static void launch_few(const Fp8Args& g, hipStream_t st) {
+  const dim3 grid((unsigned)((g.N + 15) / 16)), block(64 * kFewWaves);
+  if constexpr (16 * kFm <= kFewQuantize) {
+    if (g.x) {
+      hipLaunchKernelGGL((fp8_block_few_kernel<kFm, true>), grid, block, 0, st, g);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((fp8_block_few_kernel<kFm, false>), grid, block, 0, st, g);
+}
+
+static int64_t blocks_of(int64_t K) { return (K + kBlock - 1) / kBlock; }
+
+static int check_sizes(int64_t M, int64_t K, const char* what) {
+  WANMI_REQUIRE(M >= 0 && M < (1LL << 27), WANMI_ERR_ARG, "%s: %lld rows: at most 2^27 - 1", what, (long long)M);
+  WANMI_REQUIRE(K >= 16 && K % 16 == 0 && K < (1 << 22), WANMI_ERR_ARG, "%s: K=%lld must be a multiple of 16 below 2^22", what, (long long)K);
+  return WANMI_OK;
+}
+
+}  // namespace wanmi
+
+extern "C" int wanmi_fp8_block_quantize(const void* x, int64_t ldx, int64_t M, int64_t K, uint8_t* codes, float* scales, int64_t s_row,
+                                        int64_t s_blk, void* stream) {
+  using namespace wanmi;
+  clear_error();
+  const char* what = "wanmi_fp8_block_quantize";
+  const int bad = check_sizes(M, K, what);
+  if (bad != WANMI_OK || M == 0) return bad;
+  WANMI_REQUIRE(x && codes && scales, WANMI_ERR_ARG, "%s: null pointer", what);
+  WANMI_REQUIRE((M == 1 || ldx >= K) && ldx % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)codes % 16 == 0, WANMI_ERR_ARG,
+                "%s: rows of x (%lld apart) and the codes must be 16-byte aligned", what, (long long)ldx);
+  WANMI_REQUIRE(M * ((blocks_of(K) + 3) / 4) < (1LL << 32), WANMI_ERR_ARG, "%s: %lld x %lld is too large", what, (long long)M, (long long)K);
+  launch_quantize((const uint16_t*)x, ldx, (int)M, (int)K, codes, scales, s_row, s_blk, (hipStream_t)stream);
+  return check_launch(what);
+}
+
+extern "C" int64_t wanmi_fp8_block_workspace(int64_t M, int64_t K, int is_bf16) {
+  using namespace wanmi;
+  if (M <= 0 || K <= 0 || M <= (is_bf16 ? kFewQuantize : kFewRows)) return 0;
+  const int64_t codes = is_bf16 ? (M * K + 255) / 256 * 256 : 0;
+  return codes + M * blocks_of(K) * 4;
+}
+
+extern "C" int wanmi_fp8_block_linear(const void* x, const float* x_scales, int64_t ldx, int64_t xs_row, int64_t xs_blk, const uint8_t* w,
+                                      const float* w_scales, const float* bias, int64_t M, int64_t N, int64_t K, int gelu, void* out,
+                                      int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace wanmi;
+  clear_error();
+  const char* what = "wanmi_fp8_block_linear";
+  const int bad = check_sizes(M, K, what);
+  if (bad != WANMI_OK) return bad;
+  WANMI_REQUIRE(N >= 8 && N % 8 == 0 && N < (1 << 24), WANMI_ERR_ARG, "%s: N=%lld must be a multiple of 8 below 2^24", what, (long long)N);
+  if (M == 0) return WANMI_OK;
+  const bool is_bf16 = x_scales == nullptr;
+  const int64_t KB = blocks_of(K), align = is_bf16 ? 8 : 16;
+  WANMI_REQUIRE(x && w && w_scales && out, WANMI_ERR_ARG, "%s: null pointer", what);
+  WANMI_REQUIRE(((uintptr_t)x | (uintptr_t)w | (uintptr_t)out | (uintptr_t)bias) % 16 == 0, WANMI_ERR_ARG, "%s: x, w, bias and out must be 16-byte aligned", what);
+  WANMI_REQUIRE(ldx % align == 0 && (M == 1 || ldx >= K) && ldx < (1 << 23), WANMI_ERR_ARG, "%s: rows of x, %lld apart, must be 16-byte aligned", what, (long long)ldx);
+  WANMI_REQUIRE(ldo % 8 == 0 && ldo >= N, WANMI_ERR_ARG, "%s: the output's row stride %lld must be a multiple of 8 of at least N", what, (long long)ldo);
+  const int64_t need = wanmi_fp8_block_workspace(M, K, is_bf16);
+  WANMI_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 16 == 0)), WANMI_ERR_ARG,
+                "%s: the workspace holds %lld bytes of %lld", what, (long long)workspace_bytes, (long long)need);
+  WANMI_REQUIRE(((M + 63) / 64) * ((N + 63) / 64) < (1LL << 30) && M * ((KB + 3) / 4) < (1LL << 32), WANMI_ERR_ARG, "%s: too many tiles", what);
+  hipStream_t st = (hipStream_t)stream;
+  Fp8Args g{(const uint8_t*)x, ldx, x_scales, xs_row, xs_blk, nullptr, w, w_scales, bias, (uint16_t*)out, ldo, (int)M, (int)N, (int)K, (int)KB, gelu, 0, 0};
+  if (is_bf16 && M <= kFewQuantize) {
+    g.x = (const uint16_t*)x;
+  } else if (is_bf16) {
+    uint8_t* codes = (uint8_t*)workspace;
+    float* scales = (float*)(codes + (M * K + 255) / 256 * 256);
+    launch_quantize((const uint16_t*)x, ldx, (int)M, (int)K, codes, scales, 1, M, st);
+    g.a = codes, g.lda = K, g.a_scales = scales, g.as_row = 1, g.as_blk = M;
+  } else if (M > kFewRows && xs_row != 1) {
+    float* scales = (float*)workspace;
+    hipLaunchKernelGGL(fp8_scales_kernel, dim3((unsigned)((M + 63) / 64)), dim3(256), 0, st, x_scales, xs_row, xs_blk, (int)M, (int)KB, scales);
+    g.a_scales = scales, g.as_row = 1, g.as_blk = M;
+  }
+  if (M <= 16) {
+    launch_few<1>(g, st);
+  } else if (M <= 32) {
+    launch_few<2>(g, st);
+  } else if (M <= kFewRows) {
+    launch_few<4>(g, st);
+  } else {
+    const int cus = device_cu_count();
+    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256), mid = ((M + 127) / 128) * ((N + 127) / 128);
+    if (big >= cus) launch_tiles<256, 256, 2, 4>(g, st);
+    else if (mid >= cus) launch_tiles<128, 128, 2, 2>(g, st);
+    else launch_tiles<64, 64, 2, 2>(g, st);
+  }
+  return check_launch(what);
+}

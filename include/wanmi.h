@@ -457,7 +457,7 @@ int wanmi_relative_bias_attention(const void* q, int64_t q_ss, int64_t q_hs, con
                                   int side, int both, void* out, int64_t o_ss, int zero_rest, void* stream);
 
 /*
- * bf16 rows to e4m3fn codes with one fp32 scale for each 128 of a row: scale = max(amax, 2^-100) / 448, codes = x / scale to the nearest.
+ * bf16 rows to e4m3fn codes with one fp32 scale for each 128 of a row: scale = max(amax, 2^-100) * fp32(1 / 448), codes = x / scale to the nearest.
  * x: [M, ldx] (ldx a multiple of 8, K of 16); codes: [M, K]; the scale of block b of row m at m * s_row + b * s_blk. A block with an
  * infinity or a NaN is NaN throughout. No reference counterpart.
  */

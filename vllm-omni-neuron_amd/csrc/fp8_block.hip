@@ -8,8 +8,9 @@
 // four results belong to one row m, so a block costs one factor per fragment). A multiply-add per result is half the time
 // that its MFMA takes on the matrix pipe, and runs beside the other wave's MFMAs.
 //
-// Activations come as codes with scales, or as bf16 that is quantized on the way: amax of each 128 of a row (at least 2^-100) / 448
-// is the scale, x / scale rounded to nearest the code.
+// Activations come as codes with scales, or as bf16 that is quantized on the way: amax of each 128 of a row (at least 2^-100) times
+// fp32(1 / 448) is the scale, x / scale rounded to nearest the code. (bf16 values over their maximum fall onto the border between two codes often enough
+// that the last bit of the scale decides many codes: the product with the rounded reciprocal is what torch computes on the GPU for `/ 448`.)
 #include "wanmi_common.h"
 #include "gemm_plan.h"
 
@@ -51,7 +52,7 @@ __device__ __forceinline__ uint32_t max_magnitude(uint32_t best, uint32_t pair) 
 __device__ __forceinline__ float block_scale(uint32_t best) {
   const uint32_t top = max(best >> 16, best & 0xFFFFu);
   const float amax = bf16_to_f32((uint16_t)top);
-  return (amax < 0x1p-100f ? 0x1p-100f : amax) / 448.0f;
+  return (amax < 0x1p-100f ? 0x1p-100f : amax) * (1.0f / 448.0f);
 }
 // x / scale rounded as the division rounds it: with y the rounded reciprocal, q + (x - q scale) y rounds correctly for q = x y (Markstein);
 // nothing here underflows that could reach a code (scales are 2^-109 or more).

@@ -63,12 +63,12 @@ def _blocks(n: int) -> int:
 
 def quantize_weight_fp8_blocks(weight_kn: torch.Tensor, bias: torch.Tensor | None = None) -> FP8BlockWeight:
     """Reference-layout weight ``[K, N]`` (``x @ W``) -> :class:`FP8BlockWeight`, once at load time. A block's scale is its largest
-    magnitude (at least 2^-100) / 448."""
+    magnitude (at least 2^-100) times fp32(1 / 448)."""
     if weight_kn.dim() != 2:
         raise ValueError("weight must be [K, N]")
     K, N = weight_kn.shape
     w = torch.nn.functional.pad(weight_kn.t().to(torch.float32), (0, -K % BLOCK, 0, -N % BLOCK)).view(_blocks(N), BLOCK, _blocks(K), BLOCK)
-    scales = w.abs().amax((1, 3)).clamp_min(2.0**-100) / 448.0
+    scales = w.abs().amax((1, 3)).clamp_min(2.0**-100) * (1.0 / 448.0)
     codes = (w / scales[:, None, :, None]).view(_blocks(N) * BLOCK, -1)[:N, :K].contiguous().to(torch.float8_e4m3fn)
     return FP8BlockWeight(codes, scales, None if bias is None else bias.reshape(-1).to(torch.float32).contiguous())
 
@@ -88,7 +88,7 @@ def _check_rows(x: torch.Tensor, what: str) -> tuple:
 
 def quantize_fp8_blocks(x: torch.Tensor) -> FP8BlockTensor:
     """bf16 ``[..., K]`` (K a multiple of 16) -> :class:`FP8BlockTensor`: a block's scale is its largest magnitude (at least
-    2^-100) / 448 in fp32, the codes are ``x / scale`` to the nearest. A block that holds an infinity or a NaN is NaN throughout."""
+    2^-100) times fp32(1 / 448), the codes are ``x / scale`` to the nearest. A block that holds an infinity or a NaN is NaN throughout."""
     if not isinstance(x, torch.Tensor) or x.dtype != torch.bfloat16:
         raise ValueError("x must be a bf16 tensor [..., K]")
     lead = x.shape[:-1]

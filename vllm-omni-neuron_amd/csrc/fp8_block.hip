@@ -107,6 +107,8 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
   constexpr int kFn = kTn / kWn / 16, kFm = kTm / kWm / 16;  // fragments of a wave
   constexpr int kStage = (kTn + kTm) * kBlock;
   constexpr int kLoads = (kTn + kTm) / 8 / kWaves;           // per wave and stage
+  constexpr int kLoadsLast = kFn == 8 ? 2 : kFn == 4 ? 4 : kLoads;  // of them in a stage's last row, and as many in each of the next rows
+  static_assert(kFn % 2 == 0 && kLoads % kLoadsLast == 0 && kLoads / kLoadsLast < kFn, "fragments alternate; loads end before the wait for them");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, q = lane >> 4;
@@ -120,24 +122,17 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
   // rows 8 p + (lane >> 3) of the stage's kTn + kTm rows; slot lane & 7 takes the chunk whose slot that is
   const int lrow = lane >> 3;
   const uint32_t ce = (uint32_t)(((lane & 7) ^ lrow) << 4), co = ce ^ 16u;
-  auto load = [&](int kt) {
-    const uint32_t k0 = (uint32_t)kt * kBlock;
+  // load i of a wave, of stage kt (behind the last stage: nothing moves)
+  auto load = [&](int kt, int i) {
+    const bool some = kt < g.KB;
     const uint32_t to = lds_addr(lds) + (uint32_t)(kt & 1) * kStage;
-    const bool ie = k0 + ce < (uint32_t)g.K, io = k0 + co < (uint32_t)g.K;  // chunks behind K read as zeros
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int p = wave * kLoads + i;
-      const bool odd = i & 1;
-      const uint32_t chunk = (odd ? co : ce) + k0;
-      const bool in = odd ? io : ie;
-      if (p < kTn / 8) {
-        const uint32_t off = (uint32_t)(8 * p + lrow) * (uint32_t)g.K + chunk;
-        lds_dma_b128(rw, in ? off : 0xFFFFFFF0u, to + p * 1024);
-      } else {
-        const uint32_t off = (uint32_t)(8 * p - kTn + lrow) * (uint32_t)g.lda + chunk;
-        lds_dma_b128(ra, in ? off : 0xFFFFFFF0u, to + p * 1024);
-      }
-    }
+    const int p = wave * kLoads + i;
+    const uint32_t chunk = ((i & 1) ? co : ce) + (uint32_t)kt * kBlock;
+    const bool weight = p < kTn / 8;
+    u32x4 r = weight ? rw : ra;
+    r[2] = some ? r[2] : 0u;
+    const uint32_t off = (weight ? (uint32_t)(8 * p + lrow) * (uint32_t)g.K : (uint32_t)(8 * p - kTn + lrow) * (uint32_t)g.lda) + chunk;
+    lds_dma_b128(r, chunk < (uint32_t)g.K ? off : 0xFFFFFFF0u, to + p * 1024);  // chunks behind K read as zeros
   };
   const float* ps = g.a_scales + m0 + mw + c;  // (as_row is 1)
   int mo[kFm];
@@ -146,52 +141,99 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
   const float* pw = g.w_scales + (int64_t)(min(n0 + nw, g.N - 1) / kBlock) * g.KB;
   float sa[kFm], sw;
   auto load_scales = [&](int kt) {
+    kt = min(kt, g.KB - 1);
 #pragma unroll
     for (int j = 0; j < kFm; ++j) sa[j] = ps[(int64_t)kt * g.as_blk + mo[j]];
     sw = pw[kt];
   };
+  // lane's bytes of a row: chunks q and 4 + q (in both operands, so the order of k is of no account)
+  const int o0 = (q ^ fp8_slot(c)) << 4, o1 = ((4 + q) ^ fp8_slot(c)) << 4;
+  auto fragment = [&](int kt, int row) {
+    const uint8_t* p = lds + (kt & 1) * kStage + (row + c) * kBlock;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(p + o0), y = *reinterpret_cast<const u32x4*>(p + o1);
+    return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+  };
 
-  f32x4 acc[kFn][kFm];
+  f32x4 acc[kFn][kFm], p[kFm];
+  float s[kFm];
+  i32x8 fa[kFm], fw[2];
 #pragma unroll
-  for (int i = 0; i < kFn; ++i)
+  for (int j = 0; j < kFm; ++j) {
+    p[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    s[j] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kFm; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < kFn; ++i) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
 
+  // A stage is kFn rows of kFm MFMAs (one weight fragment each). Beside an MFMA run the multiply-adds of the same column's MFMA one row
+  // before, the reads of the next row's weight fragment and the loads of the stages ahead, in this order (the scheduling barriers keep it: left
+  // to itself the compiler put every multiply-add right behind its MFMA and waited). Before the last row every wave has read all of its stage
+  // and the next one is in LDS: the one barrier of a stage. The last row then reads the next stage's first fragments, and the stage
+  // after next is loaded into the buffer from there on.
   load_scales(0);
-  load(0);
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) load(0, i);
+#pragma unroll
+  for (int i = 0; i < kLoadsLast; ++i) load(1, i);
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(kLoadsLast));
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kFm; ++j) fa[j] = fragment(0, kTn + mw + 16 * j);
+  fw[0] = fragment(0, nw);
+  float sn[kFm];  // of the stage
+#pragma unroll
+  for (int j = 0; j < kFm; ++j) sn[j] = sa[j] * sw;
+  load_scales(1);
+
   for (int kt = 0; kt < g.KB; ++kt) {
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-    __syncthreads();  // the stage is in LDS, and every wave is done with the one before it
-    float s[kFm];
-#pragma unroll
-    for (int j = 0; j < kFm; ++j) s[j] = sa[j] * sw;
-    if (kt + 1 < g.KB) {
-      load_scales(kt + 1);
-      load(kt + 1);
-    }
-    const uint8_t* tw = lds + (kt & 1) * kStage + (nw + c) * kBlock;
-    const uint8_t* ta = lds + (kt & 1) * kStage + (kTn + mw + c) * kBlock;
-    // lane's bytes of a row: chunks q and 4 + q (in both operands, so the order of k is of no account)
-    const int o0 = (q ^ fp8_slot(c)) << 4, o1 = ((4 + q) ^ fp8_slot(c)) << 4;
-    auto fragment = [&](const uint8_t* p) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(p + o0), y = *reinterpret_cast<const u32x4*>(p + o1);
-      return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
-    };
-    i32x8 fa[kFm];
-#pragma unroll
-    for (int j = 0; j < kFm; ++j) fa[j] = fragment(ta + 16 * j * kBlock);
 #pragma unroll
     for (int i = 0; i < kFn; ++i) {
-      const i32x8 fw = fragment(tw + 16 * i * kBlock);
+      const bool last = i == kFn - 1;
+      if (last) {
+        __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0));
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+        __syncthreads();
+      }
+      if (last) fw[(i + 1) & 1] = fragment(kt + 1, nw);
+      else fw[(i + 1) & 1] = fragment(kt, nw + 16 * (i + 1));
+      float f[kFm];  // the factors of the row before
+#pragma unroll
+      for (int j = 0; j < kFm; ++j) f[j] = s[j];
+      if (i == 0) {
+#pragma unroll
+        for (int j = 0; j < kFm; ++j) s[j] = sn[j];
+      }
+      if (last) {
+#pragma unroll
+        for (int j = 0; j < kFm; ++j) sn[j] = sa[j] * sw;
+        load_scales(kt + 2);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < kFm; ++j) {
-        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-        const f32x4 p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, fa[j], zero, 0, 0, 0, 0, 0, 0);
+        const int prev = i == 0 ? kFn - 1 : i - 1;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(p[r], s[j], acc[i][j][r]);
+        for (int r = 0; r < 4; ++r) acc[prev][j][r] = fmaf(p[j][r], f[j], acc[prev][j][r]);
+        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        p[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[i & 1], fa[j], zero, 0, 0, 0, 0, 0, 0);
+        if (last) fa[j] = fragment(kt + 1, kTn + mw + 16 * j);
+        if (last) {
+#pragma unroll
+          for (int l = j * kLoadsLast / kFm; l < (j + 1) * kLoadsLast / kFm; ++l) load(kt + 2, l);
+        } else {
+#pragma unroll
+          for (int l = j * kLoadsLast / kFm; l < (j + 1) * kLoadsLast / kFm; ++l)
+            if (kLoadsLast * (i + 1) + l < kLoads) load(kt + 1, kLoadsLast * (i + 1) + l);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
+#pragma unroll
+  for (int j = 0; j < kFm; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[kFn - 1][j][r] = fmaf(p[j][r], s[j], acc[kFn - 1][j][r]);
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // (loads of stages behind the last move nothing, and are waited for)
   __syncthreads();  // LDS is free
 
   // ---- epilogue: lane holds features nw + 16 i + 4 q .. + 3 of row mw + 16 j + c; rows are staged in LDS and stored whole ----

@@ -98,8 +98,10 @@ __global__ __launch_bounds__(256) void fp8_scales_kernel(const float* __restrict
 // ------------------------------------------------------------------------------------------------
 // Many rows: tiles of kTn features x kTm rows, both operands through LDS in stages of 128 along k.
 // ------------------------------------------------------------------------------------------------
-// LDS offset of 16-byte chunk c of row r: as the MXFP8 GEMM's, sixteen rows' equal chunks on distinct banks.
-__device__ __forceinline__ int fp8_slot(int row) { return (row & 7) ^ ((row >> 3) & 1); }
+// 16-byte chunk c of row r lies in slot c ^ f(r) of its 128 bytes. One cycle of a 16-byte read serves lanes 0-3, 12-15 and 20-27 (or the others
+// of 32): all sixteen rows of a fragment, chunk q of rows 0-3 and 12-15 and chunk q ^ 1 of rows 4-11. Two rows share the 64 banks, so
+// the eight even and the eight odd rows each need eight slots: f(r) ^ (r in 4..11) has to be one to one on them.
+__device__ __forceinline__ int fp8_slot(int row) { return (row & 7) ^ ((row >> 2) & 1); }
 
 template <int kTn, int kTm, int kWn, int kWm>  // the tile and how many waves along each side
 __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Args g) {
@@ -121,13 +123,13 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
   const u32x4 ra = buffer_rsrc(g.a + (int64_t)m0 * g.lda, (uint32_t)((mv - 1) * g.lda + g.K));
   // rows 8 p + (lane >> 3) of the stage's kTn + kTm rows; slot lane & 7 takes the chunk whose slot that is
   const int lrow = lane >> 3;
-  const uint32_t ce = (uint32_t)(((lane & 7) ^ lrow) << 4), co = ce ^ 16u;
+  const uint32_t lchunk = (uint32_t)(((lane & 7) ^ fp8_slot(lrow)) << 4);
   // load i of a wave, of stage kt (behind the last stage: nothing moves)
   auto load = [&](int kt, int i) {
     const bool some = kt < g.KB;
     const uint32_t to = lds_addr(lds) + (uint32_t)(kt & 1) * kStage;
     const int p = wave * kLoads + i;
-    const uint32_t chunk = ((i & 1) ? co : ce) + (uint32_t)kt * kBlock;
+    const uint32_t chunk = lchunk + (uint32_t)kt * kBlock;
     const bool weight = p < kTn / 8;
     u32x4 r = weight ? rw : ra;
     r[2] = some ? r[2] : 0u;

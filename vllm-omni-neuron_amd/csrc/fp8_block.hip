@@ -103,173 +103,229 @@ __global__ __launch_bounds__(256) void fp8_scales_kernel(const float* __restrict
 // the eight even and the eight odd rows each need eight slots: f(r) ^ (r in 4..11) has to be one to one on them.
 __device__ __forceinline__ int fp8_slot(int row) { return (row & 7) ^ ((row >> 2) & 1); }
 
+// What one tile's loads need: the wave's operand (the first half of the waves loads the weight, the second the rows), the scales.
+struct Fp8Tile {
+  uint64_t src, scales, wscales;
+  uint32_t src_bytes, scales_bytes, wscales_bytes;  // 0: no tile, nothing moves
+  int m0, n0;
+};
+
+// 64 bits of address, 32 of extent, all the same in every lane
+__device__ __forceinline__ u32x4 uniform_rsrc(uint64_t base, uint32_t bytes) {
+  return u32x4{(uint32_t)base, (uint32_t)(base >> 32) & 0xFFFFu, bytes, 0x00020000u};
+}
+// (the same in every lane, but where the compiler does not prove it it keeps it in vector registers)
+__device__ __forceinline__ u32x4 first_lane_rsrc(const void* p, uint32_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)) & 0xFFFFu,
+               (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
+}
+__device__ __forceinline__ float uniform_load(uint64_t base, uint32_t bytes, int off) {
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
+  return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+}
+
 template <int kTn, int kTm, int kWn, int kWm>  // the tile and how many waves along each side
 __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Args g) {
+  static_assert(kTn == kTm, "half of the waves loads either operand");
   constexpr int kWaves = kWn * kWm;
   constexpr int kFn = kTn / kWn / 16, kFm = kTm / kWm / 16;  // fragments of a wave
   constexpr int kStage = (kTn + kTm) * kBlock;
   constexpr int kLoads = (kTn + kTm) / 8 / kWaves;           // per wave and stage
   constexpr int kLoadsLast = kFn == 8 ? 2 : kFn == 4 ? 4 : kLoads;  // of them in a stage's last row, and as many in each of the next rows
   static_assert(kFn % 2 == 0 && kLoads % kLoadsLast == 0 && kLoads / kLoadsLast < kFn, "fragments alternate; loads end before the wait for them");
+  constexpr int kRow = 32 * kFn;         // bytes of a wave's output row
+  constexpr int kStaging = 16 * kRow;    // sixteen rows
+  static_assert(kStaging >= 1024, "a load of the bias fits");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
+  __shared__ __attribute__((aligned(1024))) uint8_t staging[kWaves * kStaging];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, q = lane >> 4;
-  const TileAt at = tile_at(blockIdx.x, g.tiles_m, g.tiles_n, kGroupM * TM / kTm);
-  const int m0 = at.tm * kTm, n0 = at.tn * kTn;
   const int mw = (wave % kWm) * 16 * kFm, nw = (wave / kWm) * 16 * kFn;  // the wave's first row and feature
+  const bool weight = wave < kWaves / 2;
+  const uint32_t ld = weight ? (uint32_t)g.K : (uint32_t)g.lda;
+  const uint32_t row0 = (uint32_t)(wave % (kWaves / 2)) * (8 * kLoads);  // of the rows it loads
+  const int total = g.tiles_m * g.tiles_n;
+  const int stages = max(g.KB, 2);  // (the second of one block's two reads zeros)
 
-  const int mv = min(kTm, g.M - m0), nv = min(kTn, g.N - n0);
-  const u32x4 rw = buffer_rsrc(g.w + (int64_t)n0 * g.K, (uint32_t)nv * (uint32_t)g.K);
-  const u32x4 ra = buffer_rsrc(g.a + (int64_t)m0 * g.lda, (uint32_t)((mv - 1) * g.lda + g.K));
-  // rows 8 p + (lane >> 3) of the stage's kTn + kTm rows; slot lane & 7 takes the chunk whose slot that is
-  const int lrow = lane >> 3;
-  const uint32_t lchunk = (uint32_t)(((lane & 7) ^ fp8_slot(lrow)) << 4);
-  // load i of a wave, of stage kt (behind the last stage: nothing moves)
-  auto load = [&](int kt, int i) {
-    const bool some = kt < g.KB;
-    const uint32_t to = lds_addr(lds) + (uint32_t)(kt & 1) * kStage;
-    const int p = wave * kLoads + i;
-    const uint32_t chunk = lchunk + (uint32_t)kt * kBlock;
-    const bool weight = p < kTn / 8;
-    u32x4 r = weight ? rw : ra;
-    r[2] = some ? r[2] : 0u;
-    const uint32_t off = (weight ? (uint32_t)(8 * p + lrow) * (uint32_t)g.K : (uint32_t)(8 * p - kTn + lrow) * (uint32_t)g.lda) + chunk;
-    lds_dma_b128(r, chunk < (uint32_t)g.K ? off : 0xFFFFFFF0u, to + p * 1024);  // chunks behind K read as zeros
+  auto tile_of = [&](int v) {
+    Fp8Tile t;
+    const TileAt at = tile_at(min(v, total - 1), g.tiles_m, g.tiles_n, kGroupM * TM / kTm);
+    t.m0 = at.tm * kTm;
+    t.n0 = at.tn * kTn;
+    const int mv = min(kTm, g.M - t.m0), nv = min(kTn, g.N - t.n0);
+    const bool some = v < total;
+    t.src = weight ? reinterpret_cast<uint64_t>(g.w) + (uint64_t)t.n0 * (uint64_t)g.K : reinterpret_cast<uint64_t>(g.a) + (uint64_t)t.m0 * (uint64_t)g.lda;
+    t.src_bytes = some ? (uint32_t)((weight ? nv : mv) - 1) * ld + (uint32_t)g.K : 0u;
+    t.scales = reinterpret_cast<uint64_t>(g.a_scales + t.m0);  // (as_row is 1)
+    t.scales_bytes = some ? (uint32_t)mv * 4 : 0u;
+    t.wscales = reinterpret_cast<uint64_t>(g.w_scales + (int64_t)(min(t.n0 + nw, g.N - 1) / kBlock) * g.KB);
+    t.wscales_bytes = some ? (uint32_t)g.KB * 4 : 0u;
+    return t;
   };
-  const float* ps = g.a_scales + m0 + mw + c;  // (as_row is 1)
-  int mo[kFm];
-#pragma unroll
-  for (int j = 0; j < kFm; ++j) mo[j] = min(16 * j, g.M - 1 - (m0 + mw + c));  // rows past M: the last one's (maybe before this one)
-  const float* pw = g.w_scales + (int64_t)(min(n0 + nw, g.N - 1) / kBlock) * g.KB;
+
+  // rows 8 i + (lane >> 3) from row0 on; slot lane & 7 takes the chunk whose slot that is; chunks behind K read as zeros
+  const uint32_t lchunk = (uint32_t)(((lane & 7) ^ fp8_slot(lane >> 3)) << 4);
+  const uint32_t lvoff = (uint32_t)(lane >> 3) * ld + lchunk;
+  uint64_t load_base;  // of the stage that is being loaded
+  uint32_t load_bytes, load_voff, load_to;
+  auto begin_stage = [&](uint64_t src, uint32_t bytes, int kt, int buffer) {
+    const uint32_t off = row0 * ld + (uint32_t)kt * kBlock;
+    load_base = src + off;
+    load_bytes = max((int)(bytes - off), 0);
+    load_voff = lchunk + (uint32_t)kt * kBlock < (uint32_t)g.K ? lvoff : 0xFFFFFFF0u;
+    load_to = lds_addr(lds) + (uint32_t)buffer * kStage + (uint32_t)(wave * kLoads) * 1024;
+  };
+  auto load = [&](int i) {
+    const uint32_t off = (uint32_t)(8 * i) * ld;
+    lds_dma_b128_hot(uniform_rsrc(load_base + off, (uint32_t)max((int)(load_bytes - off), 0)), load_voff, load_to + i * 1024);
+  };
   float sa[kFm], sw;
-  auto load_scales = [&](int kt) {
+  auto load_scales = [&](uint64_t rows, uint32_t rows_bytes, uint64_t ws, uint32_t ws_bytes, int kt) {
     kt = min(kt, g.KB - 1);
+    const uint64_t base = rows + (uint64_t)kt * ((uint64_t)g.as_blk * 4);
 #pragma unroll
-    for (int j = 0; j < kFm; ++j) sa[j] = ps[(int64_t)kt * g.as_blk + mo[j]];
-    sw = pw[kt];
+    for (int j = 0; j < kFm; ++j) sa[j] = uniform_load(base, rows_bytes, (mw + c) * 4 + 64 * j);
+    sw = uniform_load(ws + (uint64_t)kt * 4, ws_bytes ? 4u : 0u, 0);
   };
   // lane's bytes of a row: chunks q and 4 + q (in both operands, so the order of k is of no account)
-  const int o0 = (q ^ fp8_slot(c)) << 4, o1 = ((4 + q) ^ fp8_slot(c)) << 4;
-  auto fragment = [&](int kt, int row) {
-    const uint8_t* p = lds + (kt & 1) * kStage + (row + c) * kBlock;
+  const int o0 = c * kBlock + ((q ^ fp8_slot(c)) << 4), o1 = c * kBlock + (((4 + q) ^ fp8_slot(c)) << 4);
+  auto fragment = [&](int buffer, int row) {
+    const uint8_t* p = lds + buffer * kStage + row * kBlock;
     const u32x4 x = *reinterpret_cast<const u32x4*>(p + o0), y = *reinterpret_cast<const u32x4*>(p + o1);
     return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
   };
-
-  f32x4 acc[kFn][kFm], p[kFm];
-  float s[kFm];
-  i32x8 fa[kFm], fw[2];
-#pragma unroll
-  for (int j = 0; j < kFm; ++j) {
-    p[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    s[j] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kFn; ++i) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
 
   // A stage is kFn rows of kFm MFMAs (one weight fragment each). Beside an MFMA run the multiply-adds of the same column's MFMA one row
   // before, the reads of the next row's weight fragment and the loads of the stages ahead, in this order (the scheduling barriers keep it: left
   // to itself the compiler put every multiply-add right behind its MFMA and waited). Before the last row every wave has read all of its stage
   // and the next one is in LDS: the one barrier of a stage. The last row then reads the next stage's first fragments, and the stage
-  // after next is loaded into the buffer from there on.
-  load_scales(0);
+  // after next is loaded into the buffer from there on. A tile's last stages load the first ones of the workgroup's next tile, so that only the
+  // epilogue's own work is between two tiles.
+  int v = blockIdx.x;
+  Fp8Tile t = tile_of(v), tn = tile_of(v + gridDim.x);
+  int buf = 0;  // buffer of the stage
+  load_scales(t.scales, t.scales_bytes, t.wscales, t.wscales_bytes, 0);
+  begin_stage(t.src, t.src_bytes, 0, 0);
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) load(0, i);
+  for (int i = 0; i < kLoads; ++i) load(i);
+  begin_stage(t.src, t.src_bytes, 1, 1);
 #pragma unroll
-  for (int i = 0; i < kLoadsLast; ++i) load(1, i);
+  for (int i = 0; i < kLoadsLast; ++i) load(i);
   __builtin_amdgcn_s_waitcnt(waitcnt_vm(kLoadsLast));
   __syncthreads();
+  f32x4 acc[kFn][kFm], p[kFm];
+  float s[kFm];
+  i32x8 fa[kFm], fw[2];
 #pragma unroll
   for (int j = 0; j < kFm; ++j) fa[j] = fragment(0, kTn + mw + 16 * j);
   fw[0] = fragment(0, nw);
-  float sn[kFm];  // of the stage
-#pragma unroll
-  for (int j = 0; j < kFm; ++j) sn[j] = sa[j] * sw;
-  load_scales(1);
 
-  for (int kt = 0; kt < g.KB; ++kt) {
-#pragma unroll
-    for (int i = 0; i < kFn; ++i) {
-      const bool last = i == kFn - 1;
-      if (last) {
-        __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0));
-        __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-        __syncthreads();
-      }
-      if (last) fw[(i + 1) & 1] = fragment(kt + 1, nw);
-      else fw[(i + 1) & 1] = fragment(kt, nw + 16 * (i + 1));
-      float f[kFm];  // the factors of the row before
-#pragma unroll
-      for (int j = 0; j < kFm; ++j) f[j] = s[j];
-      if (i == 0) {
-#pragma unroll
-        for (int j = 0; j < kFm; ++j) s[j] = sn[j];
-      }
-      if (last) {
-#pragma unroll
-        for (int j = 0; j < kFm; ++j) sn[j] = sa[j] * sw;
-        load_scales(kt + 2);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int j = 0; j < kFm; ++j) {
-        const int prev = i == 0 ? kFn - 1 : i - 1;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[prev][j][r] = fmaf(p[j][r], f[j], acc[prev][j][r]);
-        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-        p[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[i & 1], fa[j], zero, 0, 0, 0, 0, 0, 0);
-        if (last) fa[j] = fragment(kt + 1, kTn + mw + 16 * j);
-        if (last) {
-#pragma unroll
-          for (int l = j * kLoadsLast / kFm; l < (j + 1) * kLoadsLast / kFm; ++l) load(kt + 2, l);
-        } else {
-#pragma unroll
-          for (int l = j * kLoadsLast / kFm; l < (j + 1) * kLoadsLast / kFm; ++l)
-            if (kLoadsLast * (i + 1) + l < kLoads) load(kt + 1, kLoadsLast * (i + 1) + l);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < kFm; ++j)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) acc[kFn - 1][j][r] = fmaf(p[j][r], s[j], acc[kFn - 1][j][r]);
-  __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // (loads of stages behind the last move nothing, and are waited for)
-  __syncthreads();  // LDS is free
-
-  // ---- epilogue: lane holds features nw + 16 i + 4 q .. + 3 of row mw + 16 j + c; rows are staged in LDS and stored whole ----
-  constexpr int kRow = 32 * kFn;  // bytes of a wave's row
-  constexpr int kCh = kRow / 16;  // chunks
-  static_assert(kWaves * 16 * kFm * kRow <= 2 * kStage, "staging fits the ring");
-  uint8_t* stage = lds + wave * (16 * kFm * kRow);
-#pragma unroll
-  for (int i = 0; i < kFn; ++i) {
-    f32x4 b = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int n = n0 + nw + 16 * i + 4 * q;
-    if (g.bias && n < g.N) b = *reinterpret_cast<const f32x4*>(g.bias + n);
+  for (;;) {
 #pragma unroll
     for (int j = 0; j < kFm; ++j) {
-      float y[4];
+      p[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      s[j] = 0.0f;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        y[r] = acc[i][j][r] + b[r];
-        if (g.gelu) y[r] = gelu_tanh_f32(y[r]);
-      }
-      *reinterpret_cast<uint2*>(stage + (16 * j + c) * kRow + (((2 * i + (q >> 1)) ^ (c & (kCh - 1))) << 4) + 8 * (q & 1)) =
-          make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+      for (int i = 0; i < kFn; ++i) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-  }
-  constexpr int kPer = 64 / kCh;  // rows of a store
-  const int ch = lane % kCh;
-  const int n = n0 + nw + 8 * ch;
+    for (int kt = 0; kt < stages; ++kt) {
 #pragma unroll
-  for (int it = 0; it < 16 * kFm / kPer; ++it) {
-    const int r = it * kPer + lane / kCh;
-    const u32x4 v = *reinterpret_cast<const u32x4*>(stage + r * kRow + ((ch ^ (r & (kCh - 1))) << 4));
-    const int m = m0 + mw + r;
-    if (m < g.M && n < g.N) store_b128_guarded(v, g.out + (int64_t)m * g.ldo + n);
+      for (int i = 0; i < kFn; ++i) {
+        const bool last = i == kFn - 1;
+        if (last) {
+          __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0));
+          __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+          __syncthreads();
+          // the scales of the next stage are here: the compiler's own wait for them belongs here too, not behind the loads below
+#pragma unroll
+          for (int j = 0; j < kFm; ++j) asm volatile("" : "+v"(sa[j]));
+          asm volatile("" : "+v"(sw));
+          const bool here = kt + 2 < stages;  // (selected, not branched)
+          begin_stage(here ? t.src : tn.src, here ? t.src_bytes : tn.src_bytes, here ? kt + 2 : kt + 2 - stages, buf);
+        }
+        fw[(i + 1) & 1] = last ? fragment(buf ^ 1, nw) : fragment(buf, nw + 16 * (i + 1));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < kFm; ++j) {
+          const int prev = i == 0 ? kFn - 1 : i - 1;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[prev][j][r] = fmaf(p[j][r], s[j], acc[prev][j][r]);
+          if (i == 0) s[j] = sa[j] * sw;  // of this stage, from here on
+          const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+          p[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[i & 1], fa[j], zero, 0, 0, 0, 0, 0, 0);
+          if (last) fa[j] = fragment(buf ^ 1, kTn + mw + 16 * j);
+#pragma unroll
+          for (int l = j * kLoadsLast / kFm; l < (j + 1) * kLoadsLast / kFm; ++l) {
+            const int at = last ? l : kLoadsLast * (i + 1) + l;
+            if (at < kLoads) load(at);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (i == 0) {
+          const bool here = kt + 1 < stages;
+          load_scales(here ? t.scales : tn.scales, here ? t.scales_bytes : tn.scales_bytes, here ? t.wscales : tn.wscales,
+                      here ? t.wscales_bytes : tn.wscales_bytes, here ? kt + 1 : 0);
+          // the bias of the wave's features, where its first output rows will be staged
+          if (kt == 0)
+            lds_dma_b128(first_lane_rsrc(g.bias + t.n0 + nw, g.bias ? (uint32_t)min(max(g.N - t.n0 - nw, 0), 16 * kFn) * 4 : 0u),
+                         (uint32_t)lane * 16, lds_addr(staging) + wave * kStaging);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      buf ^= 1;
+    }
+#pragma unroll
+    for (int j = 0; j < kFm; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[kFn - 1][j][r] = fmaf(p[j][r], s[j], acc[kFn - 1][j][r]);
+
+    // ---- epilogue: lane holds features nw + 16 i + 4 q .. + 3 of row mw + 16 j + c. Sixteen rows at a time are staged in the wave's LDS
+    // and stored whole, past L2: they are written once and read by the next kernel ----
+    constexpr int kCh = kRow / 16, kPer = 64 / kCh;  // chunks of a row, rows of a store
+    uint8_t* stage = staging + wave * kStaging;
+    const int el = fresh_lane_id(), ec = el & 15, eq = el >> 4;  // (nothing of the epilogue is held through the loop)
+#pragma unroll
+    for (int i = 0; i < kFn; ++i) {
+      const f32x4 b = *reinterpret_cast<const f32x4*>(stage + 64 * i + 16 * eq);
+#pragma unroll
+      for (int j = 0; j < kFm; ++j) acc[i][j] += b;
+    }
+    const int rows = min(max(g.M - t.m0 - mw, 0), 16 * kFm);
+    const uint64_t po = reinterpret_cast<uint64_t>(g.out + (int64_t)(t.m0 + mw) * g.ldo + t.n0 + nw);
+    // (the same in every lane, which the compiler does not prove: without this each store became a loop over the lanes' values)
+    const uint32_t plo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)po), phi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(po >> 32));
+    const uint64_t pu = ((uint64_t)phi << 32) | plo;
+    const auto ro = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(pu), (short)0, (int)__builtin_amdgcn_readfirstlane((uint32_t)rows * (uint32_t)g.ldo * 2), 0x00020000);
+    const int ch = el % kCh;
+    const bool in = t.n0 + nw + 8 * ch < g.N;
+#pragma unroll
+    for (int j = 0; j < kFm; ++j) {
+#pragma unroll
+      for (int i = 0; i < kFn; ++i) {
+        float y[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          y[r] = acc[i][j][r];
+          if (g.gelu) y[r] = gelu_tanh_f32(y[r]);
+        }
+        *reinterpret_cast<uint2*>(stage + ec * kRow + (((2 * i + (eq >> 1)) ^ (ec & (kCh - 1))) << 4) + 8 * (eq & 1)) =
+            make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+      }
+#pragma unroll
+      for (int it = 0; it < 16 / kPer; ++it) {
+        const int r = it * kPer + el / kCh;
+        const u32x4 d = *reinterpret_cast<const u32x4*>(stage + r * kRow + ((ch ^ (r & (kCh - 1))) << 4));
+        const uint32_t off = (uint32_t)(16 * j + r) * (uint32_t)g.ldo * 2 + (uint32_t)ch * 16;  // (rows past M are dropped)
+        __builtin_amdgcn_raw_buffer_store_b128(d, ro, (int)(in ? off : 0xFFFFFFF0u), 0, 2);
+      }
+    }
+    v += gridDim.x;
+    if (v >= total) break;
+    t = tn;
+    tn = tile_of(v + gridDim.x);
   }
+  __builtin_amdgcn_s_waitcnt(0);  // no load may still be under way to LDS when the workgroup ends
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -371,10 +427,11 @@ static void launch_quantize(const uint16_t* x, int64_t ldx, int M, int K, uint8_
 }
 
 template <int kTn, int kTm, int kWn, int kWm>
-static void launch_tiles(Fp8Args g, hipStream_t st) {
+static void launch_tiles(Fp8Args g, int64_t wgs, hipStream_t st) {
   g.tiles_m = (g.M + kTm - 1) / kTm;
   g.tiles_n = (g.N + kTn - 1) / kTn;
-  hipLaunchKernelGGL((fp8_block_gemm_kernel<kTn, kTm, kWn, kWm>), dim3((unsigned)(g.tiles_m * g.tiles_n)), dim3(64 * kWn * kWm), 0, st, g);
+  const int64_t total = (int64_t)g.tiles_m * g.tiles_n;
+  hipLaunchKernelGGL((fp8_block_gemm_kernel<kTn, kTm, kWn, kWm>), dim3((unsigned)std::min(total, wgs)), dim3(64 * kWn * kWm), 0, st, g);
 }
 
 template <int kFm>
@@ -436,7 +493,7 @@ extern "C" int wanmi_fp8_block_linear(const void* x, const float* x_scales, int6
   WANMI_REQUIRE(x && w && w_scales && out, WANMI_ERR_ARG, "%s: null pointer", what);
   WANMI_REQUIRE(((uintptr_t)x | (uintptr_t)w | (uintptr_t)out | (uintptr_t)bias) % 16 == 0, WANMI_ERR_ARG, "%s: x, w, bias and out must be 16-byte aligned", what);
   WANMI_REQUIRE(ldx % align == 0 && (M == 1 || ldx >= K) && ldx < (1 << 23), WANMI_ERR_ARG, "%s: rows of x, %lld apart, must be 16-byte aligned", what, (long long)ldx);
-  WANMI_REQUIRE(ldo % 8 == 0 && ldo >= N, WANMI_ERR_ARG, "%s: the output's row stride %lld must be a multiple of 8 of at least N", what, (long long)ldo);
+  WANMI_REQUIRE(ldo % 8 == 0 && ldo >= N && ldo < (1 << 24), WANMI_ERR_ARG, "%s: the output's row stride %lld must be a multiple of 8 of at least N, below 2^24", what, (long long)ldo);
   const int64_t need = wanmi_fp8_block_workspace(M, K, is_bf16);
   WANMI_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 16 == 0)), WANMI_ERR_ARG,
                 "%s: the workspace holds %lld bytes of %lld", what, (long long)workspace_bytes, (long long)need);
@@ -464,9 +521,9 @@ extern "C" int wanmi_fp8_block_linear(const void* x, const float* x_scales, int6
   } else {
     const int cus = device_cu_count();
     const int64_t big = ((M + 255) / 256) * ((N + 255) / 256), mid = ((M + 127) / 128) * ((N + 127) / 128);
-    if (big >= cus) launch_tiles<256, 256, 2, 4>(g, st);
-    else if (mid >= cus) launch_tiles<128, 128, 2, 2>(g, st);
-    else launch_tiles<64, 64, 2, 2>(g, st);
+    if (big >= cus) launch_tiles<256, 256, 2, 4>(g, cus, st);
+    else if (mid >= cus) launch_tiles<128, 128, 2, 2>(g, 2 * cus, st);
+    else launch_tiles<64, 64, 2, 2>(g, 4 * cus, st);
   }
   return check_launch(what);
 }

@@ -125,7 +125,7 @@ __device__ __forceinline__ float uniform_load(uint64_t base, uint32_t bytes, int
   return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
 }
 
-template <int kTn, int kTm, int kWn, int kWm>  // the tile and how many waves along each side
+template <int kTn, int kTm, int kWn, int kWm, int kRing>  // the tile, how many waves along each side, stages in LDS
 __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Args g) {
   static_assert(kTn == kTm, "half of the waves loads either operand");
   constexpr int kWaves = kWn * kWm;
@@ -136,9 +136,16 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
   static_assert(kFn % 2 == 0 && kLoads % kLoadsLast == 0 && kLoads / kLoadsLast < kFn, "fragments alternate; loads end before the wait for them");
   constexpr int kRow = 32 * kFn;         // bytes of a wave's output row
   constexpr int kStaging = 16 * kRow;    // sixteen rows
+  // The scales of a stage: into registers one stage ahead, or with more stages in LDS through it as well (the compiler waits for loads into
+  // registers as if there were no others under way, for all of them).
+  constexpr bool kLdsScales = kRing > 2;
+  constexpr int kScales = kLdsScales ? 4 * kTm + 512 : 0;  // bytes: of the rows, of the weight (256, one value counts), unused
+  constexpr int kStageLoads = kLoads + (kLdsScales ? 1 : 0);
+  static_assert(!kLdsScales || (kTn <= kBlock && kTm / 64 < kWaves), "one weight scale a tile; a wave each for the loads of the scales");
   static_assert(kStaging >= 1024, "a load of the bias fits");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kRing * (kStage + kScales)];
   __shared__ __attribute__((aligned(1024))) uint8_t staging[kWaves * kStaging];
+  constexpr int kScalesAt = kRing * kStage;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, q = lane >> 4;
   const int mw = (wave % kWm) * 16 * kFm, nw = (wave / kWm) * 16 * kFn;  // the wave's first row and feature
@@ -188,6 +195,22 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
     for (int j = 0; j < kFm; ++j) sa[j] = uniform_load(base, rows_bytes, (mw + c) * 4 + 64 * j);
     sw = uniform_load(ws + (uint64_t)kt * 4, ws_bytes ? 4u : 0u, 0);
   };
+  // the wave's part of a stage's scales: 64 rows', the weight's one, or nothing
+  auto dma_scales = [&](uint64_t rows, uint32_t rows_bytes, uint64_t ws, uint32_t ws_bytes, int kt, int buffer) {
+    if constexpr (kLdsScales) {
+      const bool row = wave < kTm / 64, one = wave == kTm / 64;
+      kt = min(kt, g.KB - 1);
+      const uint64_t base = row ? rows + (uint64_t)kt * ((uint64_t)g.as_blk * 4) + 256 * wave : ws + (uint64_t)kt * 4;
+      const uint32_t bytes = row ? (uint32_t)max((int)rows_bytes - 256 * wave, 0) : one && ws_bytes ? 4u : 0u;
+      lds_dma_b32(uniform_rsrc(base, bytes), (uint32_t)lane * 4, lds_addr(lds) + kScalesAt + buffer * kScales + (row ? 256 * wave : one ? 4 * kTm : 4 * kTm + 256));
+    }
+  };
+  auto read_scales = [&](int buffer) {
+    const float* p = reinterpret_cast<const float*>(lds + kScalesAt + buffer * kScales);
+#pragma unroll
+    for (int j = 0; j < kFm; ++j) sa[j] = p[mw + c + 16 * j];
+    sw = p[kTm];
+  };
   // lane's bytes of a row: chunks q and 4 + q (in both operands, so the order of k is of no account)
   const int o0 = c * kBlock + ((q ^ fp8_slot(c)) << 4), o1 = c * kBlock + (((4 + q) ^ fp8_slot(c)) << 4);
   auto fragment = [&](int buffer, int row) {
@@ -205,14 +228,16 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
   int v = blockIdx.x;
   Fp8Tile t = tile_of(v), tn = tile_of(v + gridDim.x);
   int buf = 0;  // buffer of the stage
-  load_scales(t.scales, t.scales_bytes, t.wscales, t.wscales_bytes, 0);
-  begin_stage(t.src, t.src_bytes, 0, 0);
+  if constexpr (!kLdsScales) load_scales(t.scales, t.scales_bytes, t.wscales, t.wscales_bytes, 0);
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) load(i);
-  begin_stage(t.src, t.src_bytes, 1, 1);
+  for (int st = 0; st < kRing; ++st) {  // (of the last one of them only what a last row loads)
+    begin_stage(t.src, st < stages ? t.src_bytes : 0u, st, st);
+    dma_scales(t.scales, t.scales_bytes, t.wscales, t.wscales_bytes, st, st);
 #pragma unroll
-  for (int i = 0; i < kLoadsLast; ++i) load(i);
-  __builtin_amdgcn_s_waitcnt(waitcnt_vm(kLoadsLast));
+    for (int i = 0; i < (st < kRing - 1 ? kLoads : kLoadsLast); ++i) load(i);
+  }
+  constexpr int kFirstWait = (kRing - 2) * kStageLoads + kLoadsLast + (kLdsScales ? 1 : 0);  // loads behind the first stage's
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(kFirstWait));
   __syncthreads();
   f32x4 acc[kFn][kFm], p[kFm];
   float s[kFm];
@@ -220,6 +245,7 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
 #pragma unroll
   for (int j = 0; j < kFm; ++j) fa[j] = fragment(0, kTn + mw + 16 * j);
   fw[0] = fragment(0, nw);
+  if constexpr (kLdsScales) read_scales(0);
 
   for (;;) {
 #pragma unroll
@@ -235,16 +261,26 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
         const bool last = i == kFn - 1;
         if (last) {
           __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0));
-          __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+          __builtin_amdgcn_s_waitcnt(waitcnt_vm((kRing - 2) * kStageLoads));
           __syncthreads();
-          // the scales of the next stage are here: the compiler's own wait for them belongs here too, not behind the loads below
+          if constexpr (!kLdsScales) {
+            // the scales of the next stage are here: the compiler's own wait for them belongs here too, not behind the loads below
 #pragma unroll
-          for (int j = 0; j < kFm; ++j) asm volatile("" : "+v"(sa[j]));
-          asm volatile("" : "+v"(sw));
-          const bool here = kt + 2 < stages;  // (selected, not branched)
-          begin_stage(here ? t.src : tn.src, here ? t.src_bytes : tn.src_bytes, here ? kt + 2 : kt + 2 - stages, buf);
+            for (int j = 0; j < kFm; ++j) asm volatile("" : "+v"(sa[j]));
+            asm volatile("" : "+v"(sw));
+          }
+          const bool here = kt + kRing < stages;  // (selected, not branched)
+          const int ahead = here ? kt + kRing : kt + kRing - stages;
+          if constexpr (kRing == 2) {
+            begin_stage(here ? t.src : tn.src, here ? t.src_bytes : tn.src_bytes, ahead, buf);
+          } else {  // (no next tile)
+            begin_stage(t.src, here ? t.src_bytes : 0u, ahead, buf);
+            dma_scales(t.scales, t.scales_bytes, t.wscales, t.wscales_bytes, ahead, buf);
+          }
         }
-        fw[(i + 1) & 1] = last ? fragment(buf ^ 1, nw) : fragment(buf, nw + 16 * (i + 1));
+        const int next = buf + 1 == kRing ? 0 : buf + 1;
+        fw[(i + 1) & 1] = last ? fragment(next, nw) : fragment(buf, nw + 16 * (i + 1));
+        if (kLdsScales && last) read_scales(next);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < kFm; ++j) {
@@ -254,7 +290,7 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
           if (i == 0) s[j] = sa[j] * sw;  // of this stage, from here on
           const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
           p[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[i & 1], fa[j], zero, 0, 0, 0, 0, 0, 0);
-          if (last) fa[j] = fragment(buf ^ 1, kTn + mw + 16 * j);
+          if (last) fa[j] = fragment(next, kTn + mw + 16 * j);
 #pragma unroll
           for (int l = j * kLoadsLast / kFm; l < (j + 1) * kLoadsLast / kFm; ++l) {
             const int at = last ? l : kLoadsLast * (i + 1) + l;
@@ -263,8 +299,8 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
           __builtin_amdgcn_sched_barrier(0);
         }
         if (i == 0) {
-          const bool here = kt + 1 < stages;
-          load_scales(here ? t.scales : tn.scales, here ? t.scales_bytes : tn.scales_bytes, here ? t.wscales : tn.wscales,
+          [[maybe_unused]] const bool here = kt + 1 < stages;
+          if constexpr (!kLdsScales) load_scales(here ? t.scales : tn.scales, here ? t.scales_bytes : tn.scales_bytes, here ? t.wscales : tn.wscales,
                       here ? t.wscales_bytes : tn.wscales_bytes, here ? kt + 1 : 0);
           // the bias of the wave's features, where its first output rows will be staged
           if (kt == 0)
@@ -273,13 +309,14 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      buf ^= 1;
+      buf = buf + 1 == kRing ? 0 : buf + 1;
     }
 #pragma unroll
     for (int j = 0; j < kFm; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) acc[kFn - 1][j][r] = fmaf(p[j][r], s[j], acc[kFn - 1][j][r]);
 
+    if constexpr (kRing > 2) __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // the bias: the waits of a short sum may not have reached it
     // ---- epilogue: lane holds features nw + 16 i + 4 q .. + 3 of row mw + 16 j + c. Sixteen rows at a time are staged in the wave's LDS
     // and stored whole, past L2: they are written once and read by the next kernel ----
     constexpr int kCh = kRow / 16, kPer = 64 / kCh;  // chunks of a row, rows of a store
@@ -426,12 +463,12 @@ static void launch_quantize(const uint16_t* x, int64_t ldx, int M, int K, uint8_
   hipLaunchKernelGGL(fp8_block_quantize_kernel, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, x, ldx, M, K, KB, codes, scales, s_row, s_blk);
 }
 
-template <int kTn, int kTm, int kWn, int kWm>
+template <int kTn, int kTm, int kWn, int kWm, int kRing>
 static void launch_tiles(Fp8Args g, int64_t wgs, hipStream_t st) {
   g.tiles_m = (g.M + kTm - 1) / kTm;
   g.tiles_n = (g.N + kTn - 1) / kTn;
   const int64_t total = (int64_t)g.tiles_m * g.tiles_n;
-  hipLaunchKernelGGL((fp8_block_gemm_kernel<kTn, kTm, kWn, kWm>), dim3((unsigned)std::min(total, wgs)), dim3(64 * kWn * kWm), 0, st, g);
+  hipLaunchKernelGGL((fp8_block_gemm_kernel<kTn, kTm, kWn, kWm, kRing>), dim3((unsigned)std::min(total, wgs)), dim3(64 * kWn * kWm), 0, st, g);
 }
 
 template <int kFm>
@@ -471,9 +508,9 @@ extern "C" int wanmi_fp8_block_quantize(const void* x, int64_t ldx, int64_t M, i
   return check_launch(what);
 }
 
-extern "C" int64_t wanmi_fp8_block_workspace(int64_t M, int64_t K, int is_bf16) {
+extern "C" int64_t wanmi_fp8_block_workspace(int64_t M, int64_t K, int is_bf16, int64_t xs_row) {
   using namespace wanmi;
-  if (M <= 0 || K <= 0 || M <= (is_bf16 ? kFewQuantize : kFewRows)) return 0;
+  if (M <= 0 || K <= 0 || M <= (is_bf16 ? kFewQuantize : kFewRows) || (!is_bf16 && xs_row == 1)) return 0;
   const int64_t codes = is_bf16 ? (M * K + 255) / 256 * 256 : 0;
   return codes + M * blocks_of(K) * 4;
 }
@@ -494,7 +531,7 @@ extern "C" int wanmi_fp8_block_linear(const void* x, const float* x_scales, int6
   WANMI_REQUIRE(((uintptr_t)x | (uintptr_t)w | (uintptr_t)out | (uintptr_t)bias) % 16 == 0, WANMI_ERR_ARG, "%s: x, w, bias and out must be 16-byte aligned", what);
   WANMI_REQUIRE(ldx % align == 0 && (M == 1 || ldx >= K) && ldx < (1 << 23), WANMI_ERR_ARG, "%s: rows of x, %lld apart, must be 16-byte aligned", what, (long long)ldx);
   WANMI_REQUIRE(ldo % 8 == 0 && ldo >= N && ldo < (1 << 24), WANMI_ERR_ARG, "%s: the output's row stride %lld must be a multiple of 8 of at least N, below 2^24", what, (long long)ldo);
-  const int64_t need = wanmi_fp8_block_workspace(M, K, is_bf16);
+  const int64_t need = wanmi_fp8_block_workspace(M, K, is_bf16, xs_row);
   WANMI_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 16 == 0)), WANMI_ERR_ARG,
                 "%s: the workspace holds %lld bytes of %lld", what, (long long)workspace_bytes, (long long)need);
   WANMI_REQUIRE(((M + 63) / 64) * ((N + 63) / 64) < (1LL << 30) && M * ((KB + 3) / 4) < (1LL << 32), WANMI_ERR_ARG, "%s: too many tiles", what);
@@ -521,9 +558,9 @@ extern "C" int wanmi_fp8_block_linear(const void* x, const float* x_scales, int6
   } else {
     const int cus = device_cu_count();
     const int64_t big = ((M + 255) / 256) * ((N + 255) / 256), mid = ((M + 127) / 128) * ((N + 127) / 128);
-    if (big >= cus) launch_tiles<256, 256, 2, 4>(g, cus, st);
-    else if (mid >= cus) launch_tiles<128, 128, 2, 2>(g, 2 * cus, st);
-    else launch_tiles<64, 64, 2, 2>(g, 4 * cus, st);
+    if (big >= cus) launch_tiles<256, 256, 2, 4, 2>(g, cus, st);
+    else if (mid >= cus) launch_tiles<128, 128, 2, 2, 2>(g, 2 * cus, st);
+    else launch_tiles<64, 64, 2, 2, 4>(g, INT64_MAX, st);  // a tile each: with more than two stages nothing is loaded for a next one
   }
   return check_launch(what);
 }

@@ -157,7 +157,7 @@ def fp8_block_linear(x, weight: FP8BlockWeight, *, activation: str | None = None
     y = torch.empty((M, N), dtype=torch.bfloat16, device=dev) if out is None else out
     if M:
         p = _lib.ptr
-        size = _lib.load().wanmi_fp8_block_workspace(M, K, int(scales is None))
+        size = _lib.load().wanmi_fp8_block_workspace(M, K, int(scales is None), s_row)
         work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         _lib.call("wanmi_fp8_block_linear", codes.get_device(), p(codes), p(scales), ld, s_row, s_blk, p(weight.codes), p(weight.scales), p(weight.bias),
                   M, N, K, _ACTIVATIONS[activation], p(y), y.stride(0) if M > 1 else N, p(work), size)

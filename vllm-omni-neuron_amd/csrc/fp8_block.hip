@@ -366,96 +366,130 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
 }
 
 // ------------------------------------------------------------------------------------------------
-// Few rows: a workgroup of eight waves takes 16 features and all rows, the waves share out the blocks of k. The weight goes straight
-// into registers, all of a wave's loads under way together: what counts is to read it once, at the memory's rate.
+// Few rows: a workgroup of eight waves takes 16 features and all rows, the waves share out the blocks of k. What counts is to read the weight
+// once, at the memory's rate: all loads of a wave are under way together, whole 128-byte lines of eight rows to an instruction (in the
+// MFMA's own layout, half lines of sixteen rows, a launch that only read took 5.7 us in place of 2.7 on 26 MB in the caches, 7.0 and 5.9 from
+// memory), and each block then goes through 2 KB of the wave's LDS into that layout.
+// Rows in bf16 are quantized by the wave that needs them, 16 lanes to a block of a row; more than four of them in a launch of their own before
+// (16 rows here would cost every workgroup as much again as its loads).
 // ------------------------------------------------------------------------------------------------
 constexpr int kFewWaves = 8;
-constexpr int kFewAhead = 4;  // blocks whose weight is under way in a wave
+constexpr int kFewAhead = 5;      // blocks under way in a wave
+constexpr int kFewRows = 16;      // at most
+constexpr int kFewQuantize = 4;   // of them in bf16
 
-template <int kFm, bool kQuantize>
-__global__ __launch_bounds__(64 * kFewWaves) void fp8_block_few_kernel(Fp8Args g) {
-  __shared__ f32x4 red[kFewWaves][kFm][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = lane & 15, q = lane >> 4;
+__device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off, bool in) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(in ? off : 0xFFFFFFF0u), 0, 0));
+}
+
+template <bool kQuantize>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void fp8_block_few_kernel(Fp8Args g) {
+  constexpr int kPasses = kFewAhead * kFewQuantize / 4;  // four blocks of a row at a time
+  __shared__ f32x4 red[kFewWaves][64];
+  __shared__ __attribute__((aligned(16))) uint8_t turn[kFewWaves][16 * kBlock];
+  __shared__ __attribute__((aligned(16))) uint8_t codes[kQuantize ? kFewWaves : 1][kQuantize ? 4 * kPasses * kBlock : 16];
+  __shared__ float scales[kQuantize ? kFewWaves : 1][kQuantize ? 4 * kPasses : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, q = lane >> 4, r8 = lane >> 3, c8 = lane & 7;
   const int n0 = blockIdx.x * 16;
-  const uint8_t* pw = g.w + (int64_t)min(n0 + c, g.N - 1) * g.K + 32 * q;
+  // (rows behind N and chunks behind K read as zeros)
+  const auto rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(g.w) + (int64_t)n0 * g.K, (short)0, min(16, g.N - n0) * g.K, 0x00020000);
+  const void* rows = kQuantize ? (const void*)g.x : (const void*)g.a;
+  const int row_bytes = (int)g.lda * (kQuantize ? 2 : 1), k_bytes = g.K * (kQuantize ? 2 : 1);
+  const auto rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(rows), (short)0, (g.M - 1) * row_bytes + k_bytes, 0x00020000);
   const float* psw = g.w_scales + (int64_t)(n0 / kBlock) * g.KB;
-  int row[kFm];
-#pragma unroll
-  for (int j = 0; j < kFm; ++j) row[j] = min(16 * j + c, g.M - 1);
-  f32x4 acc[kFm];
-#pragma unroll
-  for (int j = 0; j < kFm; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const u32x4 none = {0u, 0u, 0u, 0u};
+  const int row = min(c, g.M - 1);
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 
   for (int b0 = wave; b0 < g.KB; b0 += kFewWaves * kFewAhead) {
-    u32x4 w[kFewAhead][2];
+    u32x4 w[kFewAhead][2], x[kQuantize ? kPasses : kFewAhead][2];
+    float sw[kFewAhead], sx[kFewAhead];
 #pragma unroll
     for (int u = 0; u < kFewAhead; ++u) {
-      const int k = (b0 + kFewWaves * u) * kBlock + 32 * q;  // K is a multiple of 16
-      w[u][0] = k < g.K ? *reinterpret_cast<const u32x4*>(pw + (k - 32 * q)) : none;
-      w[u][1] = k + 16 < g.K ? *reinterpret_cast<const u32x4*>(pw + (k - 32 * q) + 16) : none;
+      const int k = (b0 + kFewWaves * u) * kBlock + 16 * c8;
+      w[u][0] = load16(rw, (uint32_t)(r8 * g.K + k), k < g.K);
+      w[u][1] = load16(rw, (uint32_t)((8 + r8) * g.K + k), k < g.K);
     }
 #pragma unroll
     for (int u = 0; u < kFewAhead; ++u) {
-      const int b = b0 + kFewWaves * u;
-      if (b >= g.KB) break;
-      const int k = b * kBlock + 32 * q;
-      const i32x8 fw = {(int)w[u][0][0], (int)w[u][0][1], (int)w[u][0][2], (int)w[u][0][3], (int)w[u][1][0], (int)w[u][1][1], (int)w[u][1][2], (int)w[u][1][3]};
-      const float sw = psw[b];
-#pragma unroll
-      for (int j = 0; j < kFm; ++j) {
-        i32x8 fa;
-        float s;
-        if constexpr (kQuantize) {
-          const u32x4* px = reinterpret_cast<const u32x4*>(g.x + row[j] * g.lda + k);
-          u32x4 v[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = k + 16 * (i >> 1) < g.K ? px[i] : none;
-          uint32_t best = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) best = max_magnitude(best, v[i][e]);
-          best = max_magnitude(best, (uint32_t)__shfl_xor((int)best, 16, 64));
-          best = max_magnitude(best, (uint32_t)__shfl_xor((int)best, 32, 64));
-          s = block_scale(best);
-          const float y = 1.0f / s;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) fa[i] = (int)four_codes(v[i >> 1][2 * (i & 1)], v[i >> 1][2 * (i & 1) + 1], s, y);
-        } else {
-          const u32x4* pa = reinterpret_cast<const u32x4*>(g.a + row[j] * g.lda + k);
-          const u32x4 lo = k < g.K ? pa[0] : none, hi = k + 16 < g.K ? pa[1] : none;
-          fa = i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
-          s = g.a_scales[row[j] * g.as_row + b * g.as_blk];
-        }
-        s *= sw;
-        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-        const f32x4 p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, fa, zero, 0, 0, 0, 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(p[r], s, acc[j][r]);
+      const int b = min(b0 + kFewWaves * u, g.KB - 1);
+      sw[u] = psw[b];
+      if constexpr (!kQuantize) {
+        const int k = (b0 + kFewWaves * u) * kBlock + 16 * q;
+        x[u][0] = load16(rx, (uint32_t)(row * row_bytes + k), k < g.K);
+        x[u][1] = load16(rx, (uint32_t)(row * row_bytes + k + 64), k + 64 < g.K);
+        sx[u] = g.a_scales[row * g.as_row + b * g.as_blk];
       }
     }
+    if constexpr (kQuantize) {
+      // block i of the batch's M * kFewAhead: block i % kFewAhead of row i / kFewAhead; 8 values a lane
+      const int blocks = g.M * kFewAhead;
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) {
+        const int i = 4 * p + q, m = i / kFewAhead, k = (b0 + kFewWaves * (i - m * kFewAhead)) * kBlock + 8 * c;
+        if (4 * p < blocks) x[p][0] = load16(rx, (uint32_t)(m * row_bytes + 2 * k), i < blocks && k < g.K);
+      }
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) {
+        if (4 * p >= blocks) break;
+        uint32_t best = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) best = max_magnitude(best, x[p][0][e]);
+        // over the 16 lanes: quad permutes, then the half-row and row mirrors, which pair equal quads
+        best = max_magnitude(best, (uint32_t)dpp_i32<0xB1>((int)best));
+        best = max_magnitude(best, (uint32_t)dpp_i32<0x4E>((int)best));
+        best = max_magnitude(best, (uint32_t)dpp_i32<0x141>((int)best));
+        best = max_magnitude(best, (uint32_t)dpp_i32<0x140>((int)best));
+        const float s = block_scale(best), y = 1.0f / s;
+        const int i = 4 * p + q;
+        *reinterpret_cast<uint2*>(&codes[wave][i * kBlock + 8 * c]) = make_uint2(four_codes(x[p][0][0], x[p][0][1], s, y), four_codes(x[p][0][2], x[p][0][3], s, y));
+        if (c == 0) scales[wave][i] = s;
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);  // (the compiler sank the loads to their uses)
+#pragma unroll
+    for (int u = 0; u < kFewAhead; ++u) {
+      // into the MFMA's layout: row c's chunks q and 4 + q (a wave's LDS operations complete in order)
+      uint8_t* t = turn[wave];
+      *reinterpret_cast<u32x4*>(t + r8 * kBlock + ((c8 ^ fp8_slot(r8)) << 4)) = w[u][0];
+      *reinterpret_cast<u32x4*>(t + (8 + r8) * kBlock + ((c8 ^ fp8_slot(r8)) << 4)) = w[u][1];
+      const u32x4 w0 = *reinterpret_cast<const u32x4*>(t + c * kBlock + ((q ^ fp8_slot(c)) << 4));
+      const u32x4 w1 = *reinterpret_cast<const u32x4*>(t + c * kBlock + (((4 + q) ^ fp8_slot(c)) << 4));
+      const i32x8 fw = {(int)w0[0], (int)w0[1], (int)w0[2], (int)w0[3], (int)w1[0], (int)w1[1], (int)w1[2], (int)w1[3]};
+      u32x4 x0, x1;
+      float s;
+      if constexpr (kQuantize) {
+        const int i = row * kFewAhead + u;
+        x0 = *reinterpret_cast<const u32x4*>(&codes[wave][i * kBlock + 16 * q]);
+        x1 = *reinterpret_cast<const u32x4*>(&codes[wave][i * kBlock + 64 + 16 * q]);
+        s = scales[wave][i];
+      } else {
+        x0 = x[u][0], x1 = x[u][1];
+        s = sx[u];
+      }
+      const i32x8 fa = {(int)x0[0], (int)x0[1], (int)x0[2], (int)x0[3], (int)x1[0], (int)x1[1], (int)x1[2], (int)x1[3]};
+      s = b0 + kFewWaves * u < g.KB ? s * sw[u] : 0.0f;  // (blocks behind the last have codes of zero)
+      const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+      const f32x4 p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, fa, zero, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[r] = fmaf(p[r], s, acc[r]);
+    }
   }
-#pragma unroll
-  for (int j = 0; j < kFm; ++j) red[wave][j][lane] = acc[j];
+  red[wave][lane] = acc;
   __syncthreads();
-  if (wave >= kFm) return;  // wave j adds the parts of fragment j, in the waves' order
-  f32x4 y = red[0][wave][lane];
+  if (wave > 0) return;  // the parts in the waves' order
+  f32x4 y = red[0][lane];
 #pragma unroll
-  for (int w = 1; w < kFewWaves; ++w) y += red[w][wave][lane];
-  const int m = 16 * wave + c, n = n0 + 4 * q;
-  if (m >= g.M || n >= g.N) return;
+  for (int w = 1; w < kFewWaves; ++w) y += red[w][lane];
+  const int n = n0 + 4 * q;
+  if (c >= g.M || n >= g.N) return;
   if (g.bias) y += *reinterpret_cast<const f32x4*>(g.bias + n);
   if (g.gelu) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) y[r] = gelu_tanh_f32(y[r]);
   }
-  *reinterpret_cast<uint2*>(g.out + (int64_t)m * g.ldo + n) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+  *reinterpret_cast<uint2*>(g.out + (int64_t)c * g.ldo + n) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
 }
-
-constexpr int kFewRows = 64;      // at most: beyond, tiles
-constexpr int kFewQuantize = 16;  // at most, quantizing in every workgroup: beyond, once before
 
 static void launch_quantize(const uint16_t* x, int64_t ldx, int M, int K, uint8_t* codes, float* scales, int64_t s_row, int64_t s_blk, hipStream_t st) {
   const int KB = (K + kBlock - 1) / kBlock;
@@ -469,18 +503,6 @@ static void launch_tiles(Fp8Args g, int64_t wgs, hipStream_t st) {
   g.tiles_n = (g.N + kTn - 1) / kTn;
   const int64_t total = (int64_t)g.tiles_m * g.tiles_n;
   hipLaunchKernelGGL((fp8_block_gemm_kernel<kTn, kTm, kWn, kWm, kRing>), dim3((unsigned)std::min(total, wgs)), dim3(64 * kWn * kWm), 0, st, g);
-}
-
-template <int kFm>
-static void launch_few(const Fp8Args& g, hipStream_t st) {
-  const dim3 grid((unsigned)((g.N + 15) / 16)), block(64 * kFewWaves);
-  if constexpr (16 * kFm <= kFewQuantize) {
-    if (g.x) {
-      hipLaunchKernelGGL((fp8_block_few_kernel<kFm, true>), grid, block, 0, st, g);
-      return;
-    }
-  }
-  hipLaunchKernelGGL((fp8_block_few_kernel<kFm, false>), grid, block, 0, st, g);
 }
 
 static int64_t blocks_of(int64_t K) { return (K + kBlock - 1) / kBlock; }
@@ -549,12 +571,10 @@ extern "C" int wanmi_fp8_block_linear(const void* x, const float* x_scales, int6
     hipLaunchKernelGGL(fp8_scales_kernel, dim3((unsigned)((M + 63) / 64)), dim3(256), 0, st, x_scales, xs_row, xs_blk, (int)M, (int)KB, scales);
     g.a_scales = scales, g.as_row = 1, g.as_blk = M;
   }
-  if (M <= 16) {
-    launch_few<1>(g, st);
-  } else if (M <= 32) {
-    launch_few<2>(g, st);
-  } else if (M <= kFewRows) {
-    launch_few<4>(g, st);
+  if (M <= kFewRows) {
+    const dim3 grid((unsigned)((N + 15) / 16)), block(64 * kFewWaves);
+    if (g.x) hipLaunchKernelGGL((fp8_block_few_kernel<true>), grid, block, 0, st, g);
+    else hipLaunchKernelGGL((fp8_block_few_kernel<false>), grid, block, 0, st, g);
   } else {
     const int cus = device_cu_count();
     const int64_t big = ((M + 255) / 256) * ((N + 255) / 256), mid = ((M + 127) / 128) * ((N + 127) / 128);

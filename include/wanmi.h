@@ -477,9 +477,9 @@ int wanmi_fp8_block_linear(const void* x, const float* x_scales, int64_t ldx, in
                            const float* w_scales, const float* bias, int64_t M, int64_t N, int64_t K, int gelu, void* out,
                            int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Bytes of workspace that wanmi_fp8_block_linear needs for these sizes: none for few rows, and none for codes with xs_row 1 (their scales
- * block by block, as wanmi_fp8_block_quantize can write them). */
-int64_t wanmi_fp8_block_workspace(int64_t M, int64_t K, int is_bf16, int64_t xs_row);
+/* Bytes of workspace that wanmi_fp8_block_linear needs for these sizes: for the codes of bf16 rows, for scales whose xs_row is not 1 (1: block
+ * by block, as wanmi_fp8_block_quantize can write them), and for the parts of a sum that is shared out. None for few rows. */
+int64_t wanmi_fp8_block_workspace(int64_t M, int64_t N, int64_t K, int is_bf16, int64_t xs_row);
 
 /*
  * Streaming device-to-device copy of `bytes` (a multiple of 16; src and dst 16-byte aligned, not

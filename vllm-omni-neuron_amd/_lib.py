@@ -83,7 +83,7 @@ _SIGNATURES = {
                                       _i32, _vp, _i32, _i32, _vp, _i64, _i32, _vp],
     "wanmi_fp8_block_quantize": [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp],
     "wanmi_fp8_block_linear": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp],
-    "wanmi_fp8_block_workspace": [_i64, _i64, _i32, _i64],
+    "wanmi_fp8_block_workspace": [_i64, _i64, _i64, _i32, _i64],
 }
 
 _LIB = None

@@ -12,6 +12,7 @@
 // fp32(1 / 448) is the scale, x / scale rounded to nearest the code. (bf16 values over their maximum fall onto the border between two codes often enough
 // that the last bit of the scale decides many codes: the product with the rounded reciprocal is what torch computes on the GPU for `/ 448`.)
 #include "wanmi_common.h"
+#include "fp8_plan.h"
 #include "gemm_plan.h"
 
 #include <algorithm>
@@ -34,6 +35,8 @@ struct Fp8Args {
   int M, N, K, KB;
   int gelu;
   int tiles_m, tiles_n;
+  int splits;             // of the sum over k, a workgroup each (kRing > 2)
+  float* parts;           // [splits][M][N] where there are several
 };
 
 // As the MXFP8 GEMM's: gelu_tanh(x) = x / (1 + 2^(x (k0 + k1 x^2))).
@@ -153,7 +156,10 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
   const uint32_t ld = weight ? (uint32_t)g.K : (uint32_t)g.lda;
   const uint32_t row0 = (uint32_t)(wave % (kWaves / 2)) * (8 * kLoads);  // of the rows it loads
   const int total = g.tiles_m * g.tiles_n;
-  const int stages = max(g.KB, 2);  // (the second of one block's two reads zeros)
+  // the stages of the workgroup's part of the sum: [first, first + stages)
+  const int split = kRing > 2 ? (int)(blockIdx.x / (unsigned)total) : 0;
+  const int first = kRing > 2 ? (int)((int64_t)g.KB * split / g.splits) : 0;
+  const int stages = kRing > 2 ? (int)((int64_t)g.KB * (split + 1) / g.splits) - first : max(g.KB, 2);  // (the second of one block's two reads zeros)
 
   auto tile_of = [&](int v) {
     Fp8Tile t;
@@ -225,14 +231,14 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
   // and the next one is in LDS: the one barrier of a stage. The last row then reads the next stage's first fragments, and the stage
   // after next is loaded into the buffer from there on. A tile's last stages load the first ones of the workgroup's next tile, so that only the
   // epilogue's own work is between two tiles.
-  int v = blockIdx.x;
+  int v = (int)blockIdx.x - split * total;
   Fp8Tile t = tile_of(v), tn = tile_of(v + gridDim.x);
   int buf = 0;  // buffer of the stage
   if constexpr (!kLdsScales) load_scales(t.scales, t.scales_bytes, t.wscales, t.wscales_bytes, 0);
 #pragma unroll
   for (int st = 0; st < kRing; ++st) {  // (of the last one of them only what a last row loads)
-    begin_stage(t.src, st < stages ? t.src_bytes : 0u, st, st);
-    dma_scales(t.scales, t.scales_bytes, t.wscales, t.wscales_bytes, st, st);
+    begin_stage(t.src, st < stages ? t.src_bytes : 0u, first + st, st);
+    dma_scales(t.scales, t.scales_bytes, t.wscales, t.wscales_bytes, first + st, st);
 #pragma unroll
     for (int i = 0; i < (st < kRing - 1 ? kLoads : kLoadsLast); ++i) load(i);
   }
@@ -274,8 +280,8 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
           if constexpr (kRing == 2) {
             begin_stage(here ? t.src : tn.src, here ? t.src_bytes : tn.src_bytes, ahead, buf);
           } else {  // (no next tile)
-            begin_stage(t.src, here ? t.src_bytes : 0u, ahead, buf);
-            dma_scales(t.scales, t.scales_bytes, t.wscales, t.wscales_bytes, ahead, buf);
+            begin_stage(t.src, here ? t.src_bytes : 0u, first + ahead, buf);
+            dma_scales(t.scales, t.scales_bytes, t.wscales, t.wscales_bytes, first + ahead, buf);
           }
         }
         const int next = buf + 1 == kRing ? 0 : buf + 1;
@@ -319,6 +325,17 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
     if constexpr (kRing > 2) __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // the bias: the waits of a short sum may not have reached it
     // ---- epilogue: lane holds features nw + 16 i + 4 q .. + 3 of row mw + 16 j + c. Sixteen rows at a time are staged in the wave's LDS
     // and stored whole, past L2: they are written once and read by the next kernel ----
+    if (kRing > 2 && g.splits > 1) {
+      // a part of the sum, in fp32: fp8_join_kernel adds them
+      float* po = g.parts + ((int64_t)split * g.M + t.m0 + mw + c) * g.N + t.n0 + nw + 4 * q;
+#pragma unroll
+      for (int j = 0; j < kFm; ++j)
+#pragma unroll
+        for (int i = 0; i < kFn; ++i)
+          if (t.m0 + mw + 16 * j + c < g.M && t.n0 + nw + 16 * i + 4 * q < g.N)
+            store_b128_guarded(__builtin_bit_cast(u32x4, acc[i][j]), po + (int64_t)16 * j * g.N + 16 * i);
+      return;
+    }
     constexpr int kCh = kRow / 16, kPer = 64 / kCh;  // chunks of a row, rows of a store
     uint8_t* stage = staging + wave * kStaging;
     const int el = fresh_lane_id(), ec = el & 15, eq = el >> 4;  // (nothing of the epilogue is held through the loop)
@@ -363,6 +380,34 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
     tn = tile_of(v + gridDim.x);
   }
   __builtin_amdgcn_s_waitcnt(0);  // no load may still be under way to LDS when the workgroup ends
+}
+
+// out = act(sum of the parts, in their order, + bias): eight columns a thread
+__global__ __launch_bounds__(256) void fp8_join_kernel(const float* __restrict__ parts, int splits, int M, int N, const float* __restrict__ bias, int gelu,
+                                                      uint16_t* __restrict__ out, int64_t ldo) {
+  const int per_row = N / 8;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t m = id / per_row;
+  if (m >= M) return;
+  const int n = (int)(id - m * per_row) * 8;
+  f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f}, b = a;
+  const float* p = parts + m * N + n;
+  for (int s = 0; s < splits; ++s, p += (int64_t)M * N) {
+    a += *reinterpret_cast<const f32x4*>(p);
+    b += *reinterpret_cast<const f32x4*>(p + 4);
+  }
+  if (bias) {
+    a += *reinterpret_cast<const f32x4*>(bias + n);
+    b += *reinterpret_cast<const f32x4*>(bias + n + 4);
+  }
+  if (gelu) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      a[r] = gelu_tanh_f32(a[r]);
+      b[r] = gelu_tanh_f32(b[r]);
+    }
+  }
+  store_b128_guarded(u32x4{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3])}, out + m * ldo + n);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -498,11 +543,15 @@ static void launch_quantize(const uint16_t* x, int64_t ldx, int M, int K, uint8_
 }
 
 template <int kTn, int kTm, int kWn, int kWm, int kRing>
-static void launch_tiles(Fp8Args g, int64_t wgs, hipStream_t st) {
+static void launch_tiles(Fp8Args g, int64_t wgs, hipStream_t st) {  // wgs: that walk the tiles; with more than two stages each tile (and part) has its own
   g.tiles_m = (g.M + kTm - 1) / kTm;
   g.tiles_n = (g.N + kTn - 1) / kTn;
   const int64_t total = (int64_t)g.tiles_m * g.tiles_n;
-  hipLaunchKernelGGL((fp8_block_gemm_kernel<kTn, kTm, kWn, kWm, kRing>), dim3((unsigned)std::min(total, wgs)), dim3(64 * kWn * kWm), 0, st, g);
+  hipLaunchKernelGGL((fp8_block_gemm_kernel<kTn, kTm, kWn, kWm, kRing>), dim3((unsigned)(kRing > 2 ? total * g.splits : std::min(total, wgs))),
+                     dim3(64 * kWn * kWm), 0, st, g);
+  if (kRing > 2 && g.splits > 1)
+    hipLaunchKernelGGL(fp8_join_kernel, dim3((unsigned)(((int64_t)g.M * (g.N / 8) + 255) / 256)), dim3(256), 0, st, g.parts, g.splits, g.M, g.N, g.bias, g.gelu,
+                       g.out, g.ldo);
 }
 
 static int64_t blocks_of(int64_t K) { return (K + kBlock - 1) / kBlock; }
@@ -530,11 +579,31 @@ extern "C" int wanmi_fp8_block_quantize(const void* x, int64_t ldx, int64_t M, i
   return check_launch(what);
 }
 
-extern "C" int64_t wanmi_fp8_block_workspace(int64_t M, int64_t K, int is_bf16, int64_t xs_row) {
-  using namespace wanmi;
-  if (M <= 0 || K <= 0 || M <= (is_bf16 ? kFewQuantize : kFewRows) || (!is_bf16 && xs_row == 1)) return 0;
-  const int64_t codes = is_bf16 ? (M * K + 255) / 256 * 256 : 0;
-  return codes + M * blocks_of(K) * 4;
+namespace wanmi {
+
+// The workspace: codes and scales of bf16 rows, or scales alone laid out block by block; then the parts of the sum.
+struct Fp8Workspace {
+  int64_t scales_at, parts_at, bytes;
+  Fp8Plan plan;
+};
+
+static Fp8Workspace workspace_of(int64_t M, int64_t N, int64_t K, bool is_bf16, int64_t xs_row) {
+  Fp8Workspace w{0, 0, 0, {kFp8Tiles256, 1, 0}};
+  if (M <= 0 || N <= 0 || K <= 0 || M <= (is_bf16 ? kFewQuantize : kFewRows)) return w;
+  auto round_up = [](int64_t n) { return (n + 255) / 256 * 256; };
+  w.scales_at = is_bf16 ? round_up(M * K) : 0;
+  w.bytes = w.parts_at = w.scales_at + (is_bf16 || xs_row != 1 ? round_up(M * blocks_of(K) * 4) : 0);
+  if (M > kFewRows) {
+    w.plan = fp8_plan(M, N, blocks_of(K));
+    if (w.plan.splits > 1) w.bytes += w.plan.splits * M * N * 4;
+  }
+  return w;
+}
+
+}  // namespace wanmi
+
+extern "C" int64_t wanmi_fp8_block_workspace(int64_t M, int64_t N, int64_t K, int is_bf16, int64_t xs_row) {
+  return wanmi::workspace_of(M, N, K, is_bf16, xs_row).bytes;
 }
 
 extern "C" int wanmi_fp8_block_linear(const void* x, const float* x_scales, int64_t ldx, int64_t xs_row, int64_t xs_blk, const uint8_t* w,
@@ -553,17 +622,18 @@ extern "C" int wanmi_fp8_block_linear(const void* x, const float* x_scales, int6
   WANMI_REQUIRE(((uintptr_t)x | (uintptr_t)w | (uintptr_t)out | (uintptr_t)bias) % 16 == 0, WANMI_ERR_ARG, "%s: x, w, bias and out must be 16-byte aligned", what);
   WANMI_REQUIRE(ldx % align == 0 && (M == 1 || ldx >= K) && ldx < (1 << 23), WANMI_ERR_ARG, "%s: rows of x, %lld apart, must be 16-byte aligned", what, (long long)ldx);
   WANMI_REQUIRE(ldo % 8 == 0 && ldo >= N && ldo < (1 << 24), WANMI_ERR_ARG, "%s: the output's row stride %lld must be a multiple of 8 of at least N, below 2^24", what, (long long)ldo);
-  const int64_t need = wanmi_fp8_block_workspace(M, K, is_bf16, xs_row);
+  const Fp8Workspace ws = workspace_of(M, N, K, is_bf16, xs_row);
+  const int64_t need = ws.bytes;
   WANMI_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 16 == 0)), WANMI_ERR_ARG,
                 "%s: the workspace holds %lld bytes of %lld", what, (long long)workspace_bytes, (long long)need);
   WANMI_REQUIRE(((M + 63) / 64) * ((N + 63) / 64) < (1LL << 30) && M * ((KB + 3) / 4) < (1LL << 32), WANMI_ERR_ARG, "%s: too many tiles", what);
   hipStream_t st = (hipStream_t)stream;
-  Fp8Args g{(const uint8_t*)x, ldx, x_scales, xs_row, xs_blk, nullptr, w, w_scales, bias, (uint16_t*)out, ldo, (int)M, (int)N, (int)K, (int)KB, gelu, 0, 0};
+  Fp8Args g{(const uint8_t*)x, ldx, x_scales, xs_row, xs_blk, nullptr, w, w_scales, bias, (uint16_t*)out, ldo, (int)M, (int)N, (int)K, (int)KB, gelu, 0, 0, 1, nullptr};
   if (is_bf16 && M <= kFewQuantize) {
     g.x = (const uint16_t*)x;
   } else if (is_bf16) {
     uint8_t* codes = (uint8_t*)workspace;
-    float* scales = (float*)(codes + (M * K + 255) / 256 * 256);
+    float* scales = (float*)(codes + ws.scales_at);
     launch_quantize((const uint16_t*)x, ldx, (int)M, (int)K, codes, scales, 1, M, st);
     g.a = codes, g.lda = K, g.a_scales = scales, g.as_row = 1, g.as_blk = M;
   } else if (M > kFewRows && xs_row != 1) {
@@ -577,10 +647,14 @@ extern "C" int wanmi_fp8_block_linear(const void* x, const float* x_scales, int6
     else hipLaunchKernelGGL((fp8_block_few_kernel<false>), grid, block, 0, st, g);
   } else {
     const int cus = device_cu_count();
-    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256), mid = ((M + 127) / 128) * ((N + 127) / 128);
-    if (big >= cus) launch_tiles<256, 256, 2, 4, 2>(g, cus, st);
-    else if (mid >= cus) launch_tiles<128, 128, 2, 2, 2>(g, 2 * cus, st);
-    else launch_tiles<64, 64, 2, 2, 4>(g, INT64_MAX, st);  // a tile each: with more than two stages nothing is loaded for a next one
+    g.splits = ws.plan.splits;
+    g.parts = (float*)((uint8_t*)workspace + ws.parts_at);
+    switch (ws.plan.tiles) {
+      case kFp8Tiles64: launch_tiles<64, 64, 2, 2, 4>(g, 0, st); break;
+      case kFp8Tiles128Deep: launch_tiles<128, 128, 2, 4, 4>(g, 0, st); break;
+      case kFp8Tiles128: launch_tiles<128, 128, 2, 4, 2>(g, 2 * cus, st); break;
+      case kFp8Tiles256: launch_tiles<256, 256, 2, 4, 2>(g, cus, st); break;
+    }
   }
   return check_launch(what);
 }

@@ -125,6 +125,52 @@ def fp8_block_linear(x, weight: FP8BlockWeight, *, activation: str | None = None
     quantized inside the one launch."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}")
+    y = _linear_plain(x, weight, _ACTIVATIONS[activation]) if out is None else None
+    return _linear_checked(x, weight, _ACTIVATIONS[activation], out) if y is None else y
+
+
+def _launch(dev: int, px, ps, ld: int, s_row: int, s_blk: int, pw, psw, pb, M: int, N: int, K: int, gelu: int, y: torch.Tensor, ldo: int) -> None:
+    size = _lib.load().wanmi_fp8_block_workspace(M, N, K, int(ps is None), s_row)
+    work = torch.empty(size, dtype=torch.uint8, device=y.device) if size else None
+    _lib.call("wanmi_fp8_block_linear", dev, px, ps, ld, s_row, s_blk, pw, psw, pb, M, N, K, gelu, y.data_ptr(), ldo, _lib.ptr(work), size)
+
+
+def _linear_plain(x, weight, gelu: int):
+    """:func:`fp8_block_linear` for arguments of ordinary form (two dimensions, contiguous rows); None if any is not."""
+    try:
+        if type(weight) is not FP8BlockWeight:
+            return None
+        wc, wsc, wb = weight
+        N, K = wc.shape
+        dev = wc.get_device()
+        kb = (K + 127) >> 7
+        if N < 8 or N & 7 or K < 16 or K & 15 or dev < 0:
+            return None
+        ps, s_row, s_blk = None, 0, 0
+        if type(x) is FP8BlockTensor:
+            codes, scales = x
+            M = codes.shape[0]
+            px = _lib.plain_ptr(codes, torch.float8_e4m3fn, (M, K), dev)
+            if scales.dtype is not torch.float32 or scales.shape != (M, kb) or scales.get_device() != dev:
+                return None
+            s_row, s_blk = scales.stride()
+            ps = scales.data_ptr()
+        else:
+            M = x.shape[0]
+            px = _lib.plain_ptr(x, torch.bfloat16, (M, K), dev)
+        pw = _lib.plain_ptr(wc, torch.float8_e4m3fn, (N, K), dev)
+        psw = _lib.plain_ptr(wsc, torch.float32, ((N + 127) >> 7, kb), dev)
+        pb = _lib.plain_ptr(wb, torch.float32, (N,), dev)
+    except (AttributeError, IndexError, TypeError, ValueError):
+        return None
+    if M < 1 or None in (px, pw, psw) or -1 in (px, pw, psw, pb):
+        return None
+    y = torch.empty((M, N), dtype=torch.bfloat16, device=wc.device)
+    _launch(dev, px, ps, K, s_row if M > 1 else 1, s_blk, pw, psw, pb, M, N, K, gelu, y, N)
+    return y
+
+
+def _linear_checked(x, weight, gelu: int, out):
     _check_weight(weight)
     N, K = weight.codes.shape
     scales = None
@@ -157,8 +203,6 @@ def fp8_block_linear(x, weight: FP8BlockWeight, *, activation: str | None = None
     y = torch.empty((M, N), dtype=torch.bfloat16, device=dev) if out is None else out
     if M:
         p = _lib.ptr
-        size = _lib.load().wanmi_fp8_block_workspace(M, K, int(scales is None), s_row)
-        work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        _lib.call("wanmi_fp8_block_linear", codes.get_device(), p(codes), p(scales), ld, s_row, s_blk, p(weight.codes), p(weight.scales), p(weight.bias),
-                  M, N, K, _ACTIVATIONS[activation], p(y), y.stride(0) if M > 1 else N, p(work), size)
+        _launch(codes.get_device(), p(codes), p(scales), ld, s_row, s_blk, p(weight.codes), p(weight.scales), p(weight.bias), M, N, K, gelu, y,
+                y.stride(0) if M > 1 else N)
     return y if len(lead) == 1 else y.reshape(*lead, N)

@@ -89,6 +89,30 @@ def _check(q, k, v, scale, out, quant, what: str) -> float:
     return scale
 
 
+def _plain(q, k, v, scale):
+    """The shapes, strides and pointers of ordinary arguments (several rows and heads, on one GPU, aligned) in one look, or None:
+    :func:`_check` says what is wrong with them or takes them as they are."""
+    try:
+        (T, heads, D), (Tk, k_heads, Dk), vs = q.shape, k.shape, v.shape
+        dev = q.get_device()
+        strides, pointers = [], []
+        for t in (q, k, v):
+            ss, hs, es = t.stride()
+            p = t.data_ptr()
+            if t.dtype is not torch.bfloat16 or t.get_device() != dev or es != 1 or ss & 7 or hs & 7 or p & 15 or ss < D or hs < D:
+                return None
+            strides.append((ss, hs))
+            pointers.append(p)
+        scale = D**-0.5 if scale is None else scale
+        if D != Dk or vs != k.shape or dev < 0 or D not in (64, 128) or T < 2 or Tk < 2 or k_heads < 1 or heads % k_heads or type(scale) is not float:
+            return None
+        if heads < 2 or k_heads < 2 or not 0.0 < scale < math.inf:
+            return None
+    except (AttributeError, RuntimeError, TypeError, ValueError):
+        return None
+    return dev, T, heads, D, Tk, k_heads, strides, pointers, scale
+
+
 def _offsets(t, what: str, n: int | None = None) -> int:
     _lib.expect(t, what, dtype=torch.int32, shape=(n,))
     if t.shape[0] < 1:
@@ -112,6 +136,17 @@ def packed_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_
     rows, and no access out of bounds. The softmax has a running maximum (no bound on scores is needed) and fp32 sums; its weights enter the
     second product as bf16.
     """
+    if out is None and quant == "none":
+        plain = _plain(q, k, v, scale)
+        if plain is not None:
+            dev, T, heads, head_dim, Tk, k_heads, strides, pointers, s = plain
+            n = q_offsets.shape if isinstance(q_offsets, torch.Tensor) else ()
+            pq, pk = (_lib.plain_ptr(t, torch.int32, n, dev) if isinstance(t, torch.Tensor) else None for t in (q_offsets, k_offsets))
+            if len(n) == 1 and n[0] and pq not in (None, -1) and pk not in (None, -1):
+                out = torch.empty((T, heads, head_dim), dtype=torch.bfloat16, device=q.device)
+                _lib.call("wanmi_packed_cross_attention", dev, pointers[0], *strides[0], pointers[1], *strides[1], pointers[2], *strides[2], pq, pk,
+                          n[0] - 1, T, Tk, heads, k_heads, head_dim, s, out.data_ptr(), heads * head_dim, None, 1)
+                return out
     scale = _check(q, k, v, scale, out, quant, "packed_cross_attention")
     requests = _offsets(q_offsets, "q_offsets")
     _offsets(k_offsets, "k_offsets", requests + 1)
@@ -153,6 +188,21 @@ def relative_bias_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, t
     Returns bf16 ``[T, heads, D]``. Rows behind the last prompt are zeros in an output allocated here and left as they are in a
     given ``out``, which may be ``q``. Inference only: no gradient.
     """
+    if out is None:
+        plain = _plain(q, k, v, scale)
+        if plain is not None:
+            dev, T, heads, head_dim, Tk, k_heads, strides, pointers, s = plain
+            if Tk == T and k_heads == heads and isinstance(table, torch.Tensor) and isinstance(offsets, torch.Tensor) and table.dim() == 2:
+                n = offsets.shape
+                po = _lib.plain_ptr(offsets, torch.int32, n, dev)
+                pt = _lib.plain_ptr(table, table.dtype, (table.shape[0], heads), dev)
+                if len(n) == 1 and n[0] and po != -1 and pt != -1 and table.dtype in (torch.float32, torch.bfloat16):
+                    starts = _bucket_starts(table.shape[0], int(max_distance), bool(bidirectional))
+                    out = torch.empty((T, heads, head_dim), dtype=torch.bfloat16, device=q.device)
+                    _lib.call("wanmi_relative_bias_attention", dev, pointers[0], *strides[0], pointers[1], *strides[1], pointers[2], *strides[2], po,
+                              n[0] - 1, T, heads, head_dim, s, pt, int(table.dtype is torch.bfloat16), starts, len(starts), int(bool(bidirectional)),
+                              out.data_ptr(), heads * head_dim, 1)
+                    return out
     scale = _check(q, k, v, scale, out, "none", "relative_bias_attention")
     T, heads, head_dim = q.shape
     if k.shape[1] != heads or k.shape[0] != T:

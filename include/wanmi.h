@@ -435,7 +435,7 @@ int64_t wanmi_lora_workspace(int64_t T, int64_t K, int parts, int rank);
  * q_offsets, k_offsets: int32 [requests + 1] on the device, ascending from 0, held inside [0, T] and [0, Tk] (below 2^28).
  * out: bf16 [T, heads * head_dim], rows o_ss elements apart (a multiple of 16), may be q element for element; with out_scales (uint8
  * [T, heads * head_dim / 32]) e4m3fn codes and e8m0 scales as wanmi_mxfp8_gemm reads them. Rows behind the last request
- * are left, or zeroed with zero_rest. scale positive. Sums and the softmax in fp32, p enters the second product as bf16.
+ * are left, or zeroed with zero_rest. scale from 2^-64 to 2^24. Sums and the softmax in fp32, p enters the second product as bf16.
  * Stands beside wanmi_attention_const_max (one sequence, a bound in place of the maximum); no reference counterpart.
  */
 int wanmi_packed_cross_attention(const void* q, int64_t q_ss, int64_t q_hs, const void* k, int64_t k_ss, int64_t k_hs,

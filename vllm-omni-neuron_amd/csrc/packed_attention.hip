@@ -20,13 +20,14 @@
 #include "wanmi_common.h"
 
 #include <algorithm>
-#include <cmath>
 
 namespace wanmi {
 
 constexpr int kMaxSide = 128;         // bias buckets of one direction
 constexpr int kMaxSaturation = 1024;  // the distance from which on a direction's last bucket holds
 constexpr float kSlack = 8.0f;        // log2 units
+constexpr float kBiasMax = 1e30f;     // of a finite bias, in units of the scores before their scale: beyond, scores vanish beside it
+constexpr float kBiasFold = 8192.0f;  // up to here a bias that a whole half shares is taken off its maximum instead
 
 struct PackedAttnArgs {
   const uint16_t* q;  // row i, head h at q + i * q_ss + h * q_hs
@@ -39,6 +40,8 @@ struct PackedAttnArgs {
   int T, Tk;
   int heads, group;   // query heads, and how many of them share a key head
   float scale_log2;   // s log2(e)
+  float slack;        // kSlack / scale_log2
+  float inv_scale;    // 1 / s
   void* out;          // bf16 [T, heads * D], or e4m3 codes
   int64_t o_ss;
   uint8_t* out_scales;  // MX: [T, heads * D / 32]
@@ -80,8 +83,10 @@ __device__ __forceinline__ bool find_tile(const PackedAttnArgs& a, int t, int& r
   int before = 0;
   for (int c = 0; c <= a.requests; c += 64) {
     const int r = min(c + lane, a.requests);
-    const int lo = min(max(a.q_off[r], 0), a.T);
-    int hi = r < a.requests ? min(max(a.q_off[r + 1], 0), a.T) : a.zero_rest ? a.T : lo;
+    const int next = min(r + 1, a.requests);
+    const int q_lo = a.q_off[r], q_hi = a.q_off[next], k_lo = a.k_off[r], k_hi = a.k_off[next];  // (all four under way together)
+    const int lo = min(max(q_lo, 0), a.T);
+    int hi = r < a.requests ? min(max(q_hi, 0), a.T) : a.zero_rest ? a.T : lo;
     if (c + lane > a.requests) hi = lo;
     int sum = max(hi - lo + kRows - 1, 0) / kRows;
 #pragma unroll
@@ -99,14 +104,10 @@ __device__ __forceinline__ bool find_tile(const PackedAttnArgs& a, int t, int& r
       if (in_request < 0 || in_request >= end - at) return false;
       row0 = at + in_request;
       rows = min(kRows, end - row0);
-      const int q = c + l;
-      k0 = keys = 0;
-      if (q < a.requests) {
-        k0 = min(max(a.k_off[q], 0), a.Tk);
-        keys = max(min(max(a.k_off[q + 1], 0), a.Tk) - k0, 0);
-      }
-      k0 = __builtin_amdgcn_readfirstlane(k0);
-      keys = __builtin_amdgcn_readfirstlane(keys);
+      // (the rows behind the last request: k_lo and k_hi are the same)
+      const int kl = min(max(k_lo, 0), a.Tk), kn = max(min(max(k_hi, 0), a.Tk) - kl, 0);
+      k0 = __builtin_amdgcn_readfirstlane(__shfl(kl, l, 64));
+      keys = __builtin_amdgcn_readfirstlane(__shfl(kn, l, 64));
       return true;
     }
     before = __builtin_amdgcn_readfirstlane(__shfl(sum, 63, 64));
@@ -132,15 +133,16 @@ __device__ __forceinline__ int mx_codes(const uint32_t (&pp)[8], uint32_t (&code
 template <int D, bool kBias, int kSplit, bool kMx>
 __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs a, BiasArgs bias) {
   constexpr int kRows = 128 / kSplit;              // rows of a workgroup
-  constexpr int kHalves = kSplit == 1 ? 2 : 1;     // 32-key halves of a wave's part of a tile
-  constexpr int kKeys = kSplit == 1 ? 64 : 128;    // keys of a tile
+  constexpr int kHalves = kSplit == 1 ? 2 : 1;     // 32-key halves of a tile: the workgroup's of 64 keys, or a wave's own of 32
+  constexpr int kKeys = 32 * kHalves;
   constexpr int kRowB = 2 * D;                     // bytes
   constexpr int kChunks = D / 8;
   constexpr int kTile = kKeys * kRowB;             // of K, and as much of V
-  constexpr int kLoads = kTile / 4096;             // per wave, of each
+  constexpr int kLoads = kTile / (kSplit == 1 ? 4096 : 1024);  // per wave, of each
   constexpr int kRing = 2;
+  constexpr int kRingB = kRing * 2 * kTile * (kSplit == 1 ? 1 : 4);
   constexpr int kJoin = kSplit == 1 ? 0 : kSplit * 32 * (D * 4 + 8);
-  constexpr int kLds = kRing * 2 * kTile > kJoin ? kRing * 2 * kTile : kJoin;
+  constexpr int kLds = kRingB > kJoin ? kRingB : kJoin;
   constexpr int kBiasLds = kBias ? 2 * (kMaxSaturation + 63) + 2 : 1;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
   __shared__ float sbias[kBiasLds];
@@ -152,30 +154,25 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
   const int work = (int)(blockIdx.x & 7) * a.per_xcd + in_xcd;
   if (in_xcd >= a.per_xcd || work >= a.tiles * a.heads) return;
   const int head = work / a.tiles;
+
+  // ---- the head's bias over the distances -(sat + 63) .. sat + 63, over the scale: added to the scores before it. Its loads run beside
+  // those of the offsets ----
+  [[maybe_unused]] int sat = 0;
+  if constexpr (kBias) {
+    sat = bias.start[bias.side - 1];
+    for (int i = threadIdx.x; i < 2 * (sat + 63) + 1; i += 256) {
+      const int d = i - (sat + 63), n = abs(d);
+      int b = 0;
+      for (int j = 1; j < bias.side; ++j) b += n >= bias.start[j];
+      if (d > 0) b = bias.both ? b + bias.side : 0;
+      const int at = b * a.heads + head;
+      const float x = bias.bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t*>(bias.table)[at]) : reinterpret_cast<const float*>(bias.table)[at];
+      // (the lowest value of a type, as a mask has it, stays finite: a row of nothing else weighs all alike)
+      sbias[i] = fabsf(x) < INFINITY ? fminf(fmaxf(x * a.inv_scale, -kBiasMax), kBiasMax) : x;
+    }
+  }
   int row0, rows, in_request, k0, keys;
   if (!find_tile<kRows>(a, work - head * a.tiles, row0, rows, in_request, k0, keys)) return;
-
-  // ---- loads of a tile of keys: four rows (D = 64: eight) to an instruction ----
-  const int khead = head / a.group;
-  const uint16_t* kb = a.k + (int64_t)k0 * a.k_ss + (int64_t)khead * a.k_hs;
-  const uint16_t* vb = a.v + (int64_t)k0 * a.v_ss + (int64_t)khead * a.v_hs;
-  const int lrow = lane / kChunks, lslot = lane % kChunks;
-  constexpr int kPer = 64 / kChunks;  // rows of an instruction
-  const int tiles = (keys + kKeys - 1) / kKeys;
-  auto load_tile = [&](int t) {
-    const int left = min(keys - t * kKeys, kKeys);  // > 0
-    const u32x4 rk = buffer_rsrc(kb + (int64_t)t * kKeys * a.k_ss, (uint32_t)(((left - 1) * a.k_ss + D) * 2));
-    const u32x4 rv = buffer_rsrc(vb + (int64_t)t * kKeys * a.v_ss, (uint32_t)(((left - 1) * a.v_ss + D) * 2));
-    const uint32_t to = lds_addr(lds) + (uint32_t)((t % kRing) * 2 * kTile);
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int r = (wave * kLoads + j) * kPer;  // the instruction's first row; keys past the text read as zeros
-      const int key = r + lrow;
-      lds_dma_b128(rk, (uint32_t)key * (uint32_t)(a.k_ss * 2) + (uint32_t)((lslot ^ k_slot<D>(key)) << 4), to + r * kRowB);
-      lds_dma_b128(rv, (uint32_t)key * (uint32_t)(a.v_ss * 2) + (uint32_t)((lslot ^ v_slot<D>(key)) << 4), to + kTile + r * kRowB);
-    }
-  };
-  if (tiles > 0) load_tile(0);
 
   // ---- the wave's 32 queries as MFMA operands: lane holds d = 16 t + 8 hq .. + 7 of query col ----
   const int qw = kSplit == 1 ? wave * 32 : 0;  // the wave's first row in the tile
@@ -187,20 +184,34 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
     for (int t = 0; t < D / 16; ++t) qf[t] = *reinterpret_cast<const bf16x8*>(pq + 16 * t);
   }
 
-  // ---- the head's bias over the distances -(sat + 63) .. sat + 63, in log2 units ----
-  [[maybe_unused]] int sat = 0;
+  // ---- loads of a tile of keys: four rows (D = 64: eight) to an instruction; kSplit 4: the wave's own keys into its own LDS ----
+  const int khead = head / a.group;
+  const uint16_t* kb = a.k + (int64_t)k0 * a.k_ss + (int64_t)khead * a.k_hs;
+  const uint16_t* vb = a.v + (int64_t)k0 * a.v_ss + (int64_t)khead * a.v_hs;
+  const int lrow = lane / kChunks, lslot = lane % kChunks;
+  constexpr int kPer = 64 / kChunks;  // rows of an instruction
+  uint8_t* ring = lds + (kSplit == 1 ? 0 : wave * (kRing * 2 * kTile));
+  // the tile's number along the keys, and how many there are for this wave
+  auto tile_at = [&](int t) { return kSplit == 1 ? t : t * kSplit + wave; };
+  const int all = (keys + kKeys - 1) / kKeys;
+  const int tiles = kSplit == 1 ? all : (all - wave + kSplit - 1) / kSplit;
+  auto load_tile = [&](int t) {
+    const int first = tile_at(t) * kKeys, left = min(keys - first, kKeys);  // > 0
+    const u32x4 rk = buffer_rsrc(kb + (int64_t)first * a.k_ss, (uint32_t)(((left - 1) * a.k_ss + D) * 2));
+    const u32x4 rv = buffer_rsrc(vb + (int64_t)first * a.v_ss, (uint32_t)(((left - 1) * a.v_ss + D) * 2));
+    const uint32_t to = lds_addr(ring) + (uint32_t)((t % kRing) * 2 * kTile);
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int r = ((kSplit == 1 ? wave * kLoads : 0) + j) * kPer;  // the instruction's first row; keys past the text read as zeros
+      const int key = r + lrow;
+      lds_dma_b128(rk, (uint32_t)key * (uint32_t)(a.k_ss * 2) + (uint32_t)((lslot ^ k_slot<D>(key)) << 4), to + r * kRowB);
+      lds_dma_b128(rv, (uint32_t)key * (uint32_t)(a.v_ss * 2) + (uint32_t)((lslot ^ v_slot<D>(key)) << 4), to + kTile + r * kRowB);
+    }
+  };
+  if (tiles > 0) load_tile(0);
+  if (kSplit > 1 && tiles > 1) load_tile(1);
   [[maybe_unused]] float far_lo = 0.0f, far_hi = 0.0f;
   if constexpr (kBias) {
-    sat = bias.start[bias.side - 1];
-    for (int i = threadIdx.x; i < 2 * (sat + 63) + 1; i += 256) {
-      const int d = i - (sat + 63), n = abs(d);
-      int b = 0;
-      for (int j = 1; j < bias.side; ++j) b += n >= bias.start[j];
-      if (d > 0) b = bias.both ? b + bias.side : 0;
-      const int at = b * a.heads + head;
-      const float x = bias.bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t*>(bias.table)[at]) : reinterpret_cast<const float*>(bias.table)[at];
-      sbias[i] = x * 1.4426950408889634f;
-    }
     __syncthreads();
     far_lo = sbias[0];
     far_hi = sbias[2 * (sat + 63)];
@@ -211,24 +222,28 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
-  float m = -INFINITY, sum = 0.0f;
+  float m = -INFINITY, sum = 0.0f;  // m in units of the scores before their scale
   const float c = a.scale_log2;
   const bf16x2_t ones = {(__bf16)1.0f, (__bf16)1.0f};
 
   for (int t = 0; t < tiles; ++t) {
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-    __syncthreads();  // the tile is in LDS, and every wave is done with the one before it
-    if (t + 1 < tiles) load_tile(t + 1);
-    const uint8_t* tk = lds + (t % kRing) * 2 * kTile;
+    if constexpr (kSplit == 1) {
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+      __syncthreads();  // the tile is in LDS, and every wave is done with the one before it
+      if (t + 1 < tiles) load_tile(t + 1);
+    } else if (t + 1 < tiles) {
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm(2 * kLoads));  // the next tile's may be under way
+    } else {
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    }
+    const uint8_t* tk = ring + (t % kRing) * 2 * kTile;
     const uint8_t* tv = tk + kTile;
-    const int half0 = kSplit == 1 ? 0 : wave;  // the wave's first half
-    const int left = keys - t * kKeys - 32 * half0;  // keys from there on
-    if (kSplit > 1 && left <= 0) continue;
+    const int left = keys - tile_at(t) * kKeys;
 
     f32x16 s[kHalves];
 #pragma unroll
     for (int i = 0; i < kHalves; ++i) {
-      const int key = 32 * (half0 + i) + col;
+      const int key = 32 * i + col;
       const uint8_t* row = tk + key * kRowB;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[i][r] = 0.0f;
@@ -239,38 +254,47 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
       }
     }
     // register r of half i: key 32 i + 8 (r >> 2) + 4 hq + (r & 3)
+    float shared[kHalves];  // a bias of the whole half
 #pragma unroll
     for (int i = 0; i < kHalves; ++i) {
+      shared[i] = 0.0f;
       if constexpr (kBias) {
-        const int d0 = t * kKeys + 32 * (half0 + i) - (in_request + qw);  // first key - first query
-        if (d0 - 31 >= sat || d0 + 31 <= -sat) {
-          const float b = d0 > 0 ? far_hi : far_lo;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[i][r] = fmaf(s[i][r], c, b);
-        } else {
+        const int d0 = tile_at(t) * kKeys + 32 * i - (in_request + qw);  // first key - first query
+        const float far = d0 > 0 ? far_hi : far_lo;
+        if (d0 - 31 < sat && d0 + 31 > -sat) {
+          asm volatile("");  // (a branch: not both sides computed and one selected)
           const float* pb = sbias + (sat + 63 + d0 + 4 * hq - col);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[i][r] = fmaf(s[i][r], c, pb[8 * (r >> 2) + (r & 3)]);
+          for (int r = 0; r < 16; ++r) s[i][r] += pb[8 * (r >> 2) + (r & 3)];
+        } else if (fabsf(far) > kBiasFold) {
+          asm volatile("");
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[i][r] += far;
+        } else {
+          shared[i] = far;
         }
       }
     }
     if (left < 32 * kHalves) {
+      asm volatile("");
 #pragma unroll
       for (int i = 0; i < kHalves; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (32 * i + 8 * (r >> 2) + 4 * hq + (r & 3) >= left) s[i][r] = -INFINITY;
     }
-    float mx = s[0][0];
+    float mx = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kHalves; ++i)
+    for (int i = 0; i < kHalves; ++i) {
+      float h = s[i][0];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[i][r]);
+      for (int r = 1; r < 16; ++r) h = fmaxf(h, s[i][r]);
+      mx = fmaxf(mx, kBias ? h + shared[i] : h);
+    }
     mx = max_lane_xor32(mx);
-    if constexpr (!kBias) mx *= c;
-    if (__any(mx > m + kSlack)) {
+    if (__any(mx > m + a.slack)) {
       const float mn = fmaxf(m, mx);
-      const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
       m = mn;
       sum *= f;
 #pragma unroll
@@ -278,18 +302,18 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] *= f;
     }
-    const float off = m == -INFINITY ? 0.0f : m;  // no key above -inf yet: every P is 0
+    const float base = m == -INFINITY ? 0.0f : m;  // no key above -inf yet: every P is 0
 #pragma unroll
     for (int i = 0; i < kHalves; ++i) {
+      const float off = kBias ? (shared[i] - base) * c : -base * c;
       bf16x8 pf[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         uint32_t w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float s0 = s[i][8 * u + 2 * j], s1 = s[i][8 * u + 2 * j + 1];
-          const float p0 = __builtin_amdgcn_exp2f(kBias ? s0 - off : fmaf(s0, c, -off));
-          const float p1 = __builtin_amdgcn_exp2f(kBias ? s1 - off : fmaf(s1, c, -off));
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i][8 * u + 2 * j], c, off));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(s[i][8 * u + 2 * j + 1], c, off));
           w[j] = pack_bf16x2(p0, p1);
           sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w[j]), ones, sum, false);  // the P that multiplies V
         }
@@ -297,8 +321,8 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        // lane's keys: 16 u + 4 hq .. + 3 and 8 further, of d = 32 i + col; it reads four d of key + (lane & 15) / 4
-        const int key = 32 * (half0 + i) + 16 * u + 4 * hq + ((lane & 15) >> 2);
+        // lane's keys: 16 u + 4 hq .. + 3 and 8 further, of d = 32 dt + col; it reads four d of key + (lane & 15) / 4
+        const int key = 32 * i + 16 * u + 4 * hq + ((lane & 15) >> 2);
         const int ch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
         const uint8_t* p0 = tv + key * kRowB + 8 * (lane & 1);
 #pragma unroll
@@ -311,6 +335,10 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
           acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[u], acc[dt], 0, 0, 0);
         }
       }
+    }
+    if (kSplit > 1 && t + 2 < tiles) {
+      __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0));  // the wave has read its tile
+      load_tile(t + 2);
     }
   }
   sum = add_lane_xor32(sum);
@@ -383,7 +411,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
     for (int w = 0; w < kSplit; ++w) mm = fmaxf(mm, mw[w] = stats[w * 64 + col]);
 #pragma unroll
     for (int w = 0; w < kSplit; ++w) {
-      mw[w] = mw[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw[w] - mm);
+      mw[w] = mw[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mw[w] - mm) * c);
       const float part = stats[w * 64 + 32 + col];
       total += part == 0.0f ? 0.0f : mw[w] * part;
     }
@@ -452,7 +480,7 @@ static int check_args(const PackedAttnArgs& a, int64_t T, int64_t Tk, int64_t re
   WANMI_REQUIRE(T >= 0 && T < (1LL << 28) && Tk >= 0 && Tk < (1LL << 28), WANMI_ERR_ARG, "%s: %lld rows, %lld keys: at most 2^28 - 1", what, (long long)T, (long long)Tk);
   WANMI_REQUIRE(requests >= 0 && requests < (1 << 20), WANMI_ERR_ARG, "%s: %lld requests: at most 2^20 - 1", what, (long long)requests);
   WANMI_REQUIRE(heads > 0 && k_heads > 0 && heads % k_heads == 0 && heads <= 1024, WANMI_ERR_ARG, "%s: %lld heads (at most 1024) over %lld key heads", what, (long long)heads, (long long)k_heads);
-  WANMI_REQUIRE(std::isfinite(a.scale_log2) && a.scale_log2 > 0.0f, WANMI_ERR_ARG, "%s: the scale must be positive and finite", what);
+  WANMI_REQUIRE(a.inv_scale >= 0x1p-24f && a.inv_scale <= 0x1p64f, WANMI_ERR_ARG, "%s: the scale must be in 2^-64 .. 2^24", what);
   const int64_t strides[6] = {a.q_ss, a.q_hs, a.k_ss, a.k_hs, a.v_ss, a.v_hs};
   for (int64_t s : strides)
     WANMI_REQUIRE(s >= 0 && s % 8 == 0 && s < (1 << 22), WANMI_ERR_ARG, "%s: stride %lld must be a multiple of 8 below 2^22", what, (long long)s);
@@ -474,7 +502,7 @@ extern "C" int wanmi_packed_cross_attention(const void* q, int64_t q_ss, int64_t
   using namespace wanmi;
   clear_error();
   PackedAttnArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, q_ss, q_hs, k_ss, k_hs, v_ss, v_hs, q_offsets, k_offsets, (int)requests,
-                   (int)T, (int)Tk, (int)heads, (int)(k_heads > 0 ? heads / k_heads : 1), scale * 1.4426950408889634f, out, o_ss, out_scales, zero_rest, 0, 0};
+                   (int)T, (int)Tk, (int)heads, (int)(k_heads > 0 ? heads / k_heads : 1), scale * 1.4426950408889634f, kSlack / (scale * 1.4426950408889634f), 1.0f / scale, out, o_ss, out_scales, zero_rest, 0, 0};
   const int st = check_args(a, T, Tk, requests, heads, k_heads, head_dim, "wanmi_packed_cross_attention");
   if (st != WANMI_OK || T == 0) return st;
   return dispatch<false>(a, BiasArgs{}, head_dim, (hipStream_t)stream, "wanmi_packed_cross_attention");
@@ -488,7 +516,7 @@ extern "C" int wanmi_relative_bias_attention(const void* q, int64_t q_ss, int64_
   clear_error();
   const char* what = "wanmi_relative_bias_attention";
   PackedAttnArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, q_ss, q_hs, k_ss, k_hs, v_ss, v_hs, offsets, offsets, (int)requests,
-                   (int)T, (int)T, (int)heads, 1, scale * 1.4426950408889634f, out, o_ss, nullptr, zero_rest, 0, 0};
+                   (int)T, (int)T, (int)heads, 1, scale * 1.4426950408889634f, kSlack / (scale * 1.4426950408889634f), 1.0f / scale, out, o_ss, nullptr, zero_rest, 0, 0};
   const int st = check_args(a, T, T, requests, heads, heads, head_dim, what);
   if (st != WANMI_OK) return st;
   WANMI_REQUIRE(side >= 1 && side <= kMaxSide && starts, WANMI_ERR_ARG, "%s: %d buckets of one direction, at most %d", what, side, kMaxSide);

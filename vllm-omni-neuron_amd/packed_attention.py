@@ -11,7 +11,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import math
 
 import torch
 
@@ -19,6 +18,7 @@ from . import _lib
 from .common_types import MXTensor
 
 _MAX_SIDE, _MAX_SATURATION = 128, 1024
+_MIN_SCALE, _MAX_SCALE = 2.0**-64, 2.0**24
 
 
 @functools.lru_cache(maxsize=64)
@@ -66,8 +66,8 @@ def _check(q, k, v, scale, out, quant, what: str) -> float:
     if heads < 1 or k.shape[1] < 1 or heads % k.shape[1]:
         raise ValueError(f"{heads} query heads over {k.shape[1]} key heads")
     scale = head_dim**-0.5 if scale is None else float(scale)
-    if not (0.0 < scale < math.inf):
-        raise ValueError(f"scale {scale} must be positive and finite")
+    if not _MIN_SCALE <= scale <= _MAX_SCALE:
+        raise ValueError(f"scale {scale} must be between 2^-64 and 2^24")
     for name, t in (("q", q), ("k", k), ("v", v)):
         ss, hs = _strides(t)
         if ss % 8 or hs % 8 or t.data_ptr() % 16:
@@ -106,7 +106,7 @@ def _plain(q, k, v, scale):
         scale = D**-0.5 if scale is None else scale
         if D != Dk or vs != k.shape or dev < 0 or D not in (64, 128) or T < 2 or Tk < 2 or k_heads < 1 or heads % k_heads or type(scale) is not float:
             return None
-        if heads < 2 or k_heads < 2 or not 0.0 < scale < math.inf:
+        if heads < 2 or k_heads < 2 or not _MIN_SCALE <= scale <= _MAX_SCALE:
             return None
     except (AttributeError, RuntimeError, TypeError, ValueError):
         return None

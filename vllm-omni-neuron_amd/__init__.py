@@ -47,5 +47,11 @@ from . import block  # noqa: F401
 from . import comfy_fp8_checkpoint  # noqa: F401
 from . import kernels  # noqa: F401
 from . import packed_block  # noqa: F401
-from .packed_block import PackedRequests, packed_block_forward, packed_dit_forward  # noqa: F401
+from .packed_block import (  # noqa: F401
+    PackedCrossKV,
+    PackedRequests,
+    packed_block_forward,
+    packed_dit_forward,
+    project_packed_cross_kv,
+)
 from . import row_block  # noqa: F401

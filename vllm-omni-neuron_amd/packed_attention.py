@@ -128,7 +128,7 @@ def packed_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_
     head h reads key head ``h // (heads // k_heads)``); rows and heads may be strided (column blocks of a fused
     projection). ``q_offsets`` and ``k_offsets`` int32 ``[R + 1]`` on the GPU, ascending from 0: request r has the rows
     ``q_offsets[r]`` to ``q_offsets[r + 1]`` and the keys ``k_offsets[r]`` to ``k_offsets[r + 1]``
-    (:meth:`.PackedRequests.offsets`). ``scale``: ``D ** -0.5`` if None.
+    (:attr:`.PackedRequests.offsets`). ``scale``: ``D ** -0.5`` if None.
 
     Returns bf16 ``[T, heads, D]``, or with ``quant="mx"`` an :class:`MXTensor` ``[T, heads * D]`` as the MX projections read it.
     The rows of a request without keys are zeros. Rows behind the last request are zeros too in an output allocated here and

@@ -83,3 +83,175 @@ def test_relative_bias(pkg, dev, case):
     q, k, v = (qkv[: sum(lens), i * heads : (i + 1) * heads] for i in range(3))
     _check(got[: sum(lens)], q, k, v, lens, lens, 1.0, lambda n: ref.bias_matrix(table, n, far, both), float(table.abs().max()))
     assert not got[sum(lens):].any()
+
+
+@pytest.mark.parametrize("q_lens,k_lens,pad,D", [([3, 1, 9], [40, 0, 7], 4, 128), ([3, 1, 9], [40, 0, 7], 4, 64), ([200, 90], [130, 65], 7, 128), ([200, 90], [130, 65], 7, 64)])
+def test_codes_are_those_of_the_bf16_output(pkg, dev, q_lens, k_lens, pad, D):
+    q, k, v = (t.to(dev) for t in _inputs(sum(q_lens) + pad, sum(k_lens), 4, 2, D, 7))
+    qo, ko = ref.offsets(q_lens, dev), ref.offsets(k_lens, dev)
+    out = pkg.packed_cross_attention(q, k, v, qo, ko)
+    got = pkg.packed_cross_attention(q, k, v, qo, ko, quant="mx")
+    want = pkg.adaln_kernels.adaln_quant_2d(out.view(out.shape[0], -1), None, None, eps=0.0, norm_type="none", quant="mx")
+    assert torch.equal(got.codes.view(torch.uint8), want.codes.view(torch.uint8)) and torch.equal(got.scales, want.scales)
+
+
+@pytest.mark.parametrize("T", [5, 300])
+def test_given_outputs_and_layouts(pkg, dev, T):
+    """A given output keeps the rows behind the last request and may be q; heads and rows of the inputs in any order."""
+    lens, k_lens, H, D = [T - 4, 1], [70, 33], 4, 64
+    q, k, v = (t.to(dev) for t in _inputs(T, 103, H, H, D, T))
+    qo, ko = ref.offsets(lens, dev), ref.offsets(k_lens, dev)
+    want = pkg.packed_cross_attention(q, k, v, qo, ko)
+    out = torch.full((T, 2 * H, D), 7.0, dtype=BF16, device=dev)
+    got = pkg.packed_cross_attention(q, k, v, qo, ko, out=out[:, H:])
+    assert got.data_ptr() == out[:, H:].data_ptr()
+    assert torch.equal(got[: T - 3], want[: T - 3]) and bool((out[T - 3 :] == 7).all()) and bool((out[:, :H] == 7).all())
+    slab = torch.cat([q, q], 1)
+    pkg.packed_cross_attention(slab[:, :H], k, v, qo, ko, out=slab[:, :H])
+    assert torch.equal(slab[: T - 3, :H], want[: T - 3]) and torch.equal(slab[:, H:], q) and torch.equal(slab[T - 3 :, :H], q[T - 3 :])
+    head_major = [t.permute(1, 0, 2).contiguous().permute(1, 0, 2) for t in (q, k, v)]
+    assert torch.equal(pkg.packed_cross_attention(*head_major, qo, ko), want)
+    table = torch.randn(32, H, device=dev)
+    bias = pkg.relative_bias_attention(q, q, q, table, qo)
+    assert torch.equal(pkg.relative_bias_attention(*(head_major[0],) * 3, table, qo), bias)
+    again = q.clone()
+    pkg.relative_bias_attention(again, q, q, table, qo, out=again)
+    assert torch.equal(again[: T - 3], bias[: T - 3]) and torch.equal(again[T - 3 :], q[T - 3 :])
+
+
+@pytest.mark.parametrize("T", [4, 200])
+def test_scores_at_the_ends_of_their_range(pkg, dev, T):
+    """A maximum that rises with every tile, scores of ten thousand, of minus infinity and of NaN."""
+    g = torch.Generator().manual_seed(T)
+    H, D, m = 2, 128, 300
+    q = torch.rand(T, H, D, generator=g).add(0.5).to(BF16)
+    k = torch.randn(m, H, D, generator=g).to(BF16)
+    v = torch.randn(m, H, D, generator=g).to(BF16)
+    k = (k.float() * 0.1 + torch.linspace(-8, 8, m)[:, None, None]).to(BF16)  # rising
+    one = [ref.offsets([T], dev), ref.offsets([m], dev)]
+
+    def check(q, k, v, scale):
+        got = pkg.packed_cross_attention(q.to(dev), k.to(dev), v.to(dev), *one, scale=scale)
+        _check(got, q, k, v, [T], [m], scale)
+
+    check(q, k, v, 1.0)
+    check(q, k.flip(0), v, 1.0)
+    check((q.float() * 8).to(BF16), k, v, 2.0)
+    check(q, k, v, 2.0**-20)
+    low = k.clone()
+    low[7], low[290] = float("-inf"), float("-inf")  # (q is positive: their scores are -inf)
+    got = pkg.packed_cross_attention(q.to(dev), low.to(dev), v.to(dev), *one, scale=0.05)
+    keep = [i for i in range(m) if i not in (7, 290)]
+    _check(got, q, k[keep], v[keep], [T], [m - 2], 0.05)
+    low[:] = float("-inf")  # no key at all
+    assert not pkg.packed_cross_attention(q.to(dev), low.to(dev), v.to(dev), *one, scale=0.05).any()
+    bad = q.clone()
+    bad[1, 0, 3], bad[2, 1] = float("nan"), float("inf")
+    got = pkg.packed_cross_attention(bad.to(dev), k.to(dev), v.to(dev), *one, scale=0.05).cpu()
+    want = pkg.packed_cross_attention(q.to(dev), k.to(dev), v.to(dev), *one, scale=0.05).cpu()
+    assert got[1, 0].isnan().all() and got[2, 1].isnan().all()
+    got[1, 0], got[2, 1] = want[1, 0], want[2, 1]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("n", [3, 150])
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+def test_tables_that_mask(pkg, dev, n, dtype):
+    """A type's lowest value as a mask, which weighs alike where nothing else is there, and minus infinity, which leaves out."""
+    g = torch.Generator().manual_seed(n)
+    H, D = 2, 64
+    q, k, v = (torch.randn(n, H, D, generator=g).mul(0.3).to(BF16) for _ in range(3))
+    table = torch.randn(32, H, generator=g).to(dtype)
+
+    def check(table, size):
+        got = pkg.relative_bias_attention(q.to(dev), k.to(dev), v.to(dev), table.to(dev), ref.offsets([n], dev))
+        _check(got, q, k, v, [n], [n], 1.0, lambda m: ref.bias_matrix(table, m, 128, True), size)
+
+    lowest = table.clone()
+    lowest[16:] = torch.finfo(dtype).min  # nothing behind the query
+    check(lowest, float(table.float().abs().max()))
+    lowest[:] = torch.finfo(dtype).min  # nothing anywhere: all weigh alike
+    check(lowest, 0.0)
+    out = table.clone()
+    out[0] = float("-inf")  # not itself
+    out[20:] = float("-inf")
+    if n > 1:
+        check(out, float(table.float().abs().max()))
+    far = table.float()
+    far[15], far[31] = -20000.0, 20000.0  # a far bias too large to be taken off the maximum
+    far = far.to(dtype)
+    check(far, 20000.0 if n > 91 else float(table.float().abs().max()))
+
+
+def test_no_rows_no_keys_no_requests(pkg, dev):
+    q, k, v = (t.to(dev) for t in _inputs(6, 10, 2, 2, 64, 1))
+    none = torch.zeros(1, dtype=torch.int32, device=dev)
+    assert not pkg.packed_cross_attention(q, k, v, none, none).any()
+    assert pkg.packed_cross_attention(q[:0], k, v, none, none).shape == (0, 2, 64)
+    qo, ko = ref.offsets([6], dev), ref.offsets([0], dev)
+    assert not pkg.packed_cross_attention(q, k[:0], v[:0], qo, ko).any()
+    table = torch.randn(32, 2, device=dev)
+    assert not pkg.relative_bias_attention(q, q, q, table, none).any()
+    assert pkg.relative_bias_attention(q[:0], q[:0], q[:0], table, none).shape == (0, 2, 64)
+    empty = pkg.packed_cross_attention(q[:0], k, v, none, none, quant="mx")
+    assert empty.codes.shape == (0, 128) and empty.scales.shape == (0, 4)
+
+
+@pytest.mark.parametrize("T", [30, 500])
+def test_offsets_that_are_wrong_stay_inside(pkg, dev, T):
+    """Descending, negative and too large: some rows or other, no access out of bounds (the kernel holds every offset inside its tensor)."""
+    q, k, v = (t.to(dev) for t in _inputs(T, 90, 2, 2, 64, 3))
+    for qo, ko in (([0, 400000, 20], [0, 90, 90]), ([T, 0, T], [90, 0, 50]), ([-5, 7, 2**31 - 1], [-(2**31), 2**31 - 1, 12]), ([0, 10, T], [80, 20, 500])):
+        out = pkg.packed_cross_attention(q, k, v, torch.tensor(qo, dtype=torch.int32, device=dev), torch.tensor(ko, dtype=torch.int32, device=dev))
+        torch.cuda.synchronize()
+        assert out.shape == q.shape
+    pkg.relative_bias_attention(q, q, q, torch.randn(32, 2, device=dev), torch.tensor([3, 400000, -1], dtype=torch.int32, device=dev))
+    torch.cuda.synchronize()
+
+
+def test_rows_far_apart(pkg, dev):
+    """Elements beyond 2^31 from the tensor's first."""
+    rows, ss, H, D = 1100, 1 << 21, 2, 64
+    slab = torch.empty(rows, ss, dtype=BF16, device=dev)
+    q, k, v = (slab[:, i * 128 : (i + 1) * 128].view(rows, H, D) for i in range(3))
+    small = [t.to(dev) for t in _inputs(rows, rows, H, H, D, 9)]
+    for t, s in zip((q, k, v), small):
+        t.copy_(s)
+    for lens in ([700, 400], [20] * 55):
+        o = ref.offsets(lens, dev)
+        assert torch.equal(pkg.packed_cross_attention(q, k, v, o, o), pkg.packed_cross_attention(*small, o, o))
+    del slab, q, k, v
+    torch.cuda.empty_cache()
+
+
+def test_other_streams_and_replayed_graphs(pkg, dev):
+    """On a stream of its own beside other calls, and captured: replays follow offsets, queries and tables that were changed in place."""
+    q, k, v = (t.to(dev) for t in _inputs(300, 200, 4, 4, 64, 5))
+    table = torch.randn(32, 4, device=dev)
+    qo, ko, bo = ref.offsets([100, 150], dev), ref.offsets([64, 130], dev), ref.offsets([3, 200, 90], dev)
+    eager = lambda: (pkg.packed_cross_attention(q, k, v, qo, ko), pkg.relative_bias_attention(q, q, q, table, bo))  # noqa: E731
+    want = eager()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = eager()
+    mine = eager()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, other, mine))
+    graphs, outs = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(eager())
+    for a, b in (([100, 150], [64, 130]), ([1, 299], [0, 200]), ([200, 0], [3, 9])):
+        qo.copy_(ref.offsets(a))
+        ko.copy_(ref.offsets(b))
+        bo.copy_(ref.offsets([a[0], 50, 20]))
+        table.mul_(-1.5)
+        q.mul_(0.75)
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        want = eager()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for out in outs for x, y in zip(out, want))

@@ -574,7 +574,8 @@ extern "C" int wanmi_fp8_block_quantize(const void* x, int64_t ldx, int64_t M, i
   WANMI_REQUIRE(x && codes && scales, WANMI_ERR_ARG, "%s: null pointer", what);
   WANMI_REQUIRE((M == 1 || ldx >= K) && ldx % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)codes % 16 == 0, WANMI_ERR_ARG,
                 "%s: rows of x (%lld apart) and the codes must be 16-byte aligned", what, (long long)ldx);
-  WANMI_REQUIRE(M * ((blocks_of(K) + 3) / 4) < (1LL << 32), WANMI_ERR_ARG, "%s: %lld x %lld is too large", what, (long long)M, (long long)K);
+  // (a launch has fewer than 2^32 lanes)
+  WANMI_REQUIRE(M * ((blocks_of(K) + 3) / 4) < (1LL << 26) - 4, WANMI_ERR_ARG, "%s: %lld x %lld is too large", what, (long long)M, (long long)K);
   launch_quantize((const uint16_t*)x, ldx, (int)M, (int)K, codes, scales, s_row, s_blk, (hipStream_t)stream);
   return check_launch(what);
 }
@@ -626,7 +627,8 @@ extern "C" int wanmi_fp8_block_linear(const void* x, const float* x_scales, int6
   const int64_t need = ws.bytes;
   WANMI_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 16 == 0)), WANMI_ERR_ARG,
                 "%s: the workspace holds %lld bytes of %lld", what, (long long)workspace_bytes, (long long)need);
-  WANMI_REQUIRE(((M + 63) / 64) * ((N + 63) / 64) < (1LL << 30) && M * ((KB + 3) / 4) < (1LL << 32), WANMI_ERR_ARG, "%s: too many tiles", what);
+  WANMI_REQUIRE(((M + 63) / 64) * ((N + 63) / 64) * ws.plan.splits < (1LL << 24) && M * ((KB + 3) / 4) < (1LL << 26) - 4, WANMI_ERR_ARG,
+                "%s: %lld x %lld x %lld is too large for a launch", what, (long long)M, (long long)N, (long long)K);
   hipStream_t st = (hipStream_t)stream;
   Fp8Args g{(const uint8_t*)x, ldx, x_scales, xs_row, xs_blk, nullptr, w, w_scales, bias, (uint16_t*)out, ldo, (int)M, (int)N, (int)K, (int)KB, gelu, 0, 0, 1, nullptr};
   if (is_bf16 && M <= kFewQuantize) {

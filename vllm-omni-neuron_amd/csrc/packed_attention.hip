@@ -453,7 +453,8 @@ static int launch(PackedAttnArgs a, const BiasArgs& b, hipStream_t stream, const
   // every request ends in at most one part of a tile, and so do the rows behind the last
   const int64_t tiles = a.T / kRows + a.requests + 1;
   const int64_t per = (tiles * a.heads + 7) / 8;
-  WANMI_REQUIRE(tiles * a.heads < (1LL << 30), WANMI_ERR_ARG, "%s: %lld tiles of rows times %d heads are too many", what, (long long)tiles, a.heads);
+  // (a launch has fewer than 2^32 lanes)
+  WANMI_REQUIRE(tiles * a.heads < (1LL << 24) - 8, WANMI_ERR_ARG, "%s: %lld tiles of rows times %d heads are too many", what, (long long)tiles, a.heads);
   a.tiles = (int)tiles;
   a.per_xcd = (int)per;
   if constexpr (!kBias) {

@@ -150,6 +150,8 @@ def packed_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_
     scale = _check(q, k, v, scale, out, quant, "packed_cross_attention")
     requests = _offsets(q_offsets, "q_offsets")
     _offsets(k_offsets, "k_offsets", requests + 1)
+    if out is not None:
+        _lib.refuse_input(out, "out", q_offsets, k_offsets)
     _lib.require_gpu(q, k, v, q_offsets, k_offsets, out, what="packed_cross_attention")
     T, heads, head_dim = q.shape
     zero_rest = out is None
@@ -161,8 +163,6 @@ def packed_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_
     else:
         if out is None:
             out = torch.empty((T, heads, head_dim), dtype=torch.bfloat16, device=q.device)
-        else:
-            _lib.refuse_input(out, "out", q_offsets, k_offsets)
         ldo = _strides(out)[0]
     if T:
         p = _lib.ptr
@@ -212,12 +212,12 @@ def relative_bias_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, t
     _lib.expect(table, "table", dtype=table.dtype, shape=(None, heads))
     starts = _bucket_starts(table.shape[0], int(max_distance), bool(bidirectional))
     requests = _offsets(offsets, "offsets")
+    if out is not None:
+        _lib.refuse_input(out, "out", table, offsets)
     _lib.require_gpu(q, k, v, table, offsets, out, what="relative_bias_attention")
     zero_rest = out is None
     if out is None:
         out = torch.empty((T, heads, head_dim), dtype=torch.bfloat16, device=q.device)
-    else:
-        _lib.refuse_input(out, "out", table, offsets)
     if T:
         p = _lib.ptr
         _lib.call("wanmi_relative_bias_attention", q.get_device(), p(q), *_strides(q), p(k), *_strides(k), p(v), *_strides(v), p(offsets), requests,

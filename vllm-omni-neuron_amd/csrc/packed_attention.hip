@@ -54,7 +54,8 @@ struct BiasArgs {
   int bf16;
   int side;           // buckets of one direction
   int both;           // buckets for later keys follow those for earlier ones; else every later key takes bucket 0
-  int start[kMaxSide];  // smallest distance of each bucket
+  int sat;            // the distance from which on the last bucket holds
+  uint8_t bucket[kMaxSaturation + 1];  // of every distance up to there
 };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -88,29 +89,31 @@ __device__ __forceinline__ bool find_tile(const PackedAttnArgs& a, int t, int& r
     const int lo = min(max(q_lo, 0), a.T);
     int hi = r < a.requests ? min(max(q_hi, 0), a.T) : a.zero_rest ? a.T : lo;
     if (c + lane > a.requests) hi = lo;
+    // inclusive sums over the lanes: within rows of 16, then each row's last into the rows behind it
     int sum = max(hi - lo + kRows - 1, 0) / kRows;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int s = __shfl_up(sum, o, 64);
-      sum += lane >= o ? s : 0;
-    }
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x112, 0xF, 0xF, false);
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x114, 0xF, 0xF, false);
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x118, 0xF, 0xF, false);
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x142, 0xA, 0xF, false);  // row_bcast 15 into rows 1 and 3
+    sum += __builtin_amdgcn_update_dpp(0, sum, 0x143, 0xC, 0xF, false);  // row_bcast 31 into rows 2 and 3
     sum += before;
     const uint64_t hit = __ballot(sum > t);
     if (hit) {
       const int l = __builtin_ctzll(hit);
-      const int first = __builtin_amdgcn_readfirstlane(l ? __shfl(sum, l - 1, 64) : before);
-      const int at = __builtin_amdgcn_readfirstlane(__shfl(lo, l, 64)), end = __builtin_amdgcn_readfirstlane(__shfl(hi, l, 64));
+      const int first = l ? __builtin_amdgcn_readlane(sum, l - 1) : before;
+      const int at = __builtin_amdgcn_readlane(lo, l), end = __builtin_amdgcn_readlane(hi, l);
       in_request = (t - first) * kRows;
       if (in_request < 0 || in_request >= end - at) return false;
       row0 = at + in_request;
       rows = min(kRows, end - row0);
       // (the rows behind the last request: k_lo and k_hi are the same)
       const int kl = min(max(k_lo, 0), a.Tk), kn = max(min(max(k_hi, 0), a.Tk) - kl, 0);
-      k0 = __builtin_amdgcn_readfirstlane(__shfl(kl, l, 64));
-      keys = __builtin_amdgcn_readfirstlane(__shfl(kn, l, 64));
+      k0 = __builtin_amdgcn_readlane(kl, l);
+      keys = __builtin_amdgcn_readlane(kn, l);
       return true;
     }
-    before = __builtin_amdgcn_readfirstlane(__shfl(sum, 63, 64));
+    before = __builtin_amdgcn_readlane(sum, 63);
   }
   return false;
 }
@@ -133,19 +136,22 @@ __device__ __forceinline__ int mx_codes(const uint32_t (&pp)[8], uint32_t (&code
 template <int D, bool kBias, int kSplit, bool kMx>
 __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs a, BiasArgs bias) {
   constexpr int kRows = 128 / kSplit;              // rows of a workgroup
-  constexpr int kHalves = kSplit == 1 ? 2 : 1;     // 32-key halves of a tile: the workgroup's of 64 keys, or a wave's own of 32
-  constexpr int kKeys = 32 * kHalves;
+  constexpr bool kOwn = kSplit == 4;               // tiles of 32 keys, a wave's own; else 64 keys, of the workgroup
+  constexpr int kHalves = kSplit == 1 ? 2 : 1;     // 32-key halves of a tile that a wave takes
+  constexpr int kKeys = kOwn ? 32 : 64;
   constexpr int kRowB = 2 * D;                     // bytes
   constexpr int kChunks = D / 8;
   constexpr int kTile = kKeys * kRowB;             // of K, and as much of V
-  constexpr int kLoads = kTile / (kSplit == 1 ? 4096 : 1024);  // per wave, of each
+  constexpr int kLoads = kTile / (kOwn ? 1024 : 4096);  // per wave, of each
   constexpr int kRing = 2;
-  constexpr int kRingB = kRing * 2 * kTile * (kSplit == 1 ? 1 : 4);
-  constexpr int kJoin = kSplit == 1 ? 0 : kSplit * 32 * (D * 4 + 8);
+  constexpr int kRingB = kRing * 2 * kTile * (kOwn ? 4 : 1);
+  constexpr int kJoin = kOwn ? kSplit * 32 * (D * 4 + 8) : 0;
   constexpr int kLds = kRingB > kJoin ? kRingB : kJoin;
   constexpr int kBiasLds = kBias ? 2 * (kMaxSaturation + 63) + 2 : 1;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
+  __shared__ __attribute__((aligned(1024))) uint8_t squery[kOwn ? 32 * kRowB : 16];
   __shared__ float sbias[kBiasLds];
+  __shared__ float sstats[kSplit == 2 ? 128 : 1];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, hq = lane >> 5;
@@ -157,13 +163,11 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
 
   // ---- the head's bias over the distances -(sat + 63) .. sat + 63, over the scale: added to the scores before it. Its loads run beside
   // those of the offsets ----
-  [[maybe_unused]] int sat = 0;
+  [[maybe_unused]] const int sat = bias.sat;
   if constexpr (kBias) {
-    sat = bias.start[bias.side - 1];
     for (int i = threadIdx.x; i < 2 * (sat + 63) + 1; i += 256) {
-      const int d = i - (sat + 63), n = abs(d);
-      int b = 0;
-      for (int j = 1; j < bias.side; ++j) b += n >= bias.start[j];
+      const int d = i - (sat + 63);
+      int b = bias.bucket[min(abs(d), sat)];
       if (d > 0) b = bias.both ? b + bias.side : 0;
       const int at = b * a.heads + head;
       const float x = bias.bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t*>(bias.table)[at]) : reinterpret_cast<const float*>(bias.table)[at];
@@ -174,27 +178,35 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
   int row0, rows, in_request, k0, keys;
   if (!find_tile<kRows>(a, work - head * a.tiles, row0, rows, in_request, k0, keys)) return;
 
-  // ---- the wave's 32 queries as MFMA operands: lane holds d = 16 t + 8 hq .. + 7 of query col ----
-  const int qw = kSplit == 1 ? wave * 32 : 0;  // the wave's first row in the tile
-  bf16x8 qf[D / 16];
+  const int lrow = lane / kChunks, lslot = lane % kChunks;
+  constexpr int kPer = 64 / kChunks;  // rows of a load: four, or at D = 64 eight
+  uint8_t* ring = lds + (kOwn ? wave * (kRing * 2 * kTile) : 0);
+  const int qw = kSplit == 1 ? wave * 32 : kSplit == 2 ? (wave & 1) * 32 : 0;  // the wave's first row in the tile
+  const int half = kSplit == 2 ? wave >> 1 : 0;                                // and its half of the keys
+
+  // ---- the wave's 32 queries, whole rows into LDS: into the second slot, which the second tile takes later; kSplit 4: all waves have the
+  // same, eight rows are each one's part (gathered into the MFMA's layout from memory a load touches 32 bytes of 32 rows) ----
+  uint8_t* sq = kOwn ? squery : lds + 2 * kTile + wave * (32 * kRowB);
+  static_assert(kOwn || 4 * 32 * kRowB <= 2 * kTile, "the queries fit a slot");
   {
-    const int r = min(qw + col, rows - 1);  // rows behind the tile's repeat its last and are not written
-    const uint16_t* pq = a.q + (int64_t)(row0 + r) * a.q_ss + (int64_t)head * a.q_hs + 8 * hq;
+    const int live = min(rows - qw, 32);  // rows behind them read as zeros, and are not written
+    const u32x4 r = buffer_rsrc(a.q + (int64_t)(row0 + qw) * a.q_ss + (int64_t)head * a.q_hs, live > 0 ? (uint32_t)(((live - 1) * a.q_ss + D) * 2) : 0u);
+    constexpr int kN = 32 / kPer / (kOwn ? 4 : 1);
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) qf[t] = *reinterpret_cast<const bf16x8*>(pq + 16 * t);
+    for (int j = 0; j < kN; ++j) {
+      const int first = ((kOwn ? wave * kN : 0) + j) * kPer, row = first + lrow;
+      lds_dma_b128(r, (uint32_t)row * (uint32_t)(a.q_ss * 2) + (uint32_t)((lslot ^ k_slot<D>(row)) << 4), lds_addr(sq) + first * kRowB);
+    }
   }
 
-  // ---- loads of a tile of keys: four rows (D = 64: eight) to an instruction; kSplit 4: the wave's own keys into its own LDS ----
+  // ---- loads of a tile of keys; kSplit 4: the wave's own keys into its own LDS ----
   const int khead = head / a.group;
   const uint16_t* kb = a.k + (int64_t)k0 * a.k_ss + (int64_t)khead * a.k_hs;
   const uint16_t* vb = a.v + (int64_t)k0 * a.v_ss + (int64_t)khead * a.v_hs;
-  const int lrow = lane / kChunks, lslot = lane % kChunks;
-  constexpr int kPer = 64 / kChunks;  // rows of an instruction
-  uint8_t* ring = lds + (kSplit == 1 ? 0 : wave * (kRing * 2 * kTile));
   // the tile's number along the keys, and how many there are for this wave
-  auto tile_at = [&](int t) { return kSplit == 1 ? t : t * kSplit + wave; };
+  auto tile_at = [&](int t) { return kOwn ? t * kSplit + wave : t; };
   const int all = (keys + kKeys - 1) / kKeys;
-  const int tiles = kSplit == 1 ? all : (all - wave + kSplit - 1) / kSplit;
+  const int tiles = kOwn ? (all - wave + kSplit - 1) / kSplit : all;
   auto load_tile = [&](int t) {
     const int first = tile_at(t) * kKeys, left = min(keys - first, kKeys);  // > 0
     const u32x4 rk = buffer_rsrc(kb + (int64_t)first * a.k_ss, (uint32_t)(((left - 1) * a.k_ss + D) * 2));
@@ -202,17 +214,25 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
     const uint32_t to = lds_addr(ring) + (uint32_t)((t % kRing) * 2 * kTile);
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
-      const int r = ((kSplit == 1 ? wave * kLoads : 0) + j) * kPer;  // the instruction's first row; keys past the text read as zeros
+      const int r = ((kOwn ? 0 : wave * kLoads) + j) * kPer;  // the instruction's first row; keys past the text read as zeros
       const int key = r + lrow;
       lds_dma_b128(rk, (uint32_t)key * (uint32_t)(a.k_ss * 2) + (uint32_t)((lslot ^ k_slot<D>(key)) << 4), to + r * kRowB);
       lds_dma_b128(rv, (uint32_t)key * (uint32_t)(a.v_ss * 2) + (uint32_t)((lslot ^ v_slot<D>(key)) << 4), to + kTile + r * kRowB);
     }
   };
   if (tiles > 0) load_tile(0);
-  if (kSplit > 1 && tiles > 1) load_tile(1);
+  if (kOwn && tiles > 1) load_tile(1);
+
+  // ---- the queries as MFMA operands: lane holds d = 16 t + 8 hq .. + 7 of query col ----
+  // (with the first tile, which is waited for here and not at the top of the loop)
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+  if (kOwn || kBias) __syncthreads();
+  bf16x8 qf[D / 16];
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) qf[t] = *reinterpret_cast<const bf16x8*>(sq + col * kRowB + (((2 * t + hq) ^ k_slot<D>(col)) << 4));
+  __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0));  // (read before the second tile may come)
   [[maybe_unused]] float far_lo = 0.0f, far_hi = 0.0f;
   if constexpr (kBias) {
-    __syncthreads();
     far_lo = sbias[0];
     far_hi = sbias[2 * (sat + 63)];
   }
@@ -227,7 +247,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
   const bf16x2_t ones = {(__bf16)1.0f, (__bf16)1.0f};
 
   for (int t = 0; t < tiles; ++t) {
-    if constexpr (kSplit == 1) {
+    if constexpr (!kOwn) {
       __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
       __syncthreads();  // the tile is in LDS, and every wave is done with the one before it
       if (t + 1 < tiles) load_tile(t + 1);
@@ -236,9 +256,10 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
     } else {
       __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
     }
-    const uint8_t* tk = ring + (t % kRing) * 2 * kTile;
+    const uint8_t* tk = ring + (t % kRing) * 2 * kTile + half * 32 * kRowB;
     const uint8_t* tv = tk + kTile;
-    const int left = keys - tile_at(t) * kKeys;
+    const int left = keys - tile_at(t) * kKeys - half * 32;
+    if (kSplit == 2 && left <= 0) continue;  // (no key of the second half)
 
     f32x16 s[kHalves];
 #pragma unroll
@@ -259,7 +280,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
     for (int i = 0; i < kHalves; ++i) {
       shared[i] = 0.0f;
       if constexpr (kBias) {
-        const int d0 = tile_at(t) * kKeys + 32 * i - (in_request + qw);  // first key - first query
+        const int d0 = tile_at(t) * kKeys + 32 * (i + half) - (in_request + qw);  // first key - first query
         const float far = d0 > 0 ? far_hi : far_lo;
         if (d0 - 31 < sat && d0 + 31 > -sat) {
           asm volatile("");  // (a branch: not both sides computed and one selected)
@@ -336,17 +357,45 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
         }
       }
     }
-    if (kSplit > 1 && t + 2 < tiles) {
+    if (kOwn && t + 2 < tiles) {
       __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0));  // the wave has read its tile
       load_tile(t + 2);
     }
   }
   sum = add_lane_xor32(sum);
-  __syncthreads();  // LDS is free
 
-  if constexpr (kSplit == 1) {
+  // The slot that the last tile is not in: every wave is past the barrier behind its last use, and no load is under way to it.
+  uint8_t* idle = lds + (tiles % kRing) * 2 * kTile;
+  if constexpr (kSplit == 2) {
+    // ---- the second half's waves hand their part over: [d][row] sums of P V, and each row's maximum and sum ----
+    float* part = reinterpret_cast<float*>(idle) + (wave & 1) * (32 * D);
+    static_assert(2 * 32 * D * 4 <= 2 * kTile, "two parts fit a slot");
+    __syncthreads();  // (idle: without a tile, or with one alone, it holds queries)
+    if (half == 1) {
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) part[(32 * dt + 8 * (r >> 2) + 4 * hq + (r & 3)) * 32 + col] = acc[dt][r];
+      if (hq == 0) {
+        sstats[(wave & 1) * 64 + col] = m;
+        sstats[(wave & 1) * 64 + 32 + col] = sum;
+      }
+    }
+    __syncthreads();
+    if (half == 1) return;
+    const float mo = sstats[(wave & 1) * 64 + col], so = sstats[(wave & 1) * 64 + 32 + col], mm = fmaxf(m, mo);
+    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mm) * c), fo = mo == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mo - mm) * c);
+    sum = (sum == 0.0f ? 0.0f : f * sum) + (so == 0.0f ? 0.0f : fo * so);  // (a NaN maximum is no maximum, but its sum is NaN)
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[dt][r] = fmaf(fo, part[(32 * dt + 8 * (r >> 2) + 4 * hq + (r & 3)) * 32 + col], f * acc[dt][r]);
+  }
+
+  if constexpr (!kOwn) {
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no keys: zeros; NaN stays
-    uint8_t* stage = lds + wave * (32 * kRowB);
+    // (kSplit 2: over the wave's own part, which it has read)
+    uint8_t* stage = idle + (kSplit == 2 ? (wave & 1) * (64 * kRowB) : wave * (32 * kRowB));
     const int live = min(rows - qw, 32);  // rows of the wave
     [[maybe_unused]] uint32_t sbytes = 0;
 #pragma unroll
@@ -394,6 +443,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
     }
   } else {
     // ---- join the waves' parts: [wave][d][row] sums of P V, then [wave][row] maxima and sums ----
+    __syncthreads();  // every wave is done with its tiles
     float* parts = reinterpret_cast<float*>(lds);
     float* stats = parts + kSplit * 32 * D;
 #pragma unroll
@@ -467,12 +517,11 @@ static int launch(PackedAttnArgs a, const BiasArgs& b, hipStream_t stream, const
   return check_launch(what);
 }
 
-template <bool kBias>
-static int dispatch(const PackedAttnArgs& a, const BiasArgs& b, int head_dim, hipStream_t stream, const char* what) {
+template <bool kBias, int D>
+static int dispatch(const PackedAttnArgs& a, const BiasArgs& b, hipStream_t stream, const char* what) {
   // few rows per request: a tile of 32 rows whose keys the waves share out
-  const bool few = a.T <= (int64_t)32 * a.requests;
-  if (head_dim == 64) return few ? launch<64, kBias, 4>(a, b, stream, what) : launch<64, kBias, 1>(a, b, stream, what);
-  return few ? launch<128, kBias, 4>(a, b, stream, what) : launch<128, kBias, 1>(a, b, stream, what);
+  if (a.T <= (int64_t)32 * a.requests) return launch<D, kBias, 4>(a, b, stream, what);
+  return launch<D, kBias, 1>(a, b, stream, what);
 }
 
 // What both entry points check: sizes, strides and alignment that the kernel's 16-byte accesses and 32-bit offsets need.
@@ -506,7 +555,8 @@ extern "C" int wanmi_packed_cross_attention(const void* q, int64_t q_ss, int64_t
                    (int)T, (int)Tk, (int)heads, (int)(k_heads > 0 ? heads / k_heads : 1), scale * 1.4426950408889634f, kSlack / (scale * 1.4426950408889634f), 1.0f / scale, out, o_ss, out_scales, zero_rest, 0, 0};
   const int st = check_args(a, T, Tk, requests, heads, k_heads, head_dim, "wanmi_packed_cross_attention");
   if (st != WANMI_OK || T == 0) return st;
-  return dispatch<false>(a, BiasArgs{}, head_dim, (hipStream_t)stream, "wanmi_packed_cross_attention");
+  const char* what = "wanmi_packed_cross_attention";
+  return head_dim == 64 ? dispatch<false, 64>(a, BiasArgs{}, (hipStream_t)stream, what) : dispatch<false, 128>(a, BiasArgs{}, (hipStream_t)stream, what);
 }
 
 extern "C" int wanmi_relative_bias_attention(const void* q, int64_t q_ss, int64_t q_hs, const void* k, int64_t k_ss, int64_t k_hs,
@@ -521,13 +571,15 @@ extern "C" int wanmi_relative_bias_attention(const void* q, int64_t q_ss, int64_
   const int st = check_args(a, T, T, requests, heads, heads, head_dim, what);
   if (st != WANMI_OK) return st;
   WANMI_REQUIRE(side >= 1 && side <= kMaxSide && starts, WANMI_ERR_ARG, "%s: %d buckets of one direction, at most %d", what, side, kMaxSide);
-  BiasArgs b{table, table_bf16, side, both, {0}};
-  for (int i = 0; i < side; ++i) {
-    WANMI_REQUIRE(starts[i] >= (i ? starts[i - 1] : 0) && starts[i] <= kMaxSaturation, WANMI_ERR_ARG,
+  for (int i = 0; i < side; ++i)
+    WANMI_REQUIRE(starts[i] >= (i ? starts[i - 1] : 0) && starts[i] <= kMaxSaturation && starts[0] == 0, WANMI_ERR_ARG,
                   "%s: the buckets' first distances must ascend from 0 to at most %d", what, kMaxSaturation);
-    b.start[i] = starts[i];
+  BiasArgs b{table, table_bf16, side, both, starts[side - 1], {0}};
+  for (int n = 0, i = 0; n <= b.sat; ++n) {
+    while (i + 1 < side && starts[i + 1] <= n) ++i;
+    b.bucket[n] = (uint8_t)i;
   }
   if (T == 0) return WANMI_OK;
   WANMI_REQUIRE(table, WANMI_ERR_ARG, "%s: null pointer", what);
-  return dispatch<true>(a, b, head_dim, (hipStream_t)stream, what);
+  return head_dim == 64 ? dispatch<true, 64>(a, b, (hipStream_t)stream, what) : dispatch<true, 128>(a, b, (hipStream_t)stream, what);
 }

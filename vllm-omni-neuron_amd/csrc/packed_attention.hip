@@ -118,6 +118,14 @@ __device__ __forceinline__ bool find_tile(const PackedAttnArgs& a, int t, int& r
   return false;
 }
 
+// Rows of the output for a wave's stores: those past the extent are dropped. (Address and extent are the same in every lane, which the compiler
+// does not prove: kept in vector registers each store would be a loop over the lanes' values.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(void* p, uint32_t bytes) {
+  const uint64_t at = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at), hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), (short)0, (int)__builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+}
+
 // 16 outputs of a lane (d = 8 g + 4 hq + q of a block of 32) as bf16 pairs; kMx: as four words of codes and the block's
 // scale byte. The block's other half is lane ^ 32's.
 __device__ __forceinline__ int mx_codes(const uint32_t (&pp)[8], uint32_t (&codes)[4]) {
@@ -195,7 +203,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
 #pragma unroll
     for (int j = 0; j < kN; ++j) {
       const int first = ((kOwn ? wave * kN : 0) + j) * kPer, row = first + lrow;
-      lds_dma_b128(r, (uint32_t)row * (uint32_t)(a.q_ss * 2) + (uint32_t)((lslot ^ k_slot<D>(row)) << 4), lds_addr(sq) + first * kRowB);
+      lds_dma_b128(r, (uint32_t)__umul24((uint32_t)row, (uint32_t)(a.q_ss * 2)) + (uint32_t)((lslot ^ k_slot<D>(row)) << 4), lds_addr(sq) + first * kRowB);
     }
   }
 
@@ -216,8 +224,8 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
     for (int j = 0; j < kLoads; ++j) {
       const int r = ((kOwn ? 0 : wave * kLoads) + j) * kPer;  // the instruction's first row; keys past the text read as zeros
       const int key = r + lrow;
-      lds_dma_b128(rk, (uint32_t)key * (uint32_t)(a.k_ss * 2) + (uint32_t)((lslot ^ k_slot<D>(key)) << 4), to + r * kRowB);
-      lds_dma_b128(rv, (uint32_t)key * (uint32_t)(a.v_ss * 2) + (uint32_t)((lslot ^ v_slot<D>(key)) << 4), to + kTile + r * kRowB);
+      lds_dma_b128(rk, (uint32_t)__umul24((uint32_t)key, (uint32_t)(a.k_ss * 2)) + (uint32_t)((lslot ^ k_slot<D>(key)) << 4), to + r * kRowB);
+      lds_dma_b128(rv, (uint32_t)__umul24((uint32_t)key, (uint32_t)(a.v_ss * 2)) + (uint32_t)((lslot ^ v_slot<D>(key)) << 4), to + kTile + r * kRowB);
     }
   };
   if (tiles > 0) load_tile(0);
@@ -243,7 +251,9 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
   float m = -INFINITY, sum = 0.0f;  // m in units of the scores before their scale
-  const float c = a.scale_log2;
+  // (in a vector register: a multiply-add that reads a scalar one takes 4.5 cycles in place of 2.7)
+  float c = a.scale_log2;
+  asm volatile("" : "+v"(c));
   const bf16x2_t ones = {(__bf16)1.0f, (__bf16)1.0f};
 
   for (int t = 0; t < tiles; ++t) {
@@ -298,11 +308,12 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
     }
     if (left < 32 * kHalves) {
       asm volatile("");
+      const int mine = left - 4 * hq;
 #pragma unroll
       for (int i = 0; i < kHalves; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (32 * i + 8 * (r >> 2) + 4 * hq + (r & 3) >= left) s[i][r] = -INFINITY;
+          if (32 * i + 8 * (r >> 2) + (r & 3) >= mine) s[i][r] = -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -317,11 +328,13 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
       const float mn = fmaxf(m, mx);
       const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
       m = mn;
-      sum *= f;
+      if (t > 0) {  // (before, there is nothing to rescale)
+        sum *= f;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i)
+        for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][r] *= f;
+          for (int r = 0; r < 16; ++r) acc[i][r] *= f;
+      }
     }
     const float base = m == -INFINITY ? 0.0f : m;  // no key above -inf yet: every P is 0
 #pragma unroll
@@ -417,15 +430,16 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
           *reinterpret_cast<uint2*>(stage + col * kRowB + (((4 * dt + g) ^ (col & (kChunks - 1))) << 4) + 8 * hq) = make_uint2(pp[2 * g], pp[2 * g + 1]);
       }
     }
-    // (a wave's LDS operations complete in order: no barrier before its own rows are read back)
+    // (a wave's LDS operations complete in order: no barrier before its own rows are read back; rows behind the wave's are dropped)
+    const int64_t item = kMx ? 1 : 2;
+    const auto ro = row_rsrc(reinterpret_cast<uint8_t*>(a.out) + ((int64_t)(row0 + qw) * a.o_ss + head * D) * item, (uint32_t)max(live, 0) * (uint32_t)(a.o_ss * item));
     if constexpr (kMx) {
-      uint8_t* po = reinterpret_cast<uint8_t*>(a.out) + (int64_t)(row0 + qw) * a.o_ss + head * D;
       constexpr int kPerRow = D / 16, kStep = 64 / kPerRow;
 #pragma unroll
       for (int it = 0; it < 32 / kStep; ++it) {
         const int r = it * kStep + lane / kPerRow, chunk = lane % kPerRow;
         const u32x4 x = *reinterpret_cast<const u32x4*>(stage + r * D + ((chunk ^ ((r >> 1) & (D / 16 - 1))) << 4));
-        if (r < live) store_b128_guarded(x, po + (int64_t)r * a.o_ss + chunk * 16);
+        __builtin_amdgcn_raw_buffer_store_b128(x, ro, (int)(__umul24((uint32_t)r, (uint32_t)a.o_ss) + chunk * 16), 0, 2);
       }
       if (hq == 0 && col < live) {
         uint8_t* ps = a.out_scales + (int64_t)(row0 + qw + col) * (a.heads * (D / 32)) + head * (D / 32);
@@ -433,12 +447,11 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
         else *reinterpret_cast<uint16_t*>(ps) = (uint16_t)sbytes;
       }
     } else {
-      uint16_t* po = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(row0 + qw) * a.o_ss + head * D;
 #pragma unroll
       for (int it = 0; it < 32 / kPer; ++it) {
         const int r = it * kPer + lrow;
         const u32x4 x = *reinterpret_cast<const u32x4*>(stage + r * kRowB + ((lslot ^ (r & (kChunks - 1))) << 4));
-        if (r < live) store_b128_guarded(x, po + (int64_t)r * a.o_ss + lslot * 8);
+        __builtin_amdgcn_raw_buffer_store_b128(x, ro, (int)(__umul24((uint32_t)r, (uint32_t)(a.o_ss * 2)) + lslot * 16), 0, 2);
       }
     }
   } else {
@@ -539,7 +552,7 @@ static int check_args(const PackedAttnArgs& a, int64_t T, int64_t Tk, int64_t re
   WANMI_REQUIRE(((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) % 16 == 0, WANMI_ERR_ARG, "%s: q, k, v and out must be 16-byte aligned", what);
   WANMI_REQUIRE(T == 1 || a.q_ss >= head_dim, WANMI_ERR_ARG, "%s: rows of q overlap", what);
   WANMI_REQUIRE(Tk <= 1 || (a.k_ss >= head_dim && a.v_ss >= head_dim), WANMI_ERR_ARG, "%s: rows of k or v overlap", what);
-  WANMI_REQUIRE(a.o_ss % 16 == 0 && a.o_ss >= heads * head_dim, WANMI_ERR_ARG, "%s: the output's row stride must be a multiple of 16 of at least %lld", what, (long long)(heads * head_dim));
+  WANMI_REQUIRE(a.o_ss % 16 == 0 && a.o_ss >= heads * head_dim && a.o_ss < (1 << 22), WANMI_ERR_ARG, "%s: the output's row stride must be a multiple of 16 of at least %lld, below 2^22", what, (long long)(heads * head_dim));
   return WANMI_OK;
 }
 

@@ -41,6 +41,12 @@ CROSS = [
     ([64] * 70, [3 + i for i in range(70)], 9, 2, 2, 64),
     ([2] * 130, [i % 5 for i in range(130)], 0, 2, 2, 128),
     ([1000, 24], [2000, 1], 0, 2, 2, 128),
+    # as many heads as take tiles of 128 rows
+    ([129], [65], 0, 60, 30, 128),
+    ([33, 31, 32], [129, 127, 128], 1, 90, 30, 64),
+    ([200, 3, 500], [33, 700, 97], 5, 24, 6, 64),
+    ([1000, 24], [2000, 1], 0, 10, 10, 128),
+    ([100, 200, 0], [0, 300, 128], 30, 40, 8, 128),
 ]
 
 
@@ -66,6 +72,12 @@ BIAS = [
     ([257, 64], 0, 2, 64, 32, 128, False, torch.float32),
     ([5, 6, 7], 0, 2, 128, 4, 3, True, BF16),
     ([1500], 0, 1, 64, 256, 1024, True, torch.float32),
+    # as many heads as take tiles of 128 rows
+    ([40, 1, 0, 300], 5, 40, 64, 32, 128, True, BF16),
+    ([511, 130], 0, 15, 128, 20, 250, True, torch.float32),
+    ([700], 1, 30, 64, 8, 20, True, torch.float32),
+    ([257, 64], 0, 48, 64, 32, 128, False, torch.float32),
+    ([1500], 0, 12, 64, 256, 1024, True, torch.float32),
 ]
 
 
@@ -85,9 +97,10 @@ def test_relative_bias(pkg, dev, case):
     assert not got[sum(lens):].any()
 
 
-@pytest.mark.parametrize("q_lens,k_lens,pad,D", [([3, 1, 9], [40, 0, 7], 4, 128), ([3, 1, 9], [40, 0, 7], 4, 64), ([200, 90], [130, 65], 7, 128), ([200, 90], [130, 65], 7, 64)])
-def test_codes_are_those_of_the_bf16_output(pkg, dev, q_lens, k_lens, pad, D):
-    q, k, v = (t.to(dev) for t in _inputs(sum(q_lens) + pad, sum(k_lens), 4, 2, D, 7))
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("q_lens,k_lens,pad,heads", [([3, 1, 9], [40, 0, 7], 4, 4), ([200, 90], [130, 65], 7, 4), ([200, 90], [130, 65], 7, 50)])
+def test_codes_are_those_of_the_bf16_output(pkg, dev, q_lens, k_lens, pad, heads, D):
+    q, k, v = (t.to(dev) for t in _inputs(sum(q_lens) + pad, sum(k_lens), heads, heads // 2, D, 7))
     qo, ko = ref.offsets(q_lens, dev), ref.offsets(k_lens, dev)
     out = pkg.packed_cross_attention(q, k, v, qo, ko)
     got = pkg.packed_cross_attention(q, k, v, qo, ko, quant="mx")
@@ -119,11 +132,11 @@ def test_given_outputs_and_layouts(pkg, dev, T):
     assert torch.equal(again[: T - 3], bias[: T - 3]) and torch.equal(again[T - 3 :], q[T - 3 :])
 
 
-@pytest.mark.parametrize("T", [4, 200])
-def test_scores_at_the_ends_of_their_range(pkg, dev, T):
+@pytest.mark.parametrize("T,H", [(4, 2), (200, 2), (200, 40)])
+def test_scores_at_the_ends_of_their_range(pkg, dev, T, H):
     """A maximum that rises with every tile, scores of ten thousand, of minus infinity and of NaN."""
     g = torch.Generator().manual_seed(T)
-    H, D, m = 2, 128, 300
+    D, m = 128, 300
     q = torch.rand(T, H, D, generator=g).add(0.5).to(BF16)
     k = torch.randn(m, H, D, generator=g).to(BF16)
     v = torch.randn(m, H, D, generator=g).to(BF16)
@@ -154,12 +167,12 @@ def test_scores_at_the_ends_of_their_range(pkg, dev, T):
     assert torch.equal(got, want)
 
 
-@pytest.mark.parametrize("n", [3, 150])
+@pytest.mark.parametrize("n,H", [(3, 2), (150, 2), (150, 110)])
 @pytest.mark.parametrize("dtype", [torch.float32, BF16])
-def test_tables_that_mask(pkg, dev, n, dtype):
+def test_tables_that_mask(pkg, dev, n, H, dtype):
     """A type's lowest value as a mask, which weighs alike where nothing else is there, and minus infinity, which leaves out."""
     g = torch.Generator().manual_seed(n)
-    H, D = 2, 64
+    D = 64
     q, k, v = (torch.randn(n, H, D, generator=g).mul(0.3).to(BF16) for _ in range(3))
     table = torch.randn(32, H, generator=g).to(dtype)
 
@@ -197,23 +210,23 @@ def test_no_rows_no_keys_no_requests(pkg, dev):
     assert empty.codes.shape == (0, 128) and empty.scales.shape == (0, 4)
 
 
-@pytest.mark.parametrize("T", [30, 500])
-def test_offsets_that_are_wrong_stay_inside(pkg, dev, T):
+@pytest.mark.parametrize("T,H", [(30, 2), (500, 2), (500, 40)])
+def test_offsets_that_are_wrong_stay_inside(pkg, dev, T, H):
     """Descending, negative and too large: some rows or other, no access out of bounds (the kernel holds every offset inside its tensor)."""
-    q, k, v = (t.to(dev) for t in _inputs(T, 90, 2, 2, 64, 3))
+    q, k, v = (t.to(dev) for t in _inputs(T, 90, H, H, 64, 3))
     for qo, ko in (([0, 400000, 20], [0, 90, 90]), ([T, 0, T], [90, 0, 50]), ([-5, 7, 2**31 - 1], [-(2**31), 2**31 - 1, 12]), ([0, 10, T], [80, 20, 500])):
         out = pkg.packed_cross_attention(q, k, v, torch.tensor(qo, dtype=torch.int32, device=dev), torch.tensor(ko, dtype=torch.int32, device=dev))
         torch.cuda.synchronize()
         assert out.shape == q.shape
-    pkg.relative_bias_attention(q, q, q, torch.randn(32, 2, device=dev), torch.tensor([3, 400000, -1], dtype=torch.int32, device=dev))
+    pkg.relative_bias_attention(q, q, q, torch.randn(32, H, device=dev), torch.tensor([3, 400000, -1], dtype=torch.int32, device=dev))
     torch.cuda.synchronize()
 
 
 def test_rows_far_apart(pkg, dev):
     """Elements beyond 2^31 from the tensor's first."""
-    rows, ss, H, D = 1100, 1 << 21, 2, 64
+    rows, ss, H, D = 1100, 1 << 21, 20, 64
     slab = torch.empty(rows, ss, dtype=BF16, device=dev)
-    q, k, v = (slab[:, i * 128 : (i + 1) * 128].view(rows, H, D) for i in range(3))
+    q, k, v = (slab[:, i * H * D : (i + 1) * H * D].view(rows, H, D) for i in range(3))
     small = [t.to(dev) for t in _inputs(rows, rows, H, H, D, 9)]
     for t, s in zip((q, k, v), small):
         t.copy_(s)

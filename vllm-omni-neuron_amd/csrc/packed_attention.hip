@@ -144,8 +144,9 @@ __device__ __forceinline__ int mx_codes(const uint32_t (&pp)[8], uint32_t (&code
 template <int D, bool kBias, int kSplit, bool kMx>
 __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs a, BiasArgs bias) {
   constexpr int kRows = 128 / kSplit;              // rows of a workgroup
+  static_assert(kSplit == 1 || kSplit == 4, "whole waves of rows or of keys");
   constexpr bool kOwn = kSplit == 4;               // tiles of 32 keys, a wave's own; else 64 keys, of the workgroup
-  constexpr int kHalves = kSplit == 1 ? 2 : 1;     // 32-key halves of a tile that a wave takes
+  constexpr int kHalves = kOwn ? 1 : 2;            // 32-key halves of a tile
   constexpr int kKeys = kOwn ? 32 : 64;
   constexpr int kRowB = 2 * D;                     // bytes
   constexpr int kChunks = D / 8;
@@ -159,7 +160,6 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
   __shared__ __attribute__((aligned(1024))) uint8_t squery[kOwn ? 32 * kRowB : 16];
   __shared__ float sbias[kBiasLds];
-  __shared__ float sstats[kSplit == 2 ? 128 : 1];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, hq = lane >> 5;
@@ -189,8 +189,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
   const int lrow = lane / kChunks, lslot = lane % kChunks;
   constexpr int kPer = 64 / kChunks;  // rows of a load: four, or at D = 64 eight
   uint8_t* ring = lds + (kOwn ? wave * (kRing * 2 * kTile) : 0);
-  const int qw = kSplit == 1 ? wave * 32 : kSplit == 2 ? (wave & 1) * 32 : 0;  // the wave's first row in the tile
-  const int half = kSplit == 2 ? wave >> 1 : 0;                                // and its half of the keys
+  const int qw = kOwn ? 0 : wave * 32;  // the wave's first row in the tile
 
   // ---- the wave's 32 queries, whole rows into LDS: into the second slot, which the second tile takes later; kSplit 4: all waves have the
   // same, eight rows are each one's part (gathered into the MFMA's layout from memory a load touches 32 bytes of 32 rows) ----
@@ -266,10 +265,9 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
     } else {
       __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
     }
-    const uint8_t* tk = ring + (t % kRing) * 2 * kTile + half * 32 * kRowB;
+    const uint8_t* tk = ring + (t % kRing) * 2 * kTile;
     const uint8_t* tv = tk + kTile;
-    const int left = keys - tile_at(t) * kKeys - half * 32;
-    if (kSplit == 2 && left <= 0) continue;  // (no key of the second half)
+    const int left = keys - tile_at(t) * kKeys;
 
     f32x16 s[kHalves];
 #pragma unroll
@@ -290,7 +288,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
     for (int i = 0; i < kHalves; ++i) {
       shared[i] = 0.0f;
       if constexpr (kBias) {
-        const int d0 = tile_at(t) * kKeys + 32 * (i + half) - (in_request + qw);  // first key - first query
+        const int d0 = tile_at(t) * kKeys + 32 * i - (in_request + qw);  // first key - first query
         const float far = d0 > 0 ? far_hi : far_lo;
         if (d0 - 31 < sat && d0 + 31 > -sat) {
           asm volatile("");  // (a branch: not both sides computed and one selected)
@@ -377,38 +375,10 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
   }
   sum = add_lane_xor32(sum);
 
-  // The slot that the last tile is not in: every wave is past the barrier behind its last use, and no load is under way to it.
-  uint8_t* idle = lds + (tiles % kRing) * 2 * kTile;
-  if constexpr (kSplit == 2) {
-    // ---- the second half's waves hand their part over: [d][row] sums of P V, and each row's maximum and sum ----
-    float* part = reinterpret_cast<float*>(idle) + (wave & 1) * (32 * D);
-    static_assert(2 * 32 * D * 4 <= 2 * kTile, "two parts fit a slot");
-    __syncthreads();  // (idle: without a tile, or with one alone, it holds queries)
-    if (half == 1) {
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) part[(32 * dt + 8 * (r >> 2) + 4 * hq + (r & 3)) * 32 + col] = acc[dt][r];
-      if (hq == 0) {
-        sstats[(wave & 1) * 64 + col] = m;
-        sstats[(wave & 1) * 64 + 32 + col] = sum;
-      }
-    }
-    __syncthreads();
-    if (half == 1) return;
-    const float mo = sstats[(wave & 1) * 64 + col], so = sstats[(wave & 1) * 64 + 32 + col], mm = fmaxf(m, mo);
-    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mm) * c), fo = mo == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mo - mm) * c);
-    sum = (sum == 0.0f ? 0.0f : f * sum) + (so == 0.0f ? 0.0f : fo * so);  // (a NaN maximum is no maximum, but its sum is NaN)
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[dt][r] = fmaf(fo, part[(32 * dt + 8 * (r >> 2) + 4 * hq + (r & 3)) * 32 + col], f * acc[dt][r]);
-  }
-
   if constexpr (!kOwn) {
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no keys: zeros; NaN stays
-    // (kSplit 2: over the wave's own part, which it has read)
-    uint8_t* stage = idle + (kSplit == 2 ? (wave & 1) * (64 * kRowB) : wave * (32 * kRowB));
+    // The slot that the last tile is not in: every wave is past the barrier behind its last use, and no load is under way to it.
+    uint8_t* stage = lds + (tiles % kRing) * 2 * kTile + wave * (32 * kRowB);
     const int live = min(rows - qw, 32);  // rows of the wave
     [[maybe_unused]] uint32_t sbytes = 0;
 #pragma unroll
@@ -532,8 +502,13 @@ static int launch(PackedAttnArgs a, const BiasArgs& b, hipStream_t stream, const
 
 template <bool kBias, int D>
 static int dispatch(const PackedAttnArgs& a, const BiasArgs& b, hipStream_t stream, const char* what) {
-  // few rows per request: a tile of 32 rows whose keys the waves share out
-  if (a.T <= (int64_t)32 * a.requests) return launch<D, kBias, 4>(a, b, stream, what);
+  // Tiles of 32 rows whose keys the waves share out, where a request has no more rows than that, so that tiles of 128 would leave three
+  // waves of four without rows; and where all of them are on the chip at once (one to a CU with its 144 KB of LDS, two at head_dim 64) and there is
+  // more than a tile of keys to share out. 40 heads x 128, us with shared keys against 128 rows: 128 rows of one request, 512 keys 9.7 / 12.9,
+  // 2000 keys 24 / 41, 40 keys 5.9 / 5.1; past one round 200 rows 17.3 / 13.1, 400 rows 25 / 13.4. 64 heads x 64: 200 rows of 512 keys
+  // 8.7 / 9.8, 400 rows 14.9 / 13.2. 12 heads x 64 with a bias: a prompt of 1024 tokens 12.9 / 20.8.
+  const int64_t small = (int64_t)(a.T / 32 + a.requests) * a.heads;
+  if (a.T <= (int64_t)32 * a.requests || (small <= (D == 128 ? 256 : 512) && a.Tk > (int64_t)64 * a.requests)) return launch<D, kBias, 4>(a, b, stream, what);
   return launch<D, kBias, 1>(a, b, stream, what);
 }
 

@@ -47,6 +47,7 @@ struct PackedAttnArgs {
   uint8_t* out_scales;  // MX: [T, heads * D / 32]
   int zero_rest;        // rows behind the last request: written as zeros, or left
   int tiles, per_xcd;   // tiles of rows (an upper bound), workgroups per XCD
+  int together;         // heads that take the same tile one after the other; divides heads
 };
 
 struct BiasArgs {
@@ -163,11 +164,14 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, hq = lane >> 5;
-  // XCD x takes a contiguous run of (head, tile): the tiles of a head read the same keys
+  // XCD x takes a contiguous run of (group of heads, tile, head): the tiles of a head read the same keys from its L2, and the heads of a
+  // tile neighbouring parts of its rows. 32760 rows of 40 heads x 128, us with an eighth of the heads in a group against one: 64 keys 134 / 151,
+  // 512 keys 380 / 389, 1024 keys 689 / 694; 64 heads x 64: alike.
   const int in_xcd = blockIdx.x >> 3;
   const int work = (int)(blockIdx.x & 7) * a.per_xcd + in_xcd;
   if (in_xcd >= a.per_xcd || work >= a.tiles * a.heads) return;
-  const int head = work / a.tiles;
+  const int group = work / (a.tiles * a.together), in_group = work - group * (a.tiles * a.together);
+  const int tile = in_group / a.together, head = group * a.together + (in_group - tile * a.together);
 
   // ---- the head's bias over the distances -(sat + 63) .. sat + 63, over the scale: added to the scores before it. Its loads run beside
   // those of the offsets ----
@@ -184,7 +188,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
     }
   }
   int row0, rows, in_request, k0, keys;
-  if (!find_tile<kRows>(a, work - head * a.tiles, row0, rows, in_request, k0, keys)) return;
+  if (!find_tile<kRows>(a, tile, row0, rows, in_request, k0, keys)) return;
 
   const int lrow = lane / kChunks, lslot = lane % kChunks;
   constexpr int kPer = 64 / kChunks;  // rows of a load: four, or at D = 64 eight
@@ -490,6 +494,7 @@ static int launch(PackedAttnArgs a, const BiasArgs& b, hipStream_t stream, const
   WANMI_REQUIRE(tiles * a.heads < (1LL << 24) - 8, WANMI_ERR_ARG, "%s: %lld tiles of rows times %d heads are too many", what, (long long)tiles, a.heads);
   a.tiles = (int)tiles;
   a.per_xcd = (int)per;
+  a.together = a.heads % 8 == 0 ? a.heads / 8 : 1;
   if constexpr (!kBias) {
     if (a.out_scales) {
       hipLaunchKernelGGL((packed_attention_kernel<D, kBias, kSplit, true>), dim3((unsigned)(8 * per)), dim3(256), 0, stream, a, b);
@@ -540,7 +545,7 @@ extern "C" int wanmi_packed_cross_attention(const void* q, int64_t q_ss, int64_t
   using namespace wanmi;
   clear_error();
   PackedAttnArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, q_ss, q_hs, k_ss, k_hs, v_ss, v_hs, q_offsets, k_offsets, (int)requests,
-                   (int)T, (int)Tk, (int)heads, (int)(k_heads > 0 ? heads / k_heads : 1), scale * 1.4426950408889634f, kSlack / (scale * 1.4426950408889634f), 1.0f / scale, out, o_ss, out_scales, zero_rest, 0, 0};
+                   (int)T, (int)Tk, (int)heads, (int)(k_heads > 0 ? heads / k_heads : 1), scale * 1.4426950408889634f, kSlack / (scale * 1.4426950408889634f), 1.0f / scale, out, o_ss, out_scales, zero_rest, 0, 0, 1};
   const int st = check_args(a, T, Tk, requests, heads, k_heads, head_dim, "wanmi_packed_cross_attention");
   if (st != WANMI_OK || T == 0) return st;
   const char* what = "wanmi_packed_cross_attention";
@@ -555,7 +560,7 @@ extern "C" int wanmi_relative_bias_attention(const void* q, int64_t q_ss, int64_
   clear_error();
   const char* what = "wanmi_relative_bias_attention";
   PackedAttnArgs a{(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, q_ss, q_hs, k_ss, k_hs, v_ss, v_hs, offsets, offsets, (int)requests,
-                   (int)T, (int)T, (int)heads, 1, scale * 1.4426950408889634f, kSlack / (scale * 1.4426950408889634f), 1.0f / scale, out, o_ss, nullptr, zero_rest, 0, 0};
+                   (int)T, (int)T, (int)heads, 1, scale * 1.4426950408889634f, kSlack / (scale * 1.4426950408889634f), 1.0f / scale, out, o_ss, nullptr, zero_rest, 0, 0, 1};
   const int st = check_args(a, T, T, requests, heads, heads, head_dim, what);
   if (st != WANMI_OK) return st;
   WANMI_REQUIRE(side >= 1 && side <= kMaxSide && starts, WANMI_ERR_ARG, "%s: %d buckets of one direction, at most %d", what, side, kMaxSide);

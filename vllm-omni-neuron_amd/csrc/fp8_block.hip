@@ -68,27 +68,47 @@ __device__ __forceinline__ uint32_t four_codes(uint32_t p01, uint32_t p23, float
                     quotient(bf16_hi(p23), scale, y));
 }
 
-// A wave takes four blocks of a row, 16 lanes x 8 values each. K is a multiple of 16: a lane's 8 values are all inside or all behind.
-__global__ __launch_bounds__(256) void fp8_block_quantize_kernel(const uint16_t* __restrict__ x, int64_t ldx, int M, int K, int KB,
+// The largest magnitude over 16 lanes: quad permutes, then the half-row and row mirrors, which pair equal quads.
+__device__ __forceinline__ uint32_t max_of_16_lanes(uint32_t best) {
+  best = max_magnitude(best, (uint32_t)dpp_i32<0xB1>((int)best));
+  best = max_magnitude(best, (uint32_t)dpp_i32<0x4E>((int)best));
+  best = max_magnitude(best, (uint32_t)dpp_i32<0x141>((int)best));
+  return max_magnitude(best, (uint32_t)dpp_i32<0x140>((int)best));
+}
+
+// A workgroup takes four blocks of 32 rows, a wave four of the rows with all loads under way together, 16 lanes x 8 values to a block. The
+// scales leave by way of LDS, so that block by block the 32 rows' are one whole line (by itself each is 4 bytes of a line that
+// eight XCDs write to). K is a multiple of 16: a lane's 8 values are all inside or all behind.
+constexpr int kQuantRows = 32, kQuantBlocks = 4;
+__global__ __launch_bounds__(512) void fp8_block_quantize_kernel(const uint16_t* __restrict__ x, int64_t ldx, int M, int K, int KB,
                                                                 uint8_t* __restrict__ codes, float* __restrict__ scales,
                                                                 int64_t s_row, int64_t s_blk) {
-  const int lane = threadIdx.x & 63;
-  const int groups = (KB + 3) / 4;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t m = id / groups;
-  if (m >= M) return;
-  const int b = (int)(id - m * groups) * 4 + (lane >> 4);
-  const int k = b * kBlock + 8 * (lane & 15);
-  u32x4 v = {0u, 0u, 0u, 0u};
-  if (k < K) v = *reinterpret_cast<const u32x4*>(x + m * ldx + k);
-  uint32_t best = 0;
+  constexpr int kOwn = kQuantRows / 8;  // rows of a wave
+  __shared__ float turn[kQuantBlocks][kQuantRows];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int units = (KB + kQuantBlocks - 1) / kQuantBlocks;
+  const int group = (int)blockIdx.x / units, b0 = ((int)blockIdx.x - group * units) * kQuantBlocks;
+  const int64_t m0 = (int64_t)group * kQuantRows;
+  const int row = wave * kOwn, k = (b0 + (lane >> 4)) * kBlock + 8 * (lane & 15);
+  u32x4 v[kOwn];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) best = max_magnitude(best, v[i]);
+  for (int u = 0; u < kOwn; ++u) {
+    v[u] = u32x4{0u, 0u, 0u, 0u};
+    if (k < K && m0 + row + u < M) v[u] = *reinterpret_cast<const u32x4*>(x + (m0 + row + u) * ldx + k);
+  }
 #pragma unroll
-  for (int o = 1; o < 16; o <<= 1) best = max_magnitude(best, (uint32_t)__shfl_xor((int)best, o, 64));
-  const float scale = block_scale(best), y = 1.0f / scale;
-  if (k < K) *reinterpret_cast<uint2*>(codes + m * K + k) = make_uint2(four_codes(v[0], v[1], scale, y), four_codes(v[2], v[3], scale, y));
-  if (b < KB && (lane & 15) == 0) scales[m * s_row + b * s_blk] = scale;
+  for (int u = 0; u < kOwn; ++u) {
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) best = max_magnitude(best, v[u][i]);
+    const float scale = block_scale(max_of_16_lanes(best)), y = 1.0f / scale;
+    if (k < K && m0 + row + u < M)
+      *reinterpret_cast<uint2*>(codes + (m0 + row + u) * K + k) = make_uint2(four_codes(v[u][0], v[u][1], scale, y), four_codes(v[u][2], v[u][3], scale, y));
+    if ((lane & 15) == 0) turn[lane >> 4][row + u] = scale;
+  }
+  __syncthreads();
+  const int b = threadIdx.x / kQuantRows, r = threadIdx.x % kQuantRows;
+  if (b < kQuantBlocks && b0 + b < KB && m0 + r < M) scales[(m0 + r) * s_row + (b0 + b) * s_blk] = turn[b][r];
 }
 
 // scales [M, KB] of any strides -> [KB, M]
@@ -480,12 +500,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void fp8_block_few_kernel(Fp8Arg
         uint32_t best = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) best = max_magnitude(best, x[p][0][e]);
-        // over the 16 lanes: quad permutes, then the half-row and row mirrors, which pair equal quads
-        best = max_magnitude(best, (uint32_t)dpp_i32<0xB1>((int)best));
-        best = max_magnitude(best, (uint32_t)dpp_i32<0x4E>((int)best));
-        best = max_magnitude(best, (uint32_t)dpp_i32<0x141>((int)best));
-        best = max_magnitude(best, (uint32_t)dpp_i32<0x140>((int)best));
-        const float s = block_scale(best), y = 1.0f / s;
+        const float s = block_scale(max_of_16_lanes(best)), y = 1.0f / s;
         const int i = 4 * p + q;
         *reinterpret_cast<uint2*>(&codes[wave][i * kBlock + 8 * c]) = make_uint2(four_codes(x[p][0][0], x[p][0][1], s, y), four_codes(x[p][0][2], x[p][0][3], s, y));
         if (c == 0) scales[wave][i] = s;
@@ -538,8 +553,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void fp8_block_few_kernel(Fp8Arg
 
 static void launch_quantize(const uint16_t* x, int64_t ldx, int M, int K, uint8_t* codes, float* scales, int64_t s_row, int64_t s_blk, hipStream_t st) {
   const int KB = (K + kBlock - 1) / kBlock;
-  const int64_t waves = (int64_t)M * ((KB + 3) / 4);
-  hipLaunchKernelGGL(fp8_block_quantize_kernel, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, x, ldx, M, K, KB, codes, scales, s_row, s_blk);
+  const int64_t wgs = ((int64_t)M + kQuantRows - 1) / kQuantRows * ((KB + kQuantBlocks - 1) / kQuantBlocks);
+  hipLaunchKernelGGL(fp8_block_quantize_kernel, dim3((unsigned)wgs), dim3(512), 0, st, x, ldx, M, K, KB, codes, scales, s_row, s_blk);
 }
 
 template <int kTn, int kTm, int kWn, int kWm, int kRing>

@@ -85,6 +85,19 @@ def test_a_block_of_block_scaled_weights(pkg, dev):
         assert float((up - ref_up).norm() / ref_up.norm()) <= 9.2e-2, kinds.keys()
 
 
+def test_no_text_at_all(pkg, dev):
+    """Every request's text empty, without a row of context: as rows of context that belong to no text."""
+    _, packed, pos, h, temb, _ = _setup(pkg, dev, blocks=1)
+    _, ctx = _texts(dev)
+    none = [0] * len(packed.lengths)
+    for w in _block_weights(pkg, dev):
+        kv = pkg.project_packed_cross_kv(w, ctx[:0], pkg.PackedRequests.from_lengths(none, 0, dev))
+        assert kv.k.shape == kv.v.shape == (0, HEADS, 128)
+        got = pkg.packed_block_forward(w, h, temb, packed, pos, kv)
+        rows = pkg.project_packed_cross_kv(w, ctx, pkg.PackedRequests.from_lengths(none, ctx.shape[0], dev))
+        assert torch.equal(got, pkg.packed_block_forward(w, h, temb, packed, pos, rows))
+
+
 def _encoder(pkg, x, offsets, p):
     """One layer of a text encoder on packed prompts: RMSNorm, attention with a relative position bias, RMSNorm, GELU-gated FFN."""
     norm = lambda t, g: pkg.adaln_kernels.adaln_quant_2d(t, g, None, eps=1e-6, norm_type="rms_norm", quant="none")  # noqa: E731

@@ -93,7 +93,7 @@ BIAS = [
     (dict(table=z(32, H, dtype=torch.float16)), "table"), (dict(table=None, offsets=off().long()), "int32"), (dict(table=z(32, H + 1, dtype=F32)), "table"),
     (dict(table=z(H, 32, dtype=F32).t()), "contiguous"), (dict(table=z(32, dtype=F32)), "table"), (dict(table=z(31, H, dtype=F32)), "buckets"),
     (dict(table=z(2, H, dtype=F32)), "buckets"), (dict(table=z(258, H, dtype=F32), max_distance=1000), "at most 128"), (dict(max_distance=8), "exceed"),
-    (dict(max_distance=0), "exceed"), (dict(max_distance=4000), "at most 1024"), (dict(table=z(1, H, dtype=F32), bidirectional=False), "buckets"), (dict(scale=0.0), "scale"),
+    (dict(max_distance=0), "exceed"), (dict(max_distance=4000), "at most 1024"), (dict(max_distance=10**15), "at most 1024"), (dict(table=z(1, H, dtype=F32), bidirectional=False), "buckets"), (dict(scale=0.0), "scale"),
     (dict(scale=2.0**25), "scale"), (dict(offsets=off(0)), "entry"),
 ]
 

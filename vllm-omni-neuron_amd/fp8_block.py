@@ -121,8 +121,9 @@ def fp8_block_linear(x, weight: FP8BlockWeight, *, activation: str | None = None
 
     ``x``: bf16 ``[..., K]``, quantized on the way as :func:`quantize_fp8_blocks` does it, or an :class:`FP8BlockTensor`. K a multiple of 16, N
     of 8 (the last blocks may be partial). ``activation``: None or ``"gelu"`` (its tanh form). ``out``: bf16 ``[rows, N]`` with rows a
-    multiple of 8 elements apart. Any number of rows: up to 64, what counts is reading the weight once, and up to 16 rows in bf16 are
-    quantized inside the one launch."""
+    multiple of 8 elements apart. Any number of rows. Up to 16 of them take one launch that reads the weight once at the memory's
+    rate, up to 4 in bf16 are quantized inside it; more in bf16 take a launch for that and a workspace for the codes, and middling
+    sizes, whose tiles would not fill the chip, share out the sum and add its parts in another. Inference only: no gradient."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}")
     y = _linear_plain(x, weight, _ACTIVATIONS[activation]) if out is None else None

@@ -38,9 +38,9 @@ def _bucket_starts(buckets: int, max_distance: int, bidirectional: bool):
     for i in range(steps):
         while n**steps * first**i < max_distance**i * first**steps:
             n += 1
+            if n > _MAX_SATURATION:
+                raise ValueError(f"bucket {first + i} of {side} up to distance {max_distance} starts behind {_MAX_SATURATION}: at most {_MAX_SATURATION}")
         starts.append(n)
-    if starts[-1] > _MAX_SATURATION:
-        raise ValueError(f"the last bucket of {side} up to {max_distance} starts at {starts[-1]}: at most {_MAX_SATURATION}")
     return (ctypes.c_int * side)(*starts)
 
 
@@ -134,7 +134,7 @@ def packed_cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_
     The rows of a request without keys are zeros. Rows behind the last request are zeros too in an output allocated here and
     left as they are in a given ``out``, which may be ``q``. Offsets are held inside the tensors: wrong ones give wrong
     rows, and no access out of bounds. The softmax has a running maximum (no bound on scores is needed) and fp32 sums; its weights enter the
-    second product as bf16.
+    second product as bf16. Inference only: no gradient.
     """
     if out is None and quant == "none":
         plain = _plain(q, k, v, scale)

@@ -136,7 +136,8 @@ def project_packed_cross_kv(w: BlockWeights, context: torch.Tensor, text: Packed
             parts.append(mxfp8_linear(mx, weight))
     k, v = parts
     ops.qk_rmsnorm_rope_(k, w.norm_k2, eps=eps)
-    return PackedCrossKV(k.view(text.rows, -1, HEAD_DIM), v.view(text.rows, -1, HEAD_DIM), text.offsets)
+    heads = k.shape[1] // HEAD_DIM
+    return PackedCrossKV(k.view(text.rows, heads, HEAD_DIM), v.view(text.rows, heads, HEAD_DIM), text.offsets)
 
 
 def _quant(weight) -> str:

@@ -39,7 +39,7 @@ def test_quantize(pkg, dev, M, K):
 
 
 SIZES = [(1, 16, 8), (1, 5120, 640), (3, 128, 128), (16, 400, 264), (17, 1024, 72), (33, 2064, 136), (64, 640, 256), (65, 256, 64), (100, 1552, 200),
-         (129, 640, 1000), (300, 144, 5120), (700, 1024, 2048), (2000, 528, 5000), (4100, 256, 4360), (4000, 400, 8192)]
+         (129, 640, 1000), (300, 144, 5120), (700, 1024, 2048), (2000, 528, 5000), (4100, 256, 4360), (4000, 400, 8192), (1000, 1040, 5120), (2100, 1040, 8200)]
 
 
 @pytest.mark.parametrize("M,K,N", SIZES)

@@ -4,6 +4,8 @@ block-scaled weights, their keys and values for a block, and the block's cross-a
 The block's bars are those of the packed blocks against single ones: what is quantized behind an attention that rounds in
 another order is off by (2^-8 2^-3)^(1/2) of itself, the square root of the blocks as often."""
 
+import sys
+
 import pytest
 import torch
 
@@ -20,8 +22,11 @@ def _texts(dev, lens=(20, 33, 0, 59), pad=5, seed=4):
     return lens, ctx
 
 
-def test_packed_texts_give_what_each_text_gives_alone(pkg, dev):
-    """packed_dit_forward with the texts packed, against one cross-attention per request, whose text is never empty."""
+@pytest.mark.parametrize("together", [True, False])
+def test_packed_texts_give_what_each_text_gives_alone(pkg, dev, together, monkeypatch):
+    """packed_dit_forward with the texts packed, against one cross-attention per request, whose text is never empty. Self-attention
+    all together as for short requests, or request by request as for long ones."""
+    monkeypatch.setattr(sys.modules[pkg.PackedRequests.__module__], "_TOGETHER", 3600 if together else 0)
     ws, packed, pos, h, temb, _ = _setup(pkg, dev)
     lens, ctx = _texts(dev, (20, 33, 7, 59))
     text = pkg.PackedRequests.from_lengths(lens, ctx.shape[0], dev)

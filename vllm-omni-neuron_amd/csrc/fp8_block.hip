@@ -351,7 +351,7 @@ __global__ __launch_bounds__(64 * kWn * kWm, 2) void fp8_block_gemm_kernel(Fp8Ar
 #pragma unroll
       for (int r = 0; r < 4; ++r) acc[kFn - 1][j][r] = fmaf(p[j][r], s[j], acc[kFn - 1][j][r]);
 
-    if constexpr (kRing > 2) __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // the bias: the waits of a short sum may not have reached it
+    if constexpr (kRing > 2) wait_vm<0>();  // the bias: the waits of a short sum may not have reached it
     // ---- epilogue: lane holds features nw + 16 i + 4 q .. + 3 of row mw + 16 j + c. Sixteen rows at a time are staged in the wave's LDS
     // and stored whole, past L2: they are written once and read by the next kernel ----
     if (kRing > 2 && g.splits > 1) {

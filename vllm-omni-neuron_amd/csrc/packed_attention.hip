@@ -246,12 +246,12 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
 
   // ---- the queries as MFMA operands: lane holds d = 16 t + 8 hq .. + 7 of query col ----
   // (with the first tile, which is waited for here and not at the top of the loop)
-  __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+  wait_vm<0>();
   if (kOwn || kBias) __syncthreads();
   bf16x8 qf[D / 16];
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) qf[t] = *reinterpret_cast<const bf16x8*>(sq + col * kRowB + (((2 * t + hq) ^ k_slot<D>(col)) << 4));
-  __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0));  // (read before the second tile may come)
+  wait_lgkm();  // (read before the second tile may come)
   [[maybe_unused]] float far_lo = 0.0f, far_hi = 0.0f;
   if constexpr (kBias) {
     far_lo = sbias[0];
@@ -271,13 +271,13 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
 
   for (int t = 0; t < tiles; ++t) {
     if constexpr (!kOwn) {
-      __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+      wait_vm<0>();
       __syncthreads();  // the tile is in LDS, and every wave is done with the one before it
       if (t + 1 < tiles) load_tile(t + 1);
     } else if (t + 1 < tiles) {
-      __builtin_amdgcn_s_waitcnt(waitcnt_vm(2 * kLoads));  // the next tile's may be under way
+      wait_vm<2 * kLoads>();  // the next tile's may be under way
     } else {
-      __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+      wait_vm<0>();
     }
     const uint8_t* tk = ring + (t % kRing) * 2 * kTile;
     const uint8_t* tv = tk + kTile;
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
       }
     }
     if (kOwn && t + 2 < tiles) {
-      __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0));  // the wave has read its tile
+      wait_lgkm();  // the wave has read its tile
       load_tile(t + 2);
     }
   }

@@ -204,6 +204,16 @@ __device__ __forceinline__ float rsqrt_f32(float x) {
 // s_waitcnt immediates (gfx9 encoding: vmcnt[3:0] | expcnt[6:4] | lgkmcnt[11:8] | vmcnt[5:4] << 14)
 constexpr int waitcnt_vm(int n) { return (n & 0xF) | (0x7 << 4) | (0xF << 8) | ((n >> 4) << 14); }
 constexpr int waitcnt_lgkm(int n) { return 0xF | (0x7 << 4) | ((n & 0xF) << 8) | (0x3 << 14); }
+// Waits that the compiler moves no memory access across: for LDS that a load straight into it fills, read without a barrier in between.
+template <int kCount>
+__device__ __forceinline__ void wait_vm() {
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(kCount));
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void wait_lgkm() {
+  __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0));
+  asm volatile("" ::: "memory");
+}
 
 // Wavefront (64-lane) reductions via cross-lane shuffles.
 __device__ __forceinline__ int wave_max_i32(int v) {

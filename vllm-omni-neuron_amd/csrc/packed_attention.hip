@@ -37,7 +37,6 @@ constexpr int kMaxSide = 128;         // bias buckets of one direction
 constexpr int kMaxSaturation = 1024;  // the distance from which on a direction's last bucket holds
 constexpr float kSlack = 8.0f;        // log2 units
 constexpr float kBiasMax = 1e30f;     // of a finite bias, in units of the scores before their scale: beyond, scores vanish beside it
-constexpr float kBiasFold = 8192.0f;  // up to here a bias that a whole half shares is taken off its maximum instead
 
 struct PackedAttnArgs {
   const uint16_t* q;  // row i, head h at q + i * q_ss + h * q_hs
@@ -252,11 +251,6 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) qf[t] = *reinterpret_cast<const bf16x8*>(sq + col * kRowB + (((2 * t + hq) ^ k_slot<D>(col)) << 4));
   wait_lgkm();  // (read before the second tile may come)
-  [[maybe_unused]] float far_lo = 0.0f, far_hi = 0.0f;
-  if constexpr (kBias) {
-    far_lo = sbias[0];
-    far_hi = sbias[2 * (sat + 63)];
-  }
 
   f32x16 acc[D / 32];
 #pragma unroll
@@ -288,34 +282,21 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
     for (int i = 0; i < kHalves; ++i) {
       const int key = 32 * i + col;
       const uint8_t* row = tk + key * kRowB;
+      // register r of half i: key 32 i + 8 (r >> 2) + 4 hq + (r & 3). The products are added to the bias; where all of the half's distances
+      // are beyond the last bucket's first they are all alike, and read from the table's end
+      if constexpr (kBias) {
+        const int d0 = tile_at(t) * kKeys + 32 * i - (in_request + qw);  // first key - first query
+        const float* pb = sbias + (sat + 63 + min(max(d0, -(sat + 32)), sat + 32) + 4 * hq - col);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[i][r] = 0.0f;
+        for (int r = 0; r < 16; ++r) s[i][r] = pb[8 * (r >> 2) + (r & 3)];
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[i][r] = 0.0f;
+      }
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
         const bf16x8 kf = *reinterpret_cast<const bf16x8*>(row + (((2 * d + hq) ^ k_slot<D>(key)) << 4));
         s[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[d], s[i], 0, 0, 0);
-      }
-    }
-    // register r of half i: key 32 i + 8 (r >> 2) + 4 hq + (r & 3)
-    float shared[kHalves];  // a bias of the whole half
-#pragma unroll
-    for (int i = 0; i < kHalves; ++i) {
-      shared[i] = 0.0f;
-      if constexpr (kBias) {
-        const int d0 = tile_at(t) * kKeys + 32 * i - (in_request + qw);  // first key - first query
-        const float far = d0 > 0 ? far_hi : far_lo;
-        if (d0 - 31 < sat && d0 + 31 > -sat) {
-          asm volatile("");  // (a branch: not both sides computed and one selected)
-          const float* pb = sbias + (sat + 63 + d0 + 4 * hq - col);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[i][r] += pb[8 * (r >> 2) + (r & 3)];
-        } else if (fabsf(far) > kBiasFold) {
-          asm volatile("");
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[i][r] += far;
-        } else {
-          shared[i] = far;
-        }
       }
     }
     if (left < 32 * kHalves) {
@@ -333,7 +314,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
       float h = s[i][0];
 #pragma unroll
       for (int r = 1; r < 16; ++r) h = fmaxf(h, s[i][r]);
-      mx = fmaxf(mx, kBias ? h + shared[i] : h);
+      mx = fmaxf(mx, h);
     }
     mx = max_lane_xor32(mx);
     if (__any(mx > m + a.slack)) {
@@ -348,10 +329,9 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
           for (int r = 0; r < 16; ++r) acc[i][r] *= f;
       }
     }
-    const float base = m == -INFINITY ? 0.0f : m;  // no key above -inf yet: every P is 0
+    const float off = m == -INFINITY ? 0.0f : -m * c;  // no key above -inf yet: every P is 0
 #pragma unroll
     for (int i = 0; i < kHalves; ++i) {
-      const float off = kBias ? (shared[i] - base) * c : -base * c;
       bf16x8 pf[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {

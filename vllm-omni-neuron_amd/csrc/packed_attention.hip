@@ -59,6 +59,9 @@ struct PackedAttnArgs {
   int together;         // heads that take the same tile one after the other; divides heads
 };
 
+// Distances of a head's bias in LDS: -(sat + 63) .. sat + 63.
+__host__ __device__ constexpr int bias_entries(int sat) { return 2 * (sat + 63) + 1; }
+
 struct BiasArgs {
   const void* table;  // [buckets, heads], fp32 or bf16
   int bf16;
@@ -166,10 +169,9 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
   constexpr int kRingB = kRing * 2 * kTile * (kOwn ? 4 : 1);
   constexpr int kJoin = kOwn ? kSplit * 32 * (D * 4 + 8) : 0;
   constexpr int kLds = kRingB > kJoin ? kRingB : kJoin;
-  constexpr int kBiasLds = kBias ? 2 * (kMaxSaturation + 63) + 2 : 1;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
   __shared__ __attribute__((aligned(1024))) uint8_t squery[kOwn ? 32 * kRowB : 16];
-  __shared__ float sbias[kBiasLds];
+  extern __shared__ float sbias[];  // bias_entries(sat): mostly few, and with room for the most a CU of D = 64 would hold three workgroups instead of four
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, hq = lane >> 5;
@@ -186,7 +188,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
   // those of the offsets ----
   [[maybe_unused]] const int sat = bias.sat;
   if constexpr (kBias) {
-    for (int i = threadIdx.x; i < 2 * (sat + 63) + 1; i += 256) {
+    for (int i = threadIdx.x; i < bias_entries(sat); i += 256) {
       const int d = i - (sat + 63);
       int b = bias.bucket[min(abs(d), sat)];
       if (d > 0) b = bias.both ? b + bias.side : 0;
@@ -491,7 +493,7 @@ static int launch(PackedAttnArgs a, const BiasArgs& b, hipStream_t stream, const
       return check_launch(what);
     }
   }
-  hipLaunchKernelGGL((packed_attention_kernel<D, kBias, kSplit, false>), dim3((unsigned)(8 * per)), dim3(256), 0, stream, a, b);
+  hipLaunchKernelGGL((packed_attention_kernel<D, kBias, kSplit, false>), dim3((unsigned)(8 * per)), dim3(256), kBias ? bias_entries(b.sat) * sizeof(float) : 0, stream, a, b);
   return check_launch(what);
 }
 

@@ -154,6 +154,13 @@ __device__ __forceinline__ int mx_codes(const uint32_t (&pp)[8], uint32_t (&code
   return sx;
 }
 
+// LDS of a workgroup without its bias: the ring of tiles; kSplit 4: the waves' rings, or the parts that are joined.
+template <int D, int kSplit>
+constexpr int ring_bytes() {
+  constexpr int kRing = 2 * 2 * (kSplit == 4 ? 4 * 32 : 64) * 2 * D, kJoin = kSplit == 4 ? kSplit * 32 * (D * 4 + 8) : 0;
+  return kRing > kJoin ? kRing : kJoin;
+}
+
 template <int D, bool kBias, int kSplit, bool kMx>
 __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs a, BiasArgs bias) {
   constexpr int kRows = 128 / kSplit;              // rows of a workgroup
@@ -166,12 +173,12 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
   constexpr int kTile = kKeys * kRowB;             // of K, and as much of V
   constexpr int kLoads = kTile / (kOwn ? 1024 : 4096);  // per wave, of each
   constexpr int kRing = 2;
-  constexpr int kRingB = kRing * 2 * kTile * (kOwn ? 4 : 1);
-  constexpr int kJoin = kOwn ? kSplit * 32 * (D * 4 + 8) : 0;
-  constexpr int kLds = kRingB > kJoin ? kRingB : kJoin;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
+  static_assert(kRing * 2 * kTile * (kOwn ? 4 : 1) <= ring_bytes<D, kSplit>(), "the ring");
+  // (not of a size that the compiler knows: with one workgroup a CU it would take accumulation registers for the products, and copy
+  // scores and outputs from and to them; a head's bias behind it, for as many distances as its table tells apart)
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  [[maybe_unused]] float* sbias = reinterpret_cast<float*>(lds + ring_bytes<D, kSplit>());
   __shared__ __attribute__((aligned(1024))) uint8_t squery[kOwn ? 32 * kRowB : 16];
-  extern __shared__ float sbias[];  // bias_entries(sat): mostly few, and with room for the most a CU of D = 64 would hold three workgroups instead of four
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, hq = lane >> 5;
@@ -487,13 +494,14 @@ static int launch(PackedAttnArgs a, const BiasArgs& b, hipStream_t stream, const
   a.tiles = (int)tiles;
   a.per_xcd = (int)per;
   a.together = a.heads % 8 == 0 ? a.heads / 8 : 1;
+  const unsigned lds = ring_bytes<D, kSplit>() + (kBias ? (unsigned)(bias_entries(b.sat) * sizeof(float)) : 0u);
   if constexpr (!kBias) {
     if (a.out_scales) {
-      hipLaunchKernelGGL((packed_attention_kernel<D, kBias, kSplit, true>), dim3((unsigned)(8 * per)), dim3(256), 0, stream, a, b);
+      hipLaunchKernelGGL((packed_attention_kernel<D, kBias, kSplit, true>), dim3((unsigned)(8 * per)), dim3(256), lds, stream, a, b);
       return check_launch(what);
     }
   }
-  hipLaunchKernelGGL((packed_attention_kernel<D, kBias, kSplit, false>), dim3((unsigned)(8 * per)), dim3(256), kBias ? bias_entries(b.sat) * sizeof(float) : 0, stream, a, b);
+  hipLaunchKernelGGL((packed_attention_kernel<D, kBias, kSplit, false>), dim3((unsigned)(8 * per)), dim3(256), lds, stream, a, b);
   return check_launch(what);
 }
 

@@ -13,7 +13,7 @@
 // that the last bit of the scale decides many codes: the product with the rounded reciprocal is what torch computes on the GPU for `/ 448`.)
 //
 // Measured: 32760 x 15360 x 5120 from codes 2.15 ms, 2.4 PFLOP/s (a library's product of 8192^3 such codes with one scale reaches 3.0); the matrix
-// pipe is busy 65% of the cycles, at 1.75 GHz, which the chip's power sets. 7799 x 5120 x 13824 from bf16 556 us, of which 53 quantize;
+// pipe is busy 65% of the cycles, at 1.75 GHz, which the chip's power sets. 7799 x 5120 x 13824 from bf16 556 to 563 us, of which 53 quantize;
 // 1560 x 13824 x 5120 136, of which 7; 333 x 5096 x 4112 26, in three launches of 4.8, 20.9 and 4.2.
 #include "wanmi_common.h"
 #include "fp8_plan.h"
@@ -127,8 +127,8 @@ __global__ __launch_bounds__(256) void fp8_scales_kernel(const float* __restrict
 // Many rows: tiles of kTn features x kTm rows, both operands through LDS in stages of 128 along k. The matrix pipe and the chip's power bound the
 // 256 x 256 tiles: 32760 x 15360 x 5120 took 2912 us with the multiply-adds where the compiler put them, 2380 in the order below, 2322 without
 // bank conflicts, 2150 with workgroups that stay and addresses in scalar registers. A full round of 256 tiles costs 1.87 us a stage, one
-// of 122 tiles 1.25: cutting the last round's tiles in parts of their sums or in halves gained nothing. What bounds the smaller tiles is the
-// 40 to 55 KB/us that a CU streams (fp8_plan.h).
+// of 122 tiles 1.25: cutting the last round's tiles in parts of their sums or in halves gained nothing. The smaller tiles are
+// bound by LDS (128 x 128: 96 KB read and 32 written a stage, 1024 of 1340 cycles) and the stage's barrier.
 // ------------------------------------------------------------------------------------------------
 // 16-byte chunk c of row r lies in slot c ^ f(r) of its 128 bytes. One cycle of a 16-byte read serves lanes 0-3, 12-15 and 20-27 (or the others
 // of 32): all sixteen rows of a fragment, chunk q of rows 0-3 and 12-15 and chunk q ^ 1 of rows 4-11. Two rows share the 64 banks, so

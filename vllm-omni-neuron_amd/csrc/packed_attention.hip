@@ -19,11 +19,11 @@
 // 2^8 instead of 1, which costs bf16 and fp32 no precision, and nearly every tile after the first goes without a rescale.
 //
 // What bounds it: with many rows, a SIMD's matrix pipe and its VALU one after the other. 32760 rows of 40 heads x 128 over 512 and fewer keys
-// (251 GFLOP, 687 MB) take 327 us (770 TFLOP/s): the matrix pipe is busy 39% of the cycles, the VALU 42%, LDS 24%, without bank conflicts. A score
+// (251 GFLOP, 687 MB) take 325 us (770 TFLOP/s): the matrix pipe is busy 39% of the cycles, the VALU 42%, LDS 24%, without bank conflicts. A score
 // of 64 lanes costs the VALU 18 cycles (2^x 8.4, the multiply-add before it 2.7, conversion, sum and maximum 2.3 each) beside 32
 // of MFMA at D = 128 and 16 at D = 64. 64 keys more cost 37 us there (1160 TFLOP/s), the rows themselves 105 (q and o, 671 MB); 1024 keys
-// reach 1000 TFLOP/s, at 64 heads x 64 with 2048 keys 880. With few rows it is the chain of launch, offsets, first tile and join: 16 rows of
-// 40 heads over 512 keys 9.5 us for 11 MB.
+// reach 1000 TFLOP/s, at 64 heads x 64 with 2048 keys 880; prompts of 6001 tokens with a bias there (159 GFLOP) 202 us. With few rows it is the
+// chain of launch, offsets, the tiles that one CU loads, and join: 16 rows of 40 heads over 512 keys 9.3 us for 11 MB.
 // What did not help (512 keys, 380 us): scores of a tile beside the softmax of the one before (443), workgroups that stay and load
 // ahead for their next tile of rows (448), three workgroups a CU with tiles of 32 keys (386), half of the first workgroups held back or wave
 // priorities (within 1%).

@@ -132,11 +132,11 @@ def test_given_outputs_and_layouts(pkg, dev, T):
     assert torch.equal(again[: T - 3], bias[: T - 3]) and torch.equal(again[T - 3 :], q[T - 3 :])
 
 
-@pytest.mark.parametrize("T,H", [(4, 2), (200, 2), (200, 40)])
-def test_scores_at_the_ends_of_their_range(pkg, dev, T, H):
+@pytest.mark.parametrize("T,H,D", [(4, 2, 128), (200, 2, 128), (200, 40, 128), (4, 2, 64), (200, 90, 64)])
+def test_scores_at_the_ends_of_their_range(pkg, dev, T, H, D):
     """A maximum that rises with every tile, scores of ten thousand, of minus infinity and of NaN."""
     g = torch.Generator().manual_seed(T)
-    D, m = 128, 300
+    m = 300
     q = torch.rand(T, H, D, generator=g).add(0.5).to(BF16)
     k = torch.randn(m, H, D, generator=g).to(BF16)
     v = torch.randn(m, H, D, generator=g).to(BF16)

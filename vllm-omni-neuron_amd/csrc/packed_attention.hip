@@ -37,6 +37,10 @@ constexpr int kMaxSide = 128;         // bias buckets of one direction
 constexpr int kMaxSaturation = 1024;  // the distance from which on a direction's last bucket holds
 constexpr float kSlack = 8.0f;        // log2 units
 constexpr float kBiasMax = 1e30f;     // of a finite bias, in units of the scores before their scale: beyond, scores vanish beside it
+// A weight is 2^(s c - m c), by one multiply-add with the rounded m c. The rounding is up to 2^-24 of it: the same for all keys under one m, but not for
+// tiles or waves with another, and where |m c| reaches 2^31 (scores in the thousands of millions; a row of nothing but a mask's lowest value) the rounding alone
+// leaves the range of 2^x. Beyond this |m c|, where it is 2^-10 log2 units, m is subtracted from a row's scores instead, which is exact near the maximum.
+constexpr float kFar = 16384.0f;
 
 struct PackedAttnArgs {
   const uint16_t* q;  // row i, head h at q + i * q_ss + h * q_hs
@@ -267,6 +271,8 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
   float m = -INFINITY, sum = 0.0f;  // m in units of the scores before their scale
+  float off = 0.0f;                 // -m c, rounded; 0 where there is no key above -inf yet (every P is 0), and where m is subtracted from the scores
+  bool far = false, any_far = false;
   // (in a vector register: a multiply-add that reads a scalar one takes 4.5 cycles in place of 2.7)
   float c = a.scale_log2;
   asm volatile("" : "+v"(c));
@@ -329,6 +335,10 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
       const float mn = fmaxf(m, mx);
       const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
       m = mn;
+      off = m == -INFINITY ? 0.0f : -m * c;  // no key above -inf yet: every P is 0
+      far = fabsf(off) > kFar;
+      any_far = __any(far);
+      if (far) off = 0.0f;
       if (t > 0) {  // (before, there is nothing to rescale)
         sum *= f;
 #pragma unroll
@@ -337,7 +347,14 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
           for (int r = 0; r < 16; ++r) acc[i][r] *= f;
       }
     }
-    const float off = m == -INFINITY ? 0.0f : -m * c;  // no key above -inf yet: every P is 0
+    if (any_far) {
+      asm volatile("");
+      const float from = far ? m : 0.0f;
+#pragma unroll
+      for (int i = 0; i < kHalves; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[i][r] -= from;
+    }
 #pragma unroll
     for (int i = 0; i < kHalves; ++i) {
       bf16x8 pf[2];

@@ -80,3 +80,62 @@ def test_one_key_above_all(pkg, dev, T, H, D):
         got = pkg.packed_cross_attention(q.to(dev), k.to(dev), v.to(dev), ref.offsets([T], dev), ref.offsets([m], dev), scale=1.0)
         want = v[at].double().mean(0)
         _close(got, want.expand(T, H, D), (want.abs() * 2.0**-8).expand(T, H, D))
+
+
+@pytest.mark.parametrize("T,H,k_heads,D,m", [(1, 2, 2, 128, 512), (3, 4, 2, 64, 300), (16, 8, 8, 128, 500), (200, 40, 40, 128, 512), (200, 90, 30, 64, 333), (129, 2, 1, 128, 65)])
+def test_a_mean_of_equal_values_is_that_value(pkg, dev, T, H, k_heads, D, m):
+    """Every key has the same v, so that the weights do not matter as long as their sum is that of the weights which multiply v: product and
+    sum are then off by fp32's rounding of ``m`` additions alone, 512 2^-24 = 2^-15, far less than the half step of 2^-9 at which v, a bf16
+    number, would be rounded to another. Scores that rise by up to 2^8 from tile to tile (a maximum that is held), and that fall."""
+    g = torch.Generator().manual_seed(m)
+    q = torch.rand(T, H, D, generator=g).add(0.5).to(BF16)
+    v = torch.randn(1, k_heads, D, generator=g).to(BF16).expand(m, k_heads, D).contiguous()
+    noise = 0.1 * torch.randn(m, k_heads, D, generator=g)
+    for slope in (0.0, 0.02, 0.04, -0.04, 0.5):
+        k = (noise + torch.linspace(0, slope, m)[:, None, None]).to(BF16)
+        got = pkg.packed_cross_attention(q.to(dev), k.to(dev), v.to(dev), ref.offsets([T], dev), ref.offsets([m], dev), scale=1.0).cpu()
+        assert torch.equal(got, v[0].repeat_interleave(H // k_heads, 0).expand(T, H, D)), (slope, int((got != v[0].repeat_interleave(H // k_heads, 0)).sum()))
+        if k_heads == H:
+            n = min(T, m)
+            table = torch.randn(32, H, generator=g).to(dev)
+            got = pkg.relative_bias_attention(q[:n].to(dev), k[:n].to(dev), v[:n].to(dev), table, ref.offsets([n], dev)).cpu()
+            assert torch.equal(got, v[:n]), slope
+
+
+@pytest.mark.parametrize("T,H,D", [(8, 8, 128), (200, 40, 128), (200, 90, 64)])
+@pytest.mark.parametrize("mean", [0.0, 4.0])
+def test_the_error_is_that_of_rounded_weights(pkg, dev, T, H, D, mean):
+    """The root mean square over all outputs. A weight p_j is rounded to bf16 by at most 2^-8 of itself, uniformly at worst: a mean square of
+    2^-16 / 3 of p_j^2; the sum has the same rounded weights, so that the output is off by sum_j p_j d_j (v_j - o): 2^-16 / 3 of
+    sum_j p_j^2 (v_j - o)^2. The output's own rounding is 2^-16 / 3 of o^2 at most. What fp32 leaves is below 2^-13 of sum_j p_j |v_j|. A mean of all values
+    moves o and its rounding, and the first term not at all."""
+    m = 300
+    g = torch.Generator().manual_seed(T + D)
+    q = torch.randn(T, H, D, generator=g).mul(2).to(BF16)
+    k = torch.randn(m, H, D, generator=g).to(BF16)
+    v = (torch.randn(m, H, D, generator=g) + mean).to(BF16)
+    got = pkg.packed_cross_attention(q.to(dev), k.to(dev), v.to(dev), ref.offsets([T], dev), ref.offsets([m], dev)).double().cpu()
+    p = torch.softmax((q.double().transpose(0, 1) @ k.double().permute(1, 2, 0)) * D**-0.5, -1)  # [H, T, m]
+    vd = v.double().transpose(0, 1)
+    o = p @ vd
+    p2 = p.square()
+    spread = (p2 @ vd.square() - 2 * o * (p2 @ vd) + o.square() * p2.sum(-1, keepdim=True)).clamp_min(0)
+    bar = (2.0**-16 / 3 * (spread + o.square())).sqrt() + 2.0**-13 * (p @ vd.abs())
+    err = got.transpose(0, 1) - o
+    assert float(err.square().mean().sqrt()) <= float(bar.square().mean().sqrt())
+
+
+@pytest.mark.parametrize("T,H,D", [(3, 2, 64), (16, 8, 128), (200, 40, 128), (200, 90, 64)])
+def test_late_keys_that_dominate_within_the_held_maximum(pkg, dev, T, H, D):
+    """The first keys (a tile of any kind) score 0, all later ones the same 2^x with x from 0.01 to 5.5 in steps: their weights round alike, by
+    up to 2^-8, which only a sum of the same rounded weights takes out again. All have the same v, which has to come out."""
+    m = 512
+    g = torch.Generator().manual_seed(D)
+    q = torch.zeros(T, H, D, dtype=BF16)
+    q[..., 3] = 1
+    v = torch.randn(1, H, D, generator=g).to(BF16).expand(m, H, D).contiguous()
+    for i in range(24):
+        k = torch.zeros(m, H, D, dtype=BF16)
+        k[128:, :, 3] = 0.01 + 0.23 * i
+        got = pkg.packed_cross_attention(q.to(dev), k.to(dev), v.to(dev), ref.offsets([T], dev), ref.offsets([m], dev), scale=1.0).cpu()
+        assert torch.equal(got, v[:1].expand(T, H, D)), i

@@ -20,7 +20,7 @@
 //
 // What bounds it: with many rows, a SIMD's matrix pipe and its VALU one after the other. 32760 rows of 40 heads x 128 over 512 and fewer keys
 // (251 GFLOP, 687 MB) take 325 us (770 TFLOP/s): the matrix pipe is busy 39% of the cycles, the VALU 42%, LDS 24%, without bank conflicts. A score
-// of 64 lanes costs the VALU 18 cycles (2^x 8.4, the multiply-add before it 2.7, conversion, sum and maximum 2.3 to 2.5 each) beside 32
+// of 64 lanes costs the VALU 18 cycles (2^x 8.4, the multiply-add before it 2.7, conversion, sum and maximum 2.3 each) beside 32
 // of MFMA at D = 128 and 16 at D = 64. 64 keys more cost 37 us there (1160 TFLOP/s), the rows themselves 105 (q and o, 671 MB); 1024 keys
 // reach 1000 TFLOP/s, at 64 heads x 64 with 2048 keys 880; prompts of 6001 tokens with a bias there (159 GFLOP) 202 us. With few rows it is the
 // chain of launch, offsets, the tiles that one CU loads, and join: 16 rows of 40 heads over 512 keys 9.3 us for 11 MB.
@@ -276,6 +276,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
   // (in a vector register: a multiply-add that reads a scalar one takes 4.5 cycles in place of 2.7)
   float c = a.scale_log2;
   asm volatile("" : "+v"(c));
+  const bf16x2_t ones = {(__bf16)1.0f, (__bf16)1.0f};
 
   for (int t = 0; t < tiles; ++t) {
     if constexpr (!kOwn) {
@@ -366,7 +367,9 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
           const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i][8 * u + 2 * j], c, off));
           const float p1 = __builtin_amdgcn_exp2f(fmaf(s[i][8 * u + 2 * j + 1], c, off));
           w[j] = pack_bf16x2(p0, p1);
-          sum += p0 + p1;  // (a dot product of the pair with ones, one instruction, stands in the way of other waves' MFMAs)
+          // The rounded weights, those that multiply V: their rounding, up to 2^-8 each and the same for keys of one score, then leaves a mean of equal values as
+          // it is. One instruction a pair (by shifts and additions: 1024 keys 703 us in place of 687, prompts of 6001 tokens 203 in place of 194).
+          sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w[j]), ones, sum, false);
         }
         pf[u] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
       }

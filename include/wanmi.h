@@ -431,7 +431,8 @@ int64_t wanmi_lora_workspace(int64_t T, int64_t K, int parts, int rank);
  * [k_offsets[r], k_offsets[r + 1]), request by request, in one launch:
  *   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - max)          (no keys: zeros)
  * q: bf16, element (i, h, d) at i * q_ss + h * q_hs + d; k, v likewise with k_heads heads (heads a multiple of k_heads, query
- * head h reads key head h / (heads / k_heads)); strides multiples of 8 below 2^22, 16-byte aligned tensors. head_dim 64 or 128.
+ * head h reads key head h / (heads / k_heads)); strides multiples of 8, of rows below 2^22, of heads 2^40; 16-byte aligned
+ * tensors. head_dim 64 or 128.
  * q_offsets, k_offsets: int32 [requests + 1] on the device, ascending from 0, held inside [0, T] and [0, Tk] (below 2^28).
  * out: bf16 [T, heads * head_dim], rows o_ss elements apart (a multiple of 16), may be q element for element; with out_scales (uint8
  * [T, heads * head_dim / 32]) e4m3fn codes and e8m0 scales as wanmi_mxfp8_gemm reads them. Rows behind the last request

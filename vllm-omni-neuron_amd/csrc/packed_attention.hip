@@ -543,9 +543,12 @@ static int check_args(const PackedAttnArgs& a, int64_t T, int64_t Tk, int64_t re
   WANMI_REQUIRE(requests >= 0 && requests < (1 << 20), WANMI_ERR_ARG, "%s: %lld requests: at most 2^20 - 1", what, (long long)requests);
   WANMI_REQUIRE(heads > 0 && k_heads > 0 && heads % k_heads == 0 && heads <= 1024, WANMI_ERR_ARG, "%s: %lld heads (at most 1024) over %lld key heads", what, (long long)heads, (long long)k_heads);
   WANMI_REQUIRE(a.inv_scale >= 0x1p-24f && a.inv_scale <= 0x1p64f, WANMI_ERR_ARG, "%s: the scale must be in 2^-64 .. 2^24", what);
-  const int64_t strides[6] = {a.q_ss, a.q_hs, a.k_ss, a.k_hs, a.v_ss, a.v_hs};
-  for (int64_t s : strides)
-    WANMI_REQUIRE(s >= 0 && s % 8 == 0 && s < (1 << 22), WANMI_ERR_ARG, "%s: stride %lld must be a multiple of 8 below 2^22", what, (long long)s);
+  // (rows enter the 24-bit products and 32-bit offsets of a tile; heads only 64-bit addresses)
+  const int64_t rows[3] = {a.q_ss, a.k_ss, a.v_ss}, head[3] = {a.q_hs, a.k_hs, a.v_hs};
+  for (int i = 0; i < 3; ++i) {
+    WANMI_REQUIRE(rows[i] >= 0 && rows[i] % 8 == 0 && rows[i] < (1 << 22), WANMI_ERR_ARG, "%s: row stride %lld must be a multiple of 8 below 2^22", what, (long long)rows[i]);
+    WANMI_REQUIRE(head[i] >= 0 && head[i] % 8 == 0 && head[i] < (1LL << 40), WANMI_ERR_ARG, "%s: head stride %lld must be a multiple of 8 below 2^40", what, (long long)head[i]);
+  }
   if (T == 0) return WANMI_OK;
   WANMI_REQUIRE(a.q && a.out && a.q_off && a.k_off && (Tk == 0 || (a.k && a.v)), WANMI_ERR_ARG, "%s: null pointer", what);
   WANMI_REQUIRE(((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) % 16 == 0, WANMI_ERR_ARG, "%s: q, k, v and out must be 16-byte aligned", what);

@@ -42,15 +42,30 @@ from .packed_attention import packed_cross_attention
 from .row_mx_kernels import mxfp8_linear
 
 
-class PackedRequests(NamedTuple):
-    """Requests of ``lengths`` tokens, one behind the other in a batch of ``rows`` rows; the rows behind the last
-    request belong to none. ``request_ids`` int32 ``[rows]``: each row's request, -1 for those; ``offsets`` int32
-    ``[requests + 1]``: each request's first row, and the row behind the last one's."""
-
+class _Requests(NamedTuple):
     lengths: tuple
     rows: int
     request_ids: torch.Tensor
+
+
+class PackedRequests(_Requests):
+    """Requests of ``lengths`` tokens, one behind the other in a batch of ``rows`` rows; the rows behind the last
+    request belong to none. ``request_ids`` int32 ``[rows]``: each row's request, -1 for those. Beside these three fields
+    ``offsets`` int32 ``[requests + 1]``, which packed texts need: each request's first row, and the row behind the last one's."""
+
     offsets: torch.Tensor | None = None
+
+    def __new__(cls, lengths: tuple, rows: int, request_ids: torch.Tensor, offsets: torch.Tensor | None = None):
+        self = super().__new__(cls, lengths, rows, request_ids)
+        self.offsets = offsets
+        return self
+
+    def _replace(self, **fields) -> "PackedRequests":
+        """A copy with other fields. Other ``lengths`` come without offsets unless theirs are given."""
+        offsets = fields.pop("offsets", None if "lengths" in fields else self.offsets)
+        made = super()._replace(**fields)
+        made.offsets = offsets
+        return made
 
     @classmethod
     def from_lengths(cls, lengths, rows: int | None = None, device="cuda") -> "PackedRequests":

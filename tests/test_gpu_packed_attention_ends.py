@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import text_ref as ref
+from test_gpu_packed_attention import BIAS, CROSS, _inputs, _score_size
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -139,3 +140,54 @@ def test_late_keys_that_dominate_within_the_held_maximum(pkg, dev, T, H, D):
         k[128:, :, 3] = 0.01 + 0.23 * i
         got = pkg.packed_cross_attention(q.to(dev), k.to(dev), v.to(dev), ref.offsets([T], dev), ref.offsets([m], dev), scale=1.0).cpu()
         assert torch.equal(got, v[:1].expand(T, H, D)), i
+
+
+@pytest.mark.parametrize("case", range(len(CROSS)))
+def test_cross_attention_gives_numbers(pkg, dev, case):
+    q_lens, k_lens, pad, heads, k_heads, D = CROSS[case]
+    q, k, v = _inputs(sum(q_lens) + pad, sum(k_lens) + 3, heads, k_heads, D, case)
+    k, v = k.clone(), v.clone()
+    k[sum(k_lens):], v[sum(k_lens):] = float("nan"), float("nan")  # nobody's keys
+    got = pkg.packed_cross_attention(q.to(dev), k.to(dev), v.to(dev), ref.offsets(q_lens, dev), ref.offsets(k_lens, dev))
+    want, size = ref.attention(q, k[: sum(k_lens)], v[: sum(k_lens)], q_lens, k_lens, D**-0.5)
+    _close(got, want, ref.attention_bound(size, want, _score_size(q, k[: sum(k_lens)], D**-0.5), D))
+
+
+@pytest.mark.parametrize("case", range(len(BIAS)))
+def test_relative_bias_gives_numbers(pkg, dev, case):
+    lens, pad, heads, D, buckets, far, both, dtype = BIAS[case]
+    g = torch.Generator().manual_seed(50 + case)
+    qkv = torch.randn(sum(lens) + pad, 3 * heads, D, generator=g)
+    qkv[:, :heads] *= D**-0.5
+    slab = qkv.to(BF16).to(dev)
+    table = (1.5 * torch.randn(buckets, heads, generator=g)).to(dtype)
+    got = pkg.relative_bias_attention(*(slab[:, i * heads : (i + 1) * heads] for i in range(3)), table.to(dev), ref.offsets(lens, dev), max_distance=far,
+                                      bidirectional=both)
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("T,H,D", [(30, 2, 64), (30, 4, 128), (500, 2, 64), (500, 40, 64), (500, 40, 128)])
+def test_wrong_offsets_touch_nothing_outside(pkg, dev, T, H, D):
+    """Descending, negative and too large offsets, with every tensor the middle of a larger one: what is around the inputs is NaN and never read,
+    what is around the output stays. (The kernel holds each offset inside its tensor.)"""
+    Tk = 90
+    g = torch.Generator().manual_seed(T)
+
+    def middle(rows, fill):
+        slab = torch.full((rows + 80, 3 * H, D), fill, dtype=BF16, device=dev)
+        return slab, slab[40 : rows + 40, H : 2 * H]
+
+    (_, q), (_, k), (_, v), (slab, out) = middle(T, float("nan")), middle(Tk, float("nan")), middle(Tk, float("nan")), middle(T, 7.0)
+    for t in (q, k, v):
+        t.copy_(torch.randn(t.shape, generator=g))
+    table = torch.randn(32, H, device=dev)
+    wrong = [([0, 400000, 20], [0, 90, 90]), ([T, 0, T], [90, 0, 50]), ([-5, 7, 2**31 - 1], [-(2**31), 2**31 - 1, 12]), ([0, 10, T], [80, 20, 500]),
+             ([0, T, T], [0, 2**31 - 1, 2**31 - 1])]
+    for qo, ko in wrong:
+        qo, ko = (torch.tensor(o, dtype=torch.int32, device=dev) for o in (qo, ko))
+        for call in (lambda: pkg.packed_cross_attention(q, k, v, qo, ko, out=out), lambda: pkg.relative_bias_attention(q, q, q, table, qo, out=out)):  # noqa: B023
+            out.fill_(7.0)
+            call()
+            assert torch.isfinite(out).all()
+            out.fill_(7.0)
+            assert bool((slab == 7).all())

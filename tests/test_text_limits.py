@@ -5,6 +5,7 @@ import ctypes
 import pathlib
 import subprocess
 
+from attention_forms import SHARED
 from fp8_tiles import TILES
 
 
@@ -27,10 +28,10 @@ def test_strides_of_attention_over_packed_rows(pkg):
     assert cross(k_hs=1 << 23) == 0 and cross(k_hs=1 << 40) == arg
 
 
-def _plans(tmp_path, body):
-    """What a program around ``fp8_plan.h`` prints, line by line."""
+def _plans(tmp_path, body, header="fp8_plan.h"):
+    """What a program around a header of rules prints, line by line."""
     root = pathlib.Path(__file__).resolve().parents[1]
-    (tmp_path / "main.cc").write_text('#include "fp8_plan.h"\n#include <cstdio>\nusing namespace wanmi;\n' + body)
+    (tmp_path / "main.cc").write_text(f'#include "{header}"\n#include <cstdio>\nusing namespace wanmi;\n' + body)
     subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-Wextra", "-Werror", f"-I{root / 'vllm-omni-neuron_amd' / 'csrc'}", str(tmp_path / "main.cc"), "-o",
                     str(tmp_path / "main")], check=True)
     return subprocess.run([str(tmp_path / "main")], check=True, capture_output=True, text=True, timeout=120).stdout.splitlines()
@@ -66,3 +67,16 @@ int main() {
 }
 """)
     assert 1.0 < float(out[0]) < 1.9 and float(out[1]) < 400e6
+
+
+def test_the_tiles_of_attention_over_packed_rows(tmp_path):
+    """Shared keys where every tile is on the chip at once and has more than 64 keys; one long request beside many short ones, short texts
+    and many requests take 128 rows a tile, whatever their average."""
+    shared = [(sum(q) + pad, sum(k), len(q), heads, D) for q, k, pad, heads, _, D in SHARED]
+    shared += [(1, 512, 1, 40, 128), (128, 2000, 1, 40, 128), (128, 2048, 4, 40, 128), (32, 16384, 32, 8, 64), (1024, 1024, 1, 12, 64), (100, 100, 1, 12, 64),
+               (270, 270, 3, 4, 128), (201, 201, 2, 8, 64)]
+    rows = [(3127, 65536, 128, 40, 128), (1063, 32768, 64, 40, 128), (531, 16384, 32, 64, 64), (1280, 32768, 64, 40, 128), (12, 12, 1, 64, 64), (16, 64, 1, 40, 128),
+            (1, 1, 1, 1, 64), (200, 512, 1, 40, 128), (32760, 1024, 2, 40, 128), (256, 8192, 16, 40, 128)]
+    lines = "".join(f'  printf("%d\\n", packed_keys_shared({T}, {Tk}, {R}, {H}, {D}));\n' for T, Tk, R, H, D in shared + rows)
+    got = _plans(tmp_path, "int main() {\n" + lines + "}\n", "packed_attention_plan.h")
+    assert got == ["1"] * len(shared) + ["0"] * len(rows)

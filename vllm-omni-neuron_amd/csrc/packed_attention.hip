@@ -27,6 +27,7 @@
 // What did not help (512 keys, 380 us): scores of a tile beside the softmax of the one before (443), workgroups that stay and load
 // ahead for their next tile of rows (448), three workgroups a CU with tiles of 32 keys (386), half of the first workgroups held back or wave
 // priorities (within 1%).
+#include "packed_attention_plan.h"
 #include "wanmi_common.h"
 
 #include <algorithm>
@@ -526,13 +527,7 @@ static int launch(PackedAttnArgs a, const BiasArgs& b, hipStream_t stream, const
 
 template <bool kBias, int D>
 static int dispatch(const PackedAttnArgs& a, const BiasArgs& b, hipStream_t stream, const char* what) {
-  // Tiles of 32 rows whose keys the waves share out, where a request has no more rows than that, so that tiles of 128 would leave three
-  // waves of four without rows; and where all of them are on the chip at once (one to a CU with its 144 KB of LDS, two at head_dim 64) and there is
-  // more than a tile of keys to share out. 40 heads x 128, us with shared keys against 128 rows: 128 rows of one request, 512 keys 9.7 / 12.9,
-  // 2000 keys 24 / 41, 40 keys 5.9 / 5.1; past one round 200 rows 17.3 / 13.1, 400 rows 25 / 13.4. 64 heads x 64: 200 rows of 512 keys
-  // 8.7 / 9.8, 400 rows 14.9 / 13.2. 12 heads x 64 with a bias: a prompt of 1024 tokens 12.9 / 20.8.
-  const int64_t small = (int64_t)(a.T / 32 + a.requests) * a.heads;
-  if (a.T <= (int64_t)32 * a.requests || (small <= (D == 128 ? 256 : 512) && a.Tk > (int64_t)64 * a.requests)) return launch<D, kBias, 4>(a, b, stream, what);
+  if (packed_keys_shared(a.T, a.Tk, a.requests, a.heads, D)) return launch<D, kBias, 4>(a, b, stream, what);
   return launch<D, kBias, 1>(a, b, stream, what);
 }
 

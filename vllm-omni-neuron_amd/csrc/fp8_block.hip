@@ -126,7 +126,8 @@ __global__ __launch_bounds__(256) void fp8_scales_kernel(const float* __restrict
 // ------------------------------------------------------------------------------------------------
 // Many rows: tiles of kTn features x kTm rows, both operands through LDS in stages of 128 along k. The matrix pipe and the chip's power bound the
 // 256 x 256 tiles: 32760 x 15360 x 5120 took 2912 us with the multiply-adds where the compiler put them, 2380 in the order below, 2322 without
-// bank conflicts, 2150 with workgroups that stay and addresses in scalar registers. A full round of 256 tiles costs 1.87 us a stage, one
+// bank conflicts, 2150 with workgroups that stay and addresses in scalar registers (16 to 23 of them wait in lanes of a vector register between tiles; the
+// stages' loop reads none of them back, in the 64 x 64 tiles one). A full round of 256 tiles costs 1.87 us a stage, one
 // of 122 tiles 1.25: cutting the last round's tiles in parts of their sums or in halves gained nothing. The smaller tiles are
 // bound by LDS (128 x 128: 96 KB read and 32 written a stage, 1024 of 1340 cycles) and the stage's barrier.
 // ------------------------------------------------------------------------------------------------

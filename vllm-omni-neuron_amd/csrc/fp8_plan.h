@@ -25,8 +25,8 @@ constexpr int64_t kFp8PlanCus = 256;
 //   64 x 64, four stages in LDS, two workgroups a CU: 0.37, 0.55, 0.86, 1.06, 1.34 with 1 to 5 workgroups on the fullest CU
 //   128 x 128, four stages, one workgroup a CU: 0.60 to 0.68 a round of 256
 //   128 x 128, two stages, two workgroups a CU: 0.73 up to 256 tiles, 1.01 at 320, 1.36 at 432, 1.64 at 520
-//   256 x 256, two stages, one workgroup a CU: 1.3 to 1.75 a round
-// So a CU gets through 40 to 55 KB/us of tiles whichever their size (its loads could do 125: reading LDS and a barrier a stage are what takes the time), and
+//   256 x 256, two stages, one workgroup a CU: 1.25 a round of 122 tiles, 1.87 a full one (the chip's power); 1.5 is counted for either
+// So a CU gets through 35 to 65 KB/us of tiles, most with two workgroups or more (its loads could do 125: reading LDS and a barrier a stage are what takes the time), and
 // what counts is how many bytes the fullest CU takes: small tiles and parts of the sum spread them, and read more. The parts are written and read once in fp32, at 6 TB/s, and a launch of 3.8 us adds them.
 // (5120 x 5120: 20 rows 17.6 -> 12.1 us with three parts, 200 rows 24.1 -> 20.6, 333 rows, 4112 deep, 23.9 -> 22.7 with two; 512 rows 27.9
 // and 38.6 with three: not taken. 13824 deep: 64 rows 41.2 -> 22.0, 200 rows 57.5 -> 34.1, 500 rows 67.1 -> 64.3.)

@@ -10,7 +10,7 @@
 //
 // A workgroup of four waves takes one head of one tile of a request's rows: 128 rows, 32 per wave, all waves over the same
 // keys (kSplit 1), or 32 rows with the keys shared out over the waves and their parts joined through LDS at the end
-// (kSplit 4: few rows per request). K and V pass through LDS in tiles of 64 (128) keys, loaded straight into it while the
+// (kSplit 4: few tiles of rows, over long texts). K and V pass through LDS in tiles of 64 (128) keys, loaded straight into it while the
 // tile before is computed. S^T = K Q^T puts a row's scores into one lane (and lane ^ 32), so that the softmax is lane-local, and
 // its P^T is the operand of O^T = V^T P^T as it stands. V stays [key][d] in LDS; its columns are read by the transposing LDS read
 // (ds_read_b64_tr_b16: 16 lanes read four keys x 16 d and get one d's four keys each).
@@ -18,15 +18,16 @@
 // The maximum m of a row is one that its running maximum may exceed by 2^8 before sums and outputs are rescaled: P then reaches
 // 2^8 instead of 1, which costs bf16 and fp32 no precision, and nearly every tile after the first goes without a rescale.
 //
-// What bounds it: with many rows, a SIMD's matrix pipe and its VALU one after the other. 32760 rows of 40 heads x 128 over 512 and fewer keys
-// (251 GFLOP, 687 MB) take 325 us (770 TFLOP/s): the matrix pipe is busy 39% of the cycles, the VALU 42%, LDS 24%, without bank conflicts. A score
-// of 64 lanes costs the VALU 18 cycles (2^x 8.4, the multiply-add before it 2.7, conversion, sum and maximum 2.3 each) beside 32
-// of MFMA at D = 128 and 16 at D = 64. 64 keys more cost 37 us there (1160 TFLOP/s), the rows themselves 105 (q and o, 671 MB); 1024 keys
-// reach 1000 TFLOP/s, at 64 heads x 64 with 2048 keys 880; prompts of 6001 tokens with a bias there (159 GFLOP) 202 us. With few rows it is the
-// chain of launch, offsets, the tiles that one CU loads, and join: 16 rows of 40 heads over 512 keys 9.3 us for 11 MB.
-// What did not help (512 keys, 380 us): scores of a tile beside the softmax of the one before (443), workgroups that stay and load
-// ahead for their next tile of rows (448), three workgroups a CU with tiles of 32 keys (386), half of the first workgroups held back or wave
-// priorities (within 1%).
+// What bounds it: with many rows, a SIMD's matrix pipe and its VALU, which here run one after the other more than beside one another. 32760 rows of 40 heads x
+// 128 over 512 and fewer keys (251 GFLOP, 687 MB) take 317 to 341 us (740 to 790 TFLOP/s): the matrix pipe is busy 39% of the cycles, the VALU 42%, LDS
+// 24% (6% of that on bank conflicts). A score of 64 lanes costs the VALU 18 cycles (2^x 8.4, the multiply-add before it 2.7, conversion, sum and maximum 2.3
+// each) beside 32 of MFMA at D = 128 and 16 at D = 64. 64 keys more cost 37 us there (1160 TFLOP/s), the rows themselves 92 (q and o, 671 MB); 1024 keys
+// reach 1000 TFLOP/s, 8192 rows of 64 heads x 64 over 2048 keys 930; prompts of 6001 tokens with a bias there (159 GFLOP) take 195 to 213 us. With few rows it
+// is the chain of launch, offsets, the tiles that one CU loads, and join: 16 rows of 40 heads over 512 keys 8.9 us for 11 MB.
+// The constant-max kernel of attention.hip reaches 1340 TFLOP/s on long sequences with the same products and exponentials: eight waves of 32 rows over a ring of four
+// tiles, loads of K and V apart, wave priorities by step. That scheme as a whole is not tried here. What did not help by itself (512 keys, 380 us): scores of a
+// tile beside the softmax of the one before (443), workgroups that stay and load ahead for their next tile of rows (448), three workgroups a CU with tiles
+// of 32 keys (386), half of the first workgroups held back or wave priorities (within 1%).
 #include "packed_attention_plan.h"
 #include "wanmi_common.h"
 

@@ -183,7 +183,9 @@ def relative_bias_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, t
 
     Half of a direction's buckets hold one distance each, the others grow by equal ratios up to ``max_distance``, and the last
     holds everything beyond. ``bidirectional``: the first half of the table is for keys at or before the query, the second for those
-    after it. Otherwise every bucket is for the keys before, and all later ones take bucket 0 (they are not masked).
+    after it. Otherwise every bucket is for the keys before, and all later ones take bucket 0 (they are not masked). A bias of minus
+    infinity leaves a key out, and a row that has no other is zeros; the lowest finite value of a type masks too, and a row of
+    nothing else weighs all its keys alike.
 
     Returns bf16 ``[T, heads, D]``. Rows behind the last prompt are zeros in an output allocated here and left as they are in a
     given ``out``, which may be ``q``. Inference only: no gradient.

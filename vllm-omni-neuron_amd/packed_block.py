@@ -18,7 +18,7 @@ low-rank adapters. A block is that of :mod:`.block` with each request's own
 
 The texts can be packed like the rows (:func:`project_packed_cross_kv`): the cross-attention of all requests is then one launch
 (:func:`.packed_cross_attention`) in place of one each, and so is the self-attention of requests that are not long: 16 requests of 16 tokens
-take 0.42 ms in place of 0.88, 8 of 390 1.27 and 1.56, 4 of 1560 2.13 and 2.17 (and their texts' keys and values 0.42 ms a
+take 0.41 ms in place of 0.88, 8 of 390 1.28 and 1.56, 4 of 1560 2.13 and 2.17 (and their texts' keys and values 0.43 ms a
 block in place of 0.77 for 16 texts of 512 tokens). A projection whose weight is an :class:`.FP8BlockWeight` runs as
 :func:`.fp8_block_linear` on bf16 rows in place of MX codes.
 
@@ -159,8 +159,8 @@ def project_packed_cross_kv(w: BlockWeights, context: torch.Tensor, text: Packed
 
 # With packed texts, self-attention too is one launch for all requests, as long as none has more rows than this: few rows then
 # share the chip instead of waiting for one another, while the constant-max kernel is the faster one on long rows. A block of dim 5120, all together
-# against one by one, us: 16 x 16 tokens 418 / 598, 64 x 16 1061 / 1757, 8 x 390 1267 / 1430, 4 x 1560 2128 / 2168, one of 1560 713 / 704,
-# 2 x 3600 2791 / 2805, 2 x 7800 6865 / 6374.
+# against one by one, us: 16 x 16 tokens 411 / 593, 64 x 16 1004 / 1729, 8 x 390 1265 / 1423, 4 x 1560 2108 / 2148, one of 1560 707 / 694,
+# 2 x 3600 2765 / 2778, 2 x 7800 6782 / 6275.
 _TOGETHER = 3600
 
 
@@ -266,7 +266,12 @@ def packed_dit_forward(blocks, h: torch.Tensor, temb: torch.Tensor, packed: Pack
     (:func:`.block.project_cross_kv` of the request's text), or per block a :class:`PackedCrossKV` of all requests' texts. Weights may be
     :class:`.FP8BlockWeight` in place of :class:`.MXWeight`, each for itself. ``adapters``: per block a :class:`BlockAdapters` (or None);
     ``adapter_ids`` int32 ``[R]``: the adapter of each request, -1 for none. Returns bf16 ``[rows, dim]``; rows of no request
-    are zeros. The norm before a block is formed with the sum at the end of the one before it."""
+    are zeros. The norm before a block is formed with the sum at the end of the one before it.
+
+    Captured into a graph, a replay follows adapter ids, adapters, positions and the offsets of packed texts that were changed in place. Other
+    row lengths need :class:`PackedCrossKV` in every block and no request above 3600 rows at the capture (each attention is then one launch, which
+    reads its lengths on the GPU), and ``request_ids``, ``offsets`` and positions changed together; otherwise the rows of a request are those
+    of ``packed.lengths`` at the capture."""
     rows, dim = h.shape
     count = len(packed.lengths)
     if rows != packed.rows or tuple(positions.shape) != (rows, 3):
